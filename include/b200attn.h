@@ -45,6 +45,8 @@ extern "C" {
 #define B200ATTN_STATUS_LEN_OVER_CAP     2  /* seq_len[b] > capacity: clamped to capacity */
 #define B200ATTN_STATUS_WAIT_TIMEOUT     4  /* a bounded wait on a copy barrier ran out */
 #define B200ATTN_STATUS_LEN_NEGATIVE     8  /* seq_len[b] < 0: treated as 0 */
+#define B200ATTN_STATUS_BAD_PAGE        32  /* paged cache: a page number the call needs is not in [0, n_pages): its tokens are skipped */
+#define B200ATTN_STATUS_BAD_POSITION    64  /* rotary: a position or axis outside the tables: clamped to them */
 #define B200ATTN_STATUS_BOUNDS          16  /* index-checking build only (-DB200ATTN_BOUNDS=1): a kernel computed an index
                                                outside its buffer (reported, never trapped) */
 
@@ -411,6 +413,108 @@ int b200attn_dequant_prefix(const B200AttnShape* shape, int n_tokens,
  */
 int b200attn_calibrate_scales(const B200AttnShape* shape, int n_tokens,
                               const void* x_bf16, float* scale, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The cache in pages (no counterpart in the reference, whose cache is one capacity-sized block per
+ * sequence, runner/model/static_cache.py:135-158).
+ *
+ *     k_pages / v_pages : u8  [n_layers][n_pages][h_kv][page_size][head_dim]   (e4m3fn bytes)
+ *     k_scale / v_scale : f32 [n_layers][n_pages][h_kv]       one scale per (layer, page, kv head)
+ *     page_table        : i32 [batch][max_pages]              page of tokens [i * page_size, (i+1) * page_size) of a sequence
+ *
+ * A value is float(byte) * scale.  The attention calls take any scale; the append makes powers of two (below).
+ * Table entries at or beyond a sequence's last token are never read.  A page that the append writes must
+ * belong to one sequence only; pages that are only read may be shared.  Queries and new keys / values of ragged
+ * batches are packed: sequence b owns rows [q_start[b], q_start[b + 1]) of the token dimension; rows from
+ * q_start[batch] on belong to nobody: they are neither read nor written.
+ */
+typedef struct B200AttnPagedShape {
+  int n_layers;
+  int batch;         /* sequences (rows of page_table), >= 1 */
+  int h_q;           /* query heads; a multiple of h_kv, group size <= 8 */
+  int h_kv;
+  int head_dim;      /* 128 or 256 */
+  int page_size;     /* tokens per page: 16, 32, 64 or 128 */
+  int n_pages;       /* pages of the pool */
+  int max_pages;     /* columns of page_table: max_pages * page_size is a sequence's capacity */
+  long long k_layer_stride;   /* bytes between layers, 0 = dense */
+  long long v_layer_stride;
+  int reserved;      /* must be 0 */
+  int reserved2;     /* must be 0 */
+} B200AttnPagedShape;
+
+/*
+ * Rotary embedding (rotate-half on the first rotary_dim dims).  Pair j (dims j and j + rotary_dim / 2) of a token turns
+ * by the angle of row pos of the tables, pos = positions[pair_axis[j]][token]: one axis for text, three (time, height,
+ * width) for images and video.  The tables hold cosines and sines in fp32, so that far positions lose nothing (an fp32
+ * angle does).
+ */
+typedef struct B200AttnRope {
+  const float* cos;        /* [n_positions][rotary_dim / 2] */
+  const float* sin;
+  const int* positions;    /* i32 [n_axes][n_tokens]; NULL: the token's slot in its sequence, n_axes must be 1 */
+  const int* pair_axis;    /* i32 [rotary_dim / 2], values in [0, n_axes); NULL: axis 0 for all */
+  int n_positions;
+  int n_axes;              /* 1..4 */
+  int rotary_dim;          /* 16 .. head_dim, a multiple of 16 */
+  int reserved;            /* must be 0 */
+} B200AttnRope;
+
+/*
+ * Rotate queries and keys and quantise-and-append keys and values to the pages, all layers in one launch.
+ *   q, q_out : bf16 [n_layers][n_tokens][h_q][head_dim]   (q_out may be q; both NULL: keys and values only)
+ *   k, v     : bf16 [n_layers][n_tokens][h_kv][head_dim]
+ *   q_start  : i32 [batch + 1] on the device; NULL: one token per sequence, n_tokens == batch
+ *   q_norm_weight, k_norm_weight : bf16 [n_layers][head_dim] or NULL: x * rsqrt(mean(x^2) + eps) * (1 + w) before the rotation
+ *   rope     : NULL = no rotation
+ *   seq_pos  : i32 [batch], tokens cached before the call; the new ones go to slots seq_pos[b], seq_pos[b] + 1, ...
+ *   advance_pos : 1 -> seq_pos[b] += the new tokens (if they all fit), after everything is written
+ * All arithmetic is fp32 with one rounding at the end, to bf16 for q_out, to e4m3 for the cache.  The scale of a (page, kv
+ * head) is the smallest power of two that brings the largest finite |value| of the page's new tokens to at most 448; where
+ * the page already held tokens it only ever grows, and the earlier rows are then re-expressed in it (a power of two: exact
+ * but for values that become subnormal).  Infinities saturate, NaN becomes the NaN byte.  A scale is never below 2^-126.
+ * Tokens beyond a sequence's capacity are skipped (B200ATTN_STATUS_POS_AT_CAPACITY).
+ */
+int b200attn_paged_rope_append(const B200AttnPagedShape* shape, const B200AttnRope* rope, int n_tokens, const int* q_start,
+                               const void* q_bf16, const void* k_bf16, const void* v_bf16,
+                               const void* q_norm_weight_bf16, const void* k_norm_weight_bf16, float eps,
+                               void* q_out_bf16,
+                               void* k_pages_u8, void* v_pages_u8, float* k_scale, float* v_scale,
+                               const int* page_table, int* seq_pos, int advance_pos,
+                               int* status, void* stream);
+
+/*
+ * Scratch of the two attention calls below: partial results of sequences that are split over several thread blocks,
+ * and one counter per split result.  q_tokens = 0: for b200attn_paged_decode; otherwise for b200attn_paged_prefill with up
+ * to q_tokens query rows.  Zero it once with b200attn_workspace_init; every launch leaves its counters at zero.  Launches
+ * that may overlap on the device need workspaces of their own.
+ */
+int b200attn_paged_workspace_bytes(const B200AttnPagedShape* shape, int q_tokens, int max_seq_len, size_t* bytes);
+
+/*
+ * Attention of one query token per sequence over token slots [0, seq_len[b] + seq_len_offset) of its pages.  A sequence
+ * without tokens gives zeros.
+ *   q, out      : bf16 [n_layers][batch][h_q][head_dim]
+ *   max_seq_len : an upper bound of the lengths that the host knows (0: the table's capacity); it decides how the work is
+ *                 split, not what is attended: longer sequences are attended in full all the same
+ */
+int b200attn_paged_decode(const B200AttnPagedShape* shape, const void* q_bf16,
+                          const void* k_pages_u8, const void* v_pages_u8, const float* k_scale, const float* v_scale,
+                          const int* page_table, const int* seq_len, int seq_len_offset, int max_seq_len,
+                          float softmax_scale, void* workspace, size_t workspace_bytes,
+                          void* out_bf16, int* status, void* stream);
+
+/*
+ * Attention of many query tokens per sequence: prompts, pieces of prompts on top of what is cached, a few guessed tokens.
+ * The queries of sequence b are its last tokens: with causal = 1, query i of n attends slots t <= seq_len[b] - n + i (none:
+ * its row is zero); with causal = 0 all seq_len[b] slots (cross attention to states of another length).
+ *   q, out  : bf16 [n_layers][n_tokens][h_q][head_dim], q_start i32 [batch + 1]
+ */
+int b200attn_paged_prefill(const B200AttnPagedShape* shape, int n_tokens, const void* q_bf16, const int* q_start,
+                           const void* k_pages_u8, const void* v_pages_u8, const float* k_scale, const float* v_scale,
+                           const int* page_table, const int* seq_len, int max_seq_len, int causal,
+                           float softmax_scale, void* workspace, size_t workspace_bytes,
+                           void* out_bf16, int* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,7 @@ c_void_p, c_int, c_float, c_size_t, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes
 OK = 0
 ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_WORKSPACE, ERR_SPLITS, ERR_CUDA, ERR_CAPACITY, ERR_VARIANT, ERR_TOO_LARGE = range(-1, -10, -1)
 STATUS_POS_AT_CAPACITY, STATUS_LEN_OVER_CAP, STATUS_WAIT_TIMEOUT, STATUS_LEN_NEGATIVE, STATUS_BOUNDS = 1, 2, 4, 8, 16
+STATUS_BAD_PAGE, STATUS_BAD_POSITION = 32, 64
 VARIANT_AUTO, VARIANT_SIMT, VARIANT_MMA, VARIANT_UMMA2 = 0, 1, 2, 4
 VARIANTS = {"auto": VARIANT_AUTO, "simt": VARIANT_SIMT, "mma": VARIANT_MMA, "umma2": VARIANT_UMMA2}
 SCALE_PER_HEAD, SCALE_PER_TOKEN = 0, 1
@@ -37,6 +38,19 @@ class B200AttnShape(ctypes.Structure):
 class B200AttnPeerOut(ctypes.Structure):
     _fields_ = [("n_peers", c_int), ("rank", c_int), ("h_q_total", c_int), ("mode", c_int),
                 ("out", c_void_p * 8), ("out_alt", c_void_p * 8), ("staging", c_void_p * 8), ("step", c_void_p)]
+
+
+class B200AttnPagedShape(ctypes.Structure):
+    _fields_ = [
+        ("n_layers", c_int), ("batch", c_int), ("h_q", c_int), ("h_kv", c_int), ("head_dim", c_int),
+        ("page_size", c_int), ("n_pages", c_int), ("max_pages", c_int),
+        ("k_layer_stride", c_ll), ("v_layer_stride", c_ll), ("reserved", c_int), ("reserved2", c_int),
+    ]
+
+
+class B200AttnRope(ctypes.Structure):
+    _fields_ = [("cos", c_void_p), ("sin", c_void_p), ("positions", c_void_p), ("pair_axis", c_void_p),
+                ("n_positions", c_int), ("n_axes", c_int), ("rotary_dim", c_int), ("reserved", c_int)]
 
 
 # name -> (restype, argtypes); every symbol include/b200attn.h declares
@@ -80,6 +94,15 @@ PROTOTYPES = {
     "b200attn_dequant_prefix": (c_int, [ctypes.POINTER(B200AttnShape), c_int, c_void_p, c_ll, c_void_p, c_void_p,
                                         c_void_p]),
     "b200attn_calibrate_scales": (c_int, [ctypes.POINTER(B200AttnShape), c_int, c_void_p, c_void_p, c_void_p]),
+    "b200attn_paged_rope_append": (c_int, [ctypes.POINTER(B200AttnPagedShape), ctypes.POINTER(B200AttnRope), c_int, c_void_p,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "b200attn_paged_workspace_bytes": (c_int, [ctypes.POINTER(B200AttnPagedShape), c_int, c_int, ctypes.POINTER(c_size_t)]),
+    "b200attn_paged_decode": (c_int, [ctypes.POINTER(B200AttnPagedShape), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
+    "b200attn_paged_prefill": (c_int, [ctypes.POINTER(B200AttnPagedShape), c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p,
+                                       c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,64 @@
+// The paged FP8 cache: resolved geometry, launch arguments and the small device helpers its kernels share.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200attn {
+
+struct PagedGeometry {
+  int n_layers, batch, h_q, h_kv, head_dim, page_size, n_pages, max_pages, group;
+  long long k_layer_stride, v_layer_stride;   // bytes, always filled in
+};
+
+struct PagedAppendArgs {
+  const B200AttnRope* rope;   // null = no rotation
+  int n_tokens;
+  const int* q_start;         // null = one token per sequence
+  const void *q, *k, *v, *wq, *wk;
+  float eps;
+  void* q_out;
+  void *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  const int* page_table;
+  int* seq_pos;
+  int advance_pos;
+  int* status;
+};
+cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a, cudaStream_t stream);
+
+struct PagedAttnArgs {
+  const void* q;
+  const void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  const int *page_table, *seq_len;
+  int seq_len_offset, max_seq_len;
+  float softmax_scale;
+  void* workspace;
+  size_t workspace_bytes;
+  void* out;
+  int* status;
+  // many query tokens per sequence
+  int n_tokens;
+  const int* q_start;
+  int causal;
+};
+size_t paged_decode_workspace_bytes(const PagedGeometry& g, int max_seq_len);
+cudaError_t launch_paged_decode(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream);
+size_t paged_prefill_workspace_bytes(const PagedGeometry& g, int n_tokens, int max_seq_len);
+cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream);
+
+// Valid length of a sequence: negative lengths count as 0, lengths beyond the table's capacity are clamped to it.
+__device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* status, bool report) {
+  const long long cap = (long long)g.max_pages * g.page_size;
+  if (raw < 0) {
+    if (report) atomicOr(status, B200ATTN_STATUS_LEN_NEGATIVE);
+    return 0;
+  }
+  if (raw > cap) {
+    if (report) atomicOr(status, B200ATTN_STATUS_LEN_OVER_CAP);
+    return (int)cap;
+  }
+  return raw;
+}
+
+}  // namespace b200attn

@@ -1,0 +1,344 @@
+"""The FP8 cache in pages: append with rotary positions on the way, attention of one or of many query tokens, and the
+container that hands out pages.
+
+The reference keeps one capacity-sized block per sequence (runner/model/static_cache.py:135-158); a batch of sequences of
+very different lengths wants pages instead, and a prompt wants to be appended and attended without a bf16 copy of the
+cache.  torch only owns memory and streams here; all arithmetic runs in libb200attn.so.
+
+Layouts (n_layers may be dropped for a single layer):
+    k_pages, v_pages uint8 / float8_e4m3fn [n_layers, n_pages, h_kv, page_size, head_dim], page_size 16, 32, 64 or 128
+    k_scale, v_scale fp32  [n_layers, n_pages, h_kv]                a value is byte * scale
+    page_table       int32 [batch, max_pages] on the device
+    q, out           bf16  [n_layers, n_tokens, h_q, head_dim]       decode: n_tokens = batch
+    k, v             bf16  [n_layers, n_tokens, h_kv, head_dim]
+    q_start          int32 [batch + 1] on the device: sequence b owns tokens [q_start[b], q_start[b + 1])
+    seq_len, seq_pos int32 [batch] on the device
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import B200AttnPagedShape, B200AttnRope, check
+
+_BYTE_TYPES = (torch.uint8, torch.float8_e4m3fn)
+
+
+def _need(device: torch.device, dtype, **tensors) -> None:
+    """Every given tensor: on `device`, contiguous, of type `dtype`."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != device or device.type != "cuda":
+            raise ValueError(f"{name} must be on the cache's CUDA device ({device}): there is no CPU path")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+
+class _on:
+    """The tensors' device, made current for the call if it is not; gives its current stream."""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device: torch.device):
+        self.device, self.guard = device, None
+
+    def __enter__(self) -> int:
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def make_paged_shape(h_q: int, k_pages, v_pages, k_scale, page_table) -> B200AttnPagedShape:
+    """Geometry from the cache handles.  A 5-d pool may be strided over layers (dim 0) only."""
+    if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
+        raise ValueError("k_pages and v_pages must have the same shape [n_layers, n_pages, h_kv, page_size, head_dim]")
+    n = 1 if k_pages.dim() == 4 else k_pages.shape[0]
+    n_pages, h_kv, page, d = k_pages.shape[-4:]
+    for c in (k_pages, v_pages):
+        if c.dtype not in _BYTE_TYPES:
+            raise ValueError("the cache must be uint8 / float8_e4m3fn")
+        if c.stride()[-4:] != (h_kv * page * d, page * d, d, 1):
+            raise ValueError("the cache must be dense within a layer")
+    if k_scale.numel() != n * n_pages * h_kv:
+        raise ValueError("scales must be [n_layers, n_pages, h_kv]")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [batch, max_pages]")
+    return B200AttnPagedShape(n, page_table.shape[0], h_q, h_kv, d, page, n_pages, page_table.shape[1],
+                              k_pages.stride(0) if n > 1 else 0, v_pages.stride(0) if n > 1 else 0, 0, 0)
+
+
+class PagedWorkspace:
+    """Scratch of the attention calls, allocated once (before any graph capture): for decode, or with `q_tokens` for prefill
+    calls of up to that many query tokens.  `max_seq_len`: an upper bound of the lengths (default: the table's capacity); it
+    decides how the work is split.  Launches that may overlap on the device need workspaces of their own."""
+
+    def __init__(self, shape: B200AttnPagedShape, device, *, max_seq_len: int | None = None, q_tokens: int | None = None):
+        self.max_seq_len = int(max_seq_len or 0)
+        self.q_tokens = int(q_tokens or 0)
+        out = ctypes.c_size_t(0)
+        with _on(torch.device(device)) as stream:
+            check(_lib.lib().b200attn_paged_workspace_bytes(ctypes.byref(shape), self.q_tokens, self.max_seq_len, ctypes.byref(out)),
+                  "b200attn_paged_workspace_bytes")
+            self.nbytes = max(256, out.value)
+            self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+            self.status = torch.zeros(1, dtype=torch.int32, device=device)
+            check(_lib.lib().b200attn_workspace_init(self.buf.data_ptr(), self.nbytes, stream), "b200attn_workspace_init")
+
+    def read_status(self) -> int:
+        """Device status bits (synchronises; not for use inside a captured step)."""
+        return int(self.status.item())
+
+
+def _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table):
+    dev = k_pages.device
+    _need(dev, torch.float32, k_scale=k_scale, v_scale=v_scale)
+    _need(dev, torch.int32, page_table=page_table)
+    if v_pages.device != dev or v_scale.numel() != k_scale.numel():
+        raise ValueError("k_pages / v_pages and k_scale / v_scale must match")
+    return dev
+
+
+def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, seq_pos, *, q_start=None,
+                      positions=None, pair_axis=None, q_norm_weight=None, k_norm_weight=None, eps: float = 1e-6,
+                      advance: bool = True, status: torch.Tensor, q_out: torch.Tensor | None = None):
+    """Rotate queries and keys and quantise-and-append keys and values to the pages, in one launch; returns the rotated
+    queries (None if `q` is None).
+
+    Without `q_start`: one token per sequence.  `cos`, `sin`: fp32 tables [n_positions, rotary_dim / 2] (None: no rotation);
+    a token's row is its slot in the sequence, or `positions` int32 [n_tokens] or [n_axes, n_tokens] with `pair_axis` int32
+    [rotary_dim / 2] saying which axis turns which pair.  Norm weights bf16 [n_layers, head_dim]: RMS norm with weight 1 + w
+    before the rotation.  `seq_pos`: tokens cached before the call, advanced afterwards if `advance`.  Capacity, bad pages
+    and bad positions are reported in `status`."""
+    h_kv, d = k_pages.shape[-3], k_pages.shape[-1]
+    h_q = q.shape[-2] if q is not None else h_kv
+    shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
+    dev = _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table)
+    _need(dev, torch.bfloat16, q=q, k=k, v=v, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, q_out=q_out)
+    _need(dev, torch.int32, seq_pos=seq_pos, q_start=q_start, positions=positions, pair_axis=pair_axis, status=status)
+    _need(dev, torch.float32, cos=cos, sin=sin)
+    n_layers = shape.n_layers
+    n_tokens = k.numel() // (n_layers * h_kv * d)
+    if k.numel() != n_layers * n_tokens * h_kv * d or k.shape[-2:] != (h_kv, d) or v.shape != k.shape:
+        raise ValueError("k and v must be [n_layers, n_tokens, h_kv, head_dim]")
+    if q is not None and (q.numel() != n_layers * n_tokens * h_q * d or q.shape[-1] != d):
+        raise ValueError("q must be [n_layers, n_tokens, h_q, head_dim]")
+    if seq_pos.numel() != shape.batch:
+        raise ValueError("seq_pos must be int32 [batch]")
+    if q_start is None and n_tokens != shape.batch:
+        raise ValueError("without q_start there is one token per sequence")
+    if q_start is not None and q_start.numel() != shape.batch + 1:
+        raise ValueError("q_start must be int32 [batch + 1]")
+    for w in (q_norm_weight, k_norm_weight):
+        if w is not None and w.numel() != n_layers * d:
+            raise ValueError("norm weights must be [n_layers, head_dim]")
+    rope = None
+    if cos is not None and cos.shape[-1] > 0:
+        if sin is None or cos.dim() != 2 or sin.shape != cos.shape:
+            raise ValueError("cos and sin must be [n_positions, rotary_dim / 2]")
+        n_axes = 1
+        if positions is not None:
+            n_axes = 1 if positions.dim() == 1 else positions.shape[0]
+            if positions.numel() != n_axes * n_tokens:
+                raise ValueError("positions must be [n_tokens] or [n_axes, n_tokens]")
+        if pair_axis is not None and pair_axis.numel() != cos.shape[-1]:
+            raise ValueError("pair_axis must be int32 [rotary_dim / 2]")
+        rope = B200AttnRope(cos.data_ptr(), sin.data_ptr(), positions.data_ptr() if positions is not None else None,
+                            pair_axis.data_ptr() if pair_axis is not None else None, cos.shape[0], n_axes, 2 * cos.shape[-1], 0)
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        elif q_out.numel() != q.numel():
+            raise ValueError("q_out must have q's shape")
+    if n_tokens == 0:
+        return q_out if q is not None else None
+    with _on(dev) as stream:
+        rc = _lib.lib().b200attn_paged_rope_append(
+            ctypes.byref(shape), ctypes.byref(rope) if rope is not None else None, n_tokens,
+            q_start.data_ptr() if q_start is not None else None, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
+            q_norm_weight.data_ptr() if q_norm_weight is not None else None,
+            k_norm_weight.data_ptr() if k_norm_weight is not None else None, eps, q_out.data_ptr() if q is not None else None,
+            k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
+            seq_pos.data_ptr(), int(advance), status.data_ptr(), stream)
+    check(rc, "b200attn_paged_rope_append")
+    return q_out if q is not None else None
+
+
+def paged_decode_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, seq_len, *, workspace: PagedWorkspace,
+                           softmax_scale: float | None = None, seq_len_offset: int = 0, out: torch.Tensor | None = None):
+    """Attention of one query token per sequence (q bf16 [n_layers, batch, h_q, head_dim]) over the first
+    seq_len[b] + seq_len_offset tokens of its pages; bf16 with q's shape.  A sequence without tokens gives zeros."""
+    h_q, d = q.shape[-2], q.shape[-1]
+    shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
+    dev = _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table)
+    _need(dev, torch.bfloat16, q=q, out=out)
+    _need(dev, torch.int32, seq_len=seq_len)
+    if d != shape.head_dim or q.numel() != shape.n_layers * shape.batch * h_q * d:
+        raise ValueError("q must be [n_layers, batch, h_q, head_dim]")
+    if seq_len.numel() != shape.batch:
+        raise ValueError("seq_len must be int32 [batch]")
+    if workspace.q_tokens or workspace.buf.device != dev:
+        raise ValueError("the workspace must be one for decode, on the cache's device")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.numel() != q.numel():
+        raise ValueError("out must have q's shape")
+    with _on(dev) as stream:
+        rc = _lib.lib().b200attn_paged_decode(
+            ctypes.byref(shape), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            page_table.data_ptr(), seq_len.data_ptr(), seq_len_offset, workspace.max_seq_len,
+            d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(), workspace.nbytes, out.data_ptr(),
+            workspace.status.data_ptr(), stream)
+    check(rc, "b200attn_paged_decode")
+    return out
+
+
+def paged_prefill_attention(q, q_start, k_pages, v_pages, k_scale, v_scale, page_table, seq_len, *, workspace: PagedWorkspace,
+                            causal: bool = True, softmax_scale: float | None = None, out: torch.Tensor | None = None):
+    """Attention of many query tokens per sequence (q bf16 [n_layers, n_tokens, h_q, head_dim], packed by `q_start`) over the
+    first seq_len[b] tokens of its pages.  causal: a sequence's queries are its last tokens, each sees those up to itself;
+    not causal: all (cross attention).  Rows that see nothing are zero; rows behind q_start[batch] are left as they were."""
+    h_q, d = q.shape[-2], q.shape[-1]
+    shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
+    dev = _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table)
+    _need(dev, torch.bfloat16, q=q, out=out)
+    _need(dev, torch.int32, seq_len=seq_len, q_start=q_start)
+    n_tokens = q.numel() // (shape.n_layers * h_q * d)
+    if d != shape.head_dim or q.numel() != shape.n_layers * n_tokens * h_q * d:
+        raise ValueError("q must be [n_layers, n_tokens, h_q, head_dim]")
+    if seq_len.numel() != shape.batch or q_start.numel() != shape.batch + 1:
+        raise ValueError("seq_len must be int32 [batch], q_start int32 [batch + 1]")
+    if workspace.q_tokens < n_tokens or workspace.buf.device != dev:
+        raise ValueError(f"the workspace must be one for {n_tokens} query tokens, on the cache's device")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.numel() != q.numel():
+        raise ValueError("out must have q's shape")
+    if n_tokens == 0:
+        return out
+    with _on(dev) as stream:
+        rc = _lib.lib().b200attn_paged_prefill(
+            ctypes.byref(shape), n_tokens, q.data_ptr(), q_start.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(), workspace.max_seq_len, int(causal),
+            d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(), workspace.nbytes, out.data_ptr(),
+            workspace.status.data_ptr(), stream)
+    check(rc, "b200attn_paged_prefill")
+    return out
+
+
+def rope_tables(n_positions: int, rotary_dim: int, base: float = 10000.0, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin fp32 [n_positions, rotary_dim / 2] of the angles pos * base^(-2 j / rotary_dim), computed in 64 bits."""
+    freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / max(rotary_dim, 1))
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return angle.cos().float().contiguous(), angle.sin().float().contiguous()
+
+
+class PagedFP8Cache:
+    """A pool of pages for `slots` sequences, all layers: storage, page table, positions, and which pages are free.
+
+    Pages are handed out on the host, ahead of the steps that need them (`reserve`); a decode step reads table and
+    positions on the device and can be captured into a CUDA graph and replayed as long as pages are reserved."""
+
+    def __init__(self, n_layers: int, slots: int, h_q: int, h_kv: int, head_dim: int, n_pages: int, max_pages: int,
+                 page_size: int = 64, device="cuda", max_prompt_tokens: int = 0):
+        self.n_layers, self.slots, self.h_q, self.h_kv, self.head_dim = n_layers, slots, h_q, h_kv, head_dim
+        self.n_pages, self.max_pages, self.page_size = n_pages, max_pages, page_size
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        pool = (n_layers, n_pages, h_kv, page_size, head_dim)
+        self.k_pages = torch.zeros(pool, dtype=torch.uint8, device=self.device)
+        self.v_pages = torch.zeros(pool, dtype=torch.uint8, device=self.device)
+        self.k_scale = torch.ones(n_layers, n_pages, h_kv, device=self.device)
+        self.v_scale = torch.ones(n_layers, n_pages, h_kv, device=self.device)
+        self.page_table = torch.full((slots, max_pages), -1, dtype=torch.int32, device=self.device)
+        self.seq_pos = torch.zeros(slots, dtype=torch.int32, device=self.device)
+        self.host_len = [0] * slots
+        self.pages: list[list[int]] = [[] for _ in range(slots)]
+        self.free = list(range(n_pages - 1, -1, -1))
+        self.shape = make_paged_shape(h_q, self.k_pages, self.v_pages, self.k_scale, self.page_table)
+        self.workspace = PagedWorkspace(self.shape, self.device)
+        self.prompt_workspace = None
+        if max_prompt_tokens:
+            self.prompt_workspace = PagedWorkspace(self.shape, self.device, q_tokens=max_prompt_tokens)
+
+    @property
+    def status(self) -> torch.Tensor:
+        return self.workspace.status
+
+    def read_status(self) -> int:
+        st = self.workspace.read_status()
+        return st | self.prompt_workspace.read_status() if self.prompt_workspace is not None else st
+
+    def reserve(self, slot: int, n_tokens: int) -> None:
+        """Pages for `n_tokens` more tokens of a sequence; refuses, and changes nothing, if the pool or the table has no room."""
+        need = -(-(self.host_len[slot] + n_tokens) // self.page_size)
+        more = need - len(self.pages[slot])
+        if need > self.max_pages:
+            raise ValueError(f"capacity {self.max_pages * self.page_size} exceeded: {self.host_len[slot]} cached + {n_tokens}")
+        if more > len(self.free):
+            raise ValueError(f"{more} pages needed, {len(self.free)} free")
+        if more > 0:
+            first = len(self.pages[slot])
+            self.pages[slot] += [self.free.pop() for _ in range(more)]
+            self.page_table[slot, first:need] = torch.tensor(self.pages[slot][first:], dtype=torch.int32).to(self.device)
+
+    def release(self, slot: int) -> None:
+        """The sequence's pages go back to the pool (stream order: launches that read them come before)."""
+        self.free += reversed(self.pages[slot])
+        self.pages[slot] = []
+        self.host_len[slot] = 0
+        self.page_table[slot].fill_(-1)
+        self.seq_pos[slot] = 0
+
+    def prefill(self, q, k, v, cos, sin, lens, *, out=None, causal: bool = True, **rope) -> torch.Tensor:
+        """New tokens of every sequence (lens[b] of them, 0 allowed; packed along the token dimension): rotated, appended and
+        attended.  Returns bf16 [n_layers, n_tokens, h_q, head_dim].  `rope`: further arguments of `paged_rope_append`."""
+        if len(lens) != self.slots or sum(lens) != q.shape[-3]:
+            raise ValueError("lens must give every sequence's share of the tokens")
+        if self.prompt_workspace is None or self.prompt_workspace.q_tokens < sum(lens):
+            raise ValueError(f"max_prompt_tokens is too small for {sum(lens)} tokens")
+        need = [-(-(a + n) // self.page_size) - len(p) for a, n, p in zip(self.host_len, lens, self.pages)]
+        if sum(max(x, 0) for x in need) > len(self.free):
+            raise ValueError(f"{sum(max(x, 0) for x in need)} pages needed, {len(self.free)} free")
+        for a, n in zip(self.host_len, lens):
+            if a + n > self.max_pages * self.page_size:
+                raise ValueError(f"capacity {self.max_pages * self.page_size} exceeded: {a} cached + {n}")
+        for b, n in enumerate(lens):
+            self.reserve(b, n)
+        starts = [0]
+        for n in lens:
+            starts.append(starts[-1] + n)
+        q_start = torch.tensor(starts, dtype=torch.int32).to(self.device)
+        qr = paged_rope_append(q, k, v, cos, sin, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
+                               self.seq_pos, q_start=q_start, advance=True, status=self.status, **rope)
+        self.host_len = [a + n for a, n in zip(self.host_len, lens)]
+        return paged_prefill_attention(qr, q_start, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
+                                       self.seq_pos, workspace=self.prompt_workspace, causal=causal, out=out)
+
+    def step(self, q, k, v, cos, sin, *, out=None, count: bool = True, **rope) -> torch.Tensor:
+        """One decode step of all slots: rotate, append, attend, advance (graph capturable; `reserve` first)."""
+        if count:
+            for b in range(self.slots):
+                if self.host_len[b] + 1 > len(self.pages[b]) * self.page_size:
+                    raise ValueError(f"slot {b}: no page reserved for token {self.host_len[b]}")
+        qr = paged_rope_append(q, k, v, cos, sin, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
+                               self.seq_pos, advance=True, status=self.status, **rope)
+        out = paged_decode_attention(qr, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table, self.seq_pos,
+                                     workspace=self.workspace, out=out)
+        if count:
+            self.host_len = [x + 1 for x in self.host_len]
+        return out
+
+
+__all__ = ["PagedFP8Cache", "PagedWorkspace", "make_paged_shape", "paged_decode_attention", "paged_prefill_attention",
+           "paged_rope_append", "rope_tables"]

@@ -1,0 +1,391 @@
+"""GPU tests of the paged FP8 cache against plain implementations in 64 bits (paged_ref.py)."""
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(40, 8, 128), (24, 4, 256), (8, 1, 128), (3, 3, 128), (7, 1, 256)]
+
+
+def _run_attention(pkg, dev, case, *, causal=None, qlens=None, seed=0, offset=0, hint=None, softmax_scale=None, table_edit=None):
+    """Decode (qlens None) or prefill of ragged sequences; compares every sequence with the 64-bit form."""
+    n_layers, (h_q, h_kv, d), page, lens = case
+    g = torch.Generator().manual_seed(seed)
+    width = max(1, max(-(-n // page) for n in lens)) + 2
+    n_pages = sum(-(-n // page) for n in lens) + 3
+    kb, vb, ks, vs = ref.random_cache(g, n_layers, n_pages, h_kv, page, d, pow2=seed % 2 == 0)
+    table = ref.random_table(g, lens, page, width, n_pages)
+    # slots behind the last token and pages of nobody: NaN bytes, NaN scales
+    nobody = sorted(set(range(n_pages)) - set(table[table >= 0].tolist()))
+    kb[:, nobody], vb[:, nobody], ks[:, nobody], vs[:, nobody] = 0x7F, 0xFF, float("nan"), float("inf")
+    for b, n in enumerate(lens):
+        if n % page:
+            kb[:, table[b, n // page], :, n % page:] = 0x7F
+            vb[:, table[b, n // page], :, n % page:] = 0xFF
+    n = sum(qlens) if qlens is not None else len(lens)
+    tail = 3 if qlens is not None else 0                    # rows behind the last sequence
+    q = torch.randn(n_layers, n + tail, h_q, d, generator=g).to(torch.bfloat16)
+    shape = pkg.make_paged_shape(h_q, kb, vb, ks, table)
+    ws = pkg.PagedWorkspace(shape, dev, max_seq_len=hint, q_tokens=None if qlens is None else n + tail)
+    up = [t.to(dev) for t in (kb, vb, ks, vs, table)]
+    out = torch.full_like(q, 7.0).to(dev)
+    seq_len = torch.tensor(lens, dtype=torch.int32, device=dev) - offset
+    if qlens is None:
+        for _ in range(2):                                  # the second launch finds the workspace as the first left it
+            got = pkg.paged_decode_attention(q.to(dev), *up, seq_len, workspace=ws, seq_len_offset=offset, out=out, softmax_scale=softmax_scale)
+    else:
+        starts = torch.tensor([sum(qlens[:i]) for i in range(len(qlens) + 1)], dtype=torch.int32, device=dev)
+        for _ in range(2):
+            got = pkg.paged_prefill_attention(q.to(dev), starts, *up, seq_len, workspace=ws, causal=causal, out=out, softmax_scale=softmax_scale)
+    torch.cuda.synchronize()
+    assert ws.read_status() == 0
+    got = got.cpu()
+    assert (got[:, n:] == 7.0).all(), "rows behind the last sequence were written"
+    at = 0
+    for b, length in enumerate(lens):
+        m = 1 if qlens is None else qlens[b]
+        for layer in range(n_layers):
+            want, big = ref.attention(q[layer, at:at + m], kb[layer], vb[layer], ks[layer], vs[layer], table[b], length, causal=bool(causal),
+                                      softmax_scale=softmax_scale)
+            ref.assert_attention(got[layer, at:at + m], want, big, (case, b, layer))
+        at += m
+    return got
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_decode_lengths(pkg, cuda_device, heads, page):
+    """Empty, one token, ends inside and at the end of pages and tiles, all in one batch."""
+    _run_attention(pkg, cuda_device, (1, heads, page, [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 300, 511, 1000]), seed=page)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_decode_layers_and_long(pkg, cuda_device, page):
+    _run_attention(pkg, cuda_device, (3, (10, 2, 128), page, [5000, 1, 2049]), seed=page + 1)
+
+
+def test_decode_length_hint_too_small_or_absent_and_offset(pkg, cuda_device):
+    for hint in (None, 1, 700, 5000):
+        _run_attention(pkg, cuda_device, (1, (5, 1, 128), 64, [3000, 64, 1]), seed=3, hint=hint, offset=1)
+    _run_attention(pkg, cuda_device, (1, (24, 4, 256), 32, [777, 5]), seed=4, softmax_scale=0.3)
+
+
+def test_decode_only_empty_sequences(pkg, cuda_device):
+    got = _run_attention(pkg, cuda_device, (2, (40, 8, 128), 64, [0, 0, 0]), seed=5)
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads", HEADS)
+def test_prefill_ragged(pkg, cuda_device, heads, causal):
+    """Whole prompts, chunks on a prefix, single tokens, no token at all, fewer cached tokens than queries, nothing cached."""
+    lens, qlens = [130, 300, 64, 5, 1, 20, 0, 257], [130, 40, 1, 0, 1, 33, 4, 129]
+    _run_attention(pkg, cuda_device, (1, heads, 64, lens), qlens=qlens, causal=causal, seed=11)
+
+
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_prefill_pages_and_layers(pkg, cuda_device, page):
+    _run_attention(pkg, cuda_device, (2, (10, 2, 128), page, [401, 33]), qlens=[77, 33], causal=True, seed=page)
+
+
+@pytest.mark.parametrize("heads", [(5, 1, 128), (7, 1, 256)])
+def test_prefill_few_rows_on_a_long_cache(pkg, cuda_device, heads):
+    _run_attention(pkg, cuda_device, (1, heads, 64, [6000, 4097]), qlens=[3, 5], causal=True, seed=21)
+
+
+def test_scores_far_from_zero_and_queries_of_any_size(pkg, cuda_device):
+    """One key far above the rest; queries beyond the range of f16 and below it; all-zero queries."""
+    g = torch.Generator().manual_seed(9)
+    h_q, h_kv, d, page = 8, 1, 128, 64
+    for size, scale in ((1e6, 1e-7), (1e-9, 1e8), (0.0, 1.0), (30.0, 0.1)):
+        kb, vb, ks, vs = ref.random_cache(g, 1, 5, h_kv, page, d)
+        q = (torch.randn(1, 4, h_q, d, generator=g) * size).to(torch.bfloat16)
+        table = torch.tensor([[4, 0, 2]], dtype=torch.int32)
+        up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+        shape = pkg.make_paged_shape(h_q, kb, vb, ks, table)
+        lens = torch.tensor([150], dtype=torch.int32, device=cuda_device)
+        want, big = ref.attention(q[0], kb[0], vb[0], ks[0], vs[0], table[0], 150, softmax_scale=scale)
+        out = pkg.paged_prefill_attention(q.to(cuda_device), torch.tensor([0, 4], dtype=torch.int32, device=cuda_device), *up, lens, causal=False,
+                                          softmax_scale=scale, workspace=pkg.PagedWorkspace(shape, cuda_device, q_tokens=4))
+        ref.assert_attention(out[0].cpu(), want, big, ("prefill", size))
+        out = pkg.paged_decode_attention(q[:, :1].contiguous().to(cuda_device), *up, lens, softmax_scale=scale,
+                                         workspace=pkg.PagedWorkspace(shape, cuda_device))
+        ref.assert_attention(out[0].cpu(), want[:1], big[:1], ("decode", size))
+
+
+def test_bad_page_numbers_are_reported_and_skipped(pkg, cuda_device):
+    """A page number outside the pool inside the valid length: the status says so, its tokens are not attended."""
+    g = torch.Generator().manual_seed(2)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 4, 1, 64, 128)
+    q = torch.randn(1, 1, 5, 128, generator=g).to(torch.bfloat16)
+    for bad in (-1, 4, 1 << 30):
+        table = torch.tensor([[2, bad, 1]], dtype=torch.int32)
+        up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+        shape = pkg.make_paged_shape(5, kb, vb, ks, table)
+        lens = torch.tensor([160], dtype=torch.int32, device=cuda_device)
+        # the same tokens without the hole: 64 of page 2, then 32 of page 1
+        want, big = ref.attention(q[0], kb[0], vb[0], ks[0], vs[0], torch.tensor([2, 1]), 96)
+        ws = pkg.PagedWorkspace(shape, cuda_device)
+        out = pkg.paged_decode_attention(q.to(cuda_device), *up, lens, workspace=ws)
+        ref.assert_attention(out[0].cpu(), want, big, "decode")
+        assert ws.read_status() == pkg._lib.STATUS_BAD_PAGE
+        ws = pkg.PagedWorkspace(shape, cuda_device, q_tokens=1)
+        out = pkg.paged_prefill_attention(q.to(cuda_device), torch.tensor([0, 1], dtype=torch.int32, device=cuda_device), *up, lens, workspace=ws)
+        ref.assert_attention(out[0].cpu(), want, big, "prefill")
+        assert ws.read_status() == pkg._lib.STATUS_BAD_PAGE
+
+
+def test_lengths_outside_the_table_are_reported(pkg, cuda_device):
+    g = torch.Generator().manual_seed(2)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 4, 1, 64, 128)
+    q = torch.randn(1, 2, 5, 128, generator=g).to(torch.bfloat16)
+    table = torch.tensor([[2, 1], [0, 3]], dtype=torch.int32)
+    up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+    ws = pkg.PagedWorkspace(pkg.make_paged_shape(5, kb, vb, ks, table), cuda_device)
+    out = pkg.paged_decode_attention(q.to(cuda_device), *up, torch.tensor([1000, -3], dtype=torch.int32, device=cuda_device), workspace=ws).cpu()
+    want, big = ref.attention(q[0, :1], kb[0], vb[0], ks[0], vs[0], table[0], 128)
+    ref.assert_attention(out[0, :1], want, big)
+    assert (out[0, 1] == 0).all()
+    assert ws.read_status() == pkg._lib.STATUS_LEN_OVER_CAP | pkg._lib.STATUS_LEN_NEGATIVE
+
+
+# ---------------------------------------------------------------------------------------------- append
+def _append_case(pkg, dev, heads, page, pos, qlens, *, rot, axes=1, norm=False, n_layers=1, seed=0, one=False, specials=False):
+    h_q, h_kv, d = heads
+    g = torch.Generator().manual_seed(seed)
+    batch, n = len(pos), sum(qlens)
+    width = max(-(-(p + m) // page) for p, m in zip(pos, qlens)) + 1
+    n_pages = sum(-(-(p + m) // page) for p, m in zip(pos, qlens)) + 2
+    kb, vb, ks, vs = ref.random_cache(g, n_layers, n_pages, h_kv, page, d)
+    table = ref.random_table(g, [p + m for p, m in zip(pos, qlens)], page, width, n_pages)
+    tail = 0 if one else 2
+    q = torch.randn(n_layers, n + tail, h_q, d, generator=g).to(torch.bfloat16)
+    k = torch.randn(n_layers, n + tail, h_kv, d, generator=g).to(torch.bfloat16)
+    v = (torch.randn(n_layers, n + tail, h_kv, d, generator=g) * torch.exp(3 * torch.randn(1, n + tail, h_kv, 1, generator=g))).to(torch.bfloat16)
+    if specials:
+        v[0, 0, 0, :4] = torch.tensor([float("inf"), -float("inf"), float("nan"), 1.0])
+        v[0, 1] = 0
+    qw = (0.1 * torch.randn(n_layers, d, generator=g)).to(torch.bfloat16) if norm else None
+    kw = (0.1 * torch.randn(n_layers, d, generator=g)).to(torch.bfloat16) if norm else None
+    slots = torch.tensor([p + i for p, m in zip(pos, qlens) for i in range(m)] + [0] * tail)
+    cos = sin = positions = pair_axis = None
+    at = slots[None]
+    if rot:
+        cos, sin = pkg.rope_tables(int(slots.max()) + 1, rot, device="cpu")
+        if axes > 1:
+            at = torch.stack([slots // (a + 1) for a in range(axes)])
+            positions = at.to(torch.int32)
+            pair_axis = torch.randint(0, axes, (rot // 2,), generator=g).to(torch.int32)
+    starts = torch.tensor([sum(qlens[:i]) for i in range(batch + 1)], dtype=torch.int32)
+    d_ = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    up = [d_(t) for t in (kb, vb, ks, vs, table)]
+    status, seq_pos = torch.zeros(1, dtype=torch.int32, device=dev), torch.tensor(pos, dtype=torch.int32, device=dev)
+    q_out = torch.full_like(q, 7.0).to(dev)
+    pkg.paged_rope_append(d_(q), d_(k), d_(v), d_(cos), d_(sin), *up, seq_pos, q_start=None if one else d_(starts), positions=d_(positions),
+                          pair_axis=d_(pair_axis), q_norm_weight=d_(qw), k_norm_weight=d_(kw), status=status, q_out=q_out)
+    torch.cuda.synchronize()
+    assert status.item() == 0 and seq_pos.cpu().tolist() == [p + m for p, m in zip(pos, qlens)]
+    q_out = q_out.cpu()
+    assert (q_out[:, n:] == 7.0).all(), "query rows behind the last sequence were written"
+    used = torch.zeros(n_pages, page, dtype=torch.bool)
+    for layer in range(n_layers):
+        want = ref.norm_rope(q[layer, :n], None if qw is None else qw[layer], cos, sin, at[:, :n], pair_axis)
+        # bf16: half a step 2^-8 of the value; fp32 arithmetic: a few 2^-24 of the row
+        assert ((q_out[layer, :n].double() - want).abs() <= want.abs() * 2.0 ** -8 + want.abs().amax(-1, keepdim=True) * 2.0 ** -20).all()
+        for which, x, pool, scale, got_b, got_s in (("k", k, kb, ks, up[0], up[2]), ("v", v, vb, vs, up[1], up[3])):
+            rows = x[layer, :n].double()
+            if which == "k":
+                rows = ref.norm_rope(k[layer, :n], None if kw is None else kw[layer], cos, sin, at[:, :n], pair_axis)
+            vals, sc = ref.values(pool[layer]), scale[layer].double().clone()
+            for b in range(batch):
+                ref.append_rows(rows[starts[b]:starts[b + 1]], vals, sc, table[b], page, pos[b])
+                used[[int(table[b, s // page]) for s in range(pos[b], pos[b] + qlens[b])], [s % page for s in range(pos[b], pos[b] + qlens[b])]] = True
+            got_v, got_sc = ref.values(got_b[layer].cpu()), got_s[layer].cpu().double()
+            assert torch.equal(got_sc, sc), which
+            if which == "v" or (not rot and not norm):       # no arithmetic before the rounding: the same numbers
+                assert torch.equal(torch.nan_to_num(got_v, 999.0), torch.nan_to_num(vals, 999.0)), which
+            else:                                            # fp32 arithmetic may sit on the other side of a rounding border
+                near = (got_v - vals).abs() <= vals.abs() * 2.0 ** -3 + 2.0 ** -9
+                assert near.all() and (got_v != vals).double().mean() < 1e-4
+    return up
+
+
+@pytest.mark.parametrize("heads,rot,axes,norm", [((40, 8, 128), 128, 1, False), ((24, 4, 256), 64, 3, True), ((5, 1, 128), 0, 1, True),
+                                                 ((8, 1, 256), 256, 2, False), ((3, 3, 128), 16, 4, True), ((10, 2, 128), 48, 1, False)])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_append_prompts(pkg, cuda_device, heads, rot, axes, norm, page):
+    pos, qlens = [0, 5, 63, 64, 0, 17, 130], [70, 1, 2, 129, 0, 300, 7]
+    _append_case(pkg, cuda_device, heads, page, pos, qlens, rot=rot, axes=axes, norm=norm, seed=page + rot, n_layers=2 if page == 32 else 1)
+
+
+@pytest.mark.parametrize("heads,rot,axes,norm", [((40, 8, 128), 128, 1, False), ((24, 4, 256), 64, 3, True), ((5, 1, 128), 0, 1, False)])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_append_one_token_each(pkg, cuda_device, heads, rot, axes, norm, page):
+    pos = [0, 1, 15, 16, 63, 64, 127, 128, 129, 1000]
+    _append_case(pkg, cuda_device, heads, page, pos, [1] * len(pos), rot=rot, axes=axes, norm=norm, seed=page, n_layers=3, one=True)
+    _append_case(pkg, cuda_device, heads, page, pos, [1] * len(pos), rot=rot, axes=axes, norm=norm, seed=page)
+
+
+@pytest.mark.parametrize("one", [True, False])
+def test_append_infinities_nan_and_zero_rows(pkg, cuda_device, one):
+    _append_case(pkg, cuda_device, (5, 1, 128), 64, [0, 0, 70], [1, 1, 1], rot=0, one=one, specials=True, seed=1)
+
+
+def test_token_by_token_equals_one_piece(pkg, cuda_device):
+    """A page's scale only grows, by powers of two: token by token the scales are those of the whole prompt, and the bytes too
+    but for values that became subnormal on the way (rounded again: at most one subnormal step, 2^-9 of the scale)."""
+    g = torch.Generator().manual_seed(5)
+    h_kv, d, page, n = 2, 128, 32, 75
+    k = (torch.randn(n, h_kv, d, generator=g) * torch.exp(1.5 * torch.randn(n, h_kv, 1, generator=g))).to(torch.bfloat16).to(cuda_device)
+    table = torch.tensor([[3, 0, 4]], dtype=torch.int32, device=cuda_device)
+    res = []
+    for pieces in ([n], [1] * n, [10, 1, 1, 40, 23]):
+        kp = torch.zeros(1, 5, h_kv, page, d, dtype=torch.uint8, device=cuda_device)
+        vp, ks = torch.zeros_like(kp), torch.full((1, 5, h_kv), 1e30, device=cuda_device)
+        vs, pos, status, at = ks.clone(), torch.zeros(1, dtype=torch.int32, device=cuda_device), torch.zeros(1, dtype=torch.int32, device=cuda_device), 0
+        for m in pieces:
+            part = k[at:at + m].contiguous()
+            pkg.paged_rope_append(None, part, part, None, None, kp, vp, ks, vs, table, pos, status=status,
+                                  q_start=None if m == 1 and at % 2 else torch.tensor([0, m], dtype=torch.int32, device=cuda_device))
+            at += m
+        assert status.item() == 0 and pos.item() == n
+        assert torch.equal(kp, vp) and torch.equal(ks, vs)
+        res.append((ref.values(kp[0].cpu()), ks[0].cpu()))
+    for vals, sc in res[1:]:
+        assert torch.equal(sc, res[0][1])
+        assert ((vals - res[0][0]).abs() <= 2.0 ** -9).all()
+
+
+def test_append_reports_capacity_pages_and_positions(pkg, cuda_device):
+    L = pkg._lib
+    dev, h_kv, d, page = cuda_device, 2, 128, 16
+
+    def call(pos, qlens, table, one=False, n_positions=64, positions=None):
+        kp = torch.full((1, 4, h_kv, page, d), 0x11, dtype=torch.uint8, device=dev)
+        vp, ks = kp.clone(), torch.ones(1, 4, h_kv, device=dev)
+        vs, status = ks.clone(), torch.zeros(1, dtype=torch.int32, device=dev)
+        seq_pos = torch.tensor(pos, dtype=torch.int32, device=dev)
+        n = sum(qlens)
+        x = torch.ones(n, h_kv, d, dtype=torch.bfloat16, device=dev)
+        cos, sin = pkg.rope_tables(n_positions, 128, device=dev)
+        starts = torch.tensor([sum(qlens[:i]) for i in range(len(qlens) + 1)], dtype=torch.int32, device=dev)
+        pkg.paged_rope_append(x, x, x, cos, sin, kp, vp, ks, vs, torch.tensor(table, dtype=torch.int32, device=dev), seq_pos, status=status,
+                              q_start=None if one else starts, positions=positions)
+        torch.cuda.synchronize()
+        return status.item(), seq_pos.cpu().tolist(), vp.cpu()
+
+    for one in (True, False):
+        st, pos, vp = call([32, 3], [1, 1], [[0, 1], [2, 3]], one=one)           # the first sequence is full
+        assert st == L.STATUS_POS_AT_CAPACITY and pos == [32, 4]
+        assert (vp[0, [0, 1, 3]] == 0x11).all() and (vp[0, 2, :, 3] != 0x11).all()
+        for bad in (-1, 4, 1 << 30):
+            st, pos, vp = call([16, 3], [1, 1], [[0, bad], [2, 3]], one=one)
+            assert st == L.STATUS_BAD_PAGE and (vp[0, [0, 1, 3]] == 0x11).all()
+        st, pos, vp = call([-1, 3], [1, 1], [[0, 1], [2, 3]], one=one)
+        assert st & ~L.STATUS_BAD_POSITION == (L.STATUS_POS_AT_CAPACITY if one else 0) and pos == [-1, 4] and (vp[0, [0, 1, 3]] == 0x11).all()
+    st, pos, vp = call([30], [5], [[1, 2]])                                       # two fit, three do not
+    assert st == L.STATUS_POS_AT_CAPACITY and pos == [30] and (vp[0, 2, :, 14:] != 0x11).all() and (vp[0, [0, 1, 3]] == 0x11).all()
+    far = torch.tensor([0, 64, -1], dtype=torch.int32, device=dev)
+    st, pos, vp = call([0], [3], [[1, 2]], positions=far)
+    assert st == L.STATUS_BAD_POSITION and pos == [3]
+
+
+# ---------------------------------------------------------------------------------------------- together
+def _dense_attention(q, k, v, causal_from):
+    """float64 attention of q [n, h_q, d] at positions causal_from.. over k, v [t, h_kv, d]."""
+    n, h_q, d = q.shape
+    rep = h_q // k.shape[1]
+    k, v = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+    a = torch.einsum("nhd,thd->hnt", q, k) * d ** -0.5
+    a = a.masked_fill(torch.arange(k.shape[0])[None, None, :] > (causal_from + torch.arange(n))[None, :, None], float("-inf"))
+    return torch.einsum("hnt,thd->nhd", torch.softmax(a, -1), v)
+
+
+def test_serving_run(pkg, cuda_device):
+    """Prompts, decode steps captured in a graph, a sequence that ends and its pages taken by another: the cache class against
+    64-bit attention over the bf16 keys and values.  The cache keeps 4 significant bits: a key or value is off by at most
+    2^-4 of itself; compared by cosine, which random errors of that size leave above 0.998."""
+    dev, layers, slots, h_q, h_kv, d, page = cuda_device, 2, 3, 10, 2, 128, 16
+    c = pkg.PagedFP8Cache(layers, slots, h_q, h_kv, d, n_pages=30, max_pages=12, page_size=page, device=dev, max_prompt_tokens=150)
+    cos, sin = pkg.rope_tables(256, 128, device=dev)
+    g = torch.Generator().manual_seed(0)
+    hist = [[torch.zeros(layers, 0, h_kv, d, dtype=torch.float64)] * 2 for _ in range(slots)]
+    mk = lambda n, h: torch.randn(layers, n, h, d, generator=g).to(torch.bfloat16)  # noqa: E731
+
+    def check(q, k, v, out, lens):
+        at = 0
+        for b, n in enumerate(lens):
+            if n == 0:
+                continue
+            before = hist[b][0].shape[1]
+            pos = torch.arange(before, before + n)[None]
+            for i, x in ((0, torch.stack([ref.norm_rope(k[l, at:at + n], None, cos.cpu(), sin.cpu(), pos, None) for l in range(layers)])),
+                         (1, v[:, at:at + n].double())):
+                hist[b][i] = torch.cat([hist[b][i], x], 1)
+            for l in range(layers):
+                qr = ref.norm_rope(q[l, at:at + n], None, cos.cpu(), sin.cpu(), pos, None)
+                want = _dense_attention(qr, hist[b][0][l], hist[b][1][l], before)
+                got = out[l, at:at + n].cpu().double()
+                assert torch.cosine_similarity(got.flatten(), want.flatten(), dim=0) > 0.998
+            at += n
+
+    def prompt(lens):
+        q, k, v = mk(sum(lens), h_q), mk(sum(lens), h_kv), mk(sum(lens), h_kv)
+        out = c.prefill(q.to(dev), k.to(dev), v.to(dev), cos, sin, lens)
+        check(q, k, v, out, lens)
+
+    prompt([50, 7, 90])
+    prompt([0, 20, 5])                                     # a second piece on top of the first
+    buf = [mk(slots, h).to(dev) for h in (h_q, h_kv, h_kv)]
+    out = torch.empty(layers, slots, h_q, d, dtype=torch.bfloat16, device=dev)
+    for b in range(slots):
+        c.reserve(b, 40)
+    step = lambda: c.step(*buf, cos, sin, out=out, count=False)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    pos0 = c.seq_pos.clone()
+    with torch.cuda.stream(s):
+        step()                                             # warm-up; its token is written again by the first replay
+    torch.cuda.current_stream().wait_stream(s)
+    c.seq_pos.copy_(pos0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(20):
+        q, k, v = mk(slots, h_q), mk(slots, h_kv), mk(slots, h_kv)
+        for t, x in zip(buf, (q, k, v)):
+            t.copy_(x)
+        graph.replay()
+        c.host_len = [x + 1 for x in c.host_len]
+        check(q, k, v, out, [1, 1, 1])
+    torch.cuda.synchronize()
+    assert c.seq_pos.cpu().tolist() == c.host_len and c.read_status() == 0
+    c.release(1)
+    hist[1] = [torch.zeros(layers, 0, h_kv, d, dtype=torch.float64)] * 2
+    prompt([1, 60, 0])                                     # another sequence in the freed slot, on used pages
+    assert c.read_status() == 0
+
+
+def test_other_stream_and_bits_stay_the_same(pkg, cuda_device):
+    """Calls on a side stream, twenty times: the same bits (partial results are joined in a fixed order)."""
+    g = torch.Generator().manual_seed(1)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 200, 2, 64, 128)
+    table = torch.randperm(200, generator=g).to(torch.int32).view(2, 100)
+    up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+    q = torch.randn(1, 2, 10, 128, generator=g).to(torch.bfloat16).to(cuda_device)
+    starts, lens = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda_device), torch.tensor([6400, 3333], dtype=torch.int32, device=cuda_device)
+    shape = pkg.make_paged_shape(10, kb, vb, ks, table)
+    wd, wp = pkg.PagedWorkspace(shape, cuda_device), pkg.PagedWorkspace(shape, cuda_device, q_tokens=2)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        a = [pkg.paged_decode_attention(q, *up, lens, workspace=wd) for _ in range(20)]
+        b = [pkg.paged_prefill_attention(q, starts, *up, lens, workspace=wp) for _ in range(20)]
+    s.synchronize()
+    assert all(torch.equal(x, a[0]) for x in a) and all(torch.equal(x, b[0]) for x in b)
+    for i, n in enumerate([6400, 3333]):
+        want, big = ref.attention(q[0, i:i + 1].cpu(), kb[0], vb[0], ks[0], vs[0], table[i], n)
+        ref.assert_attention(a[0][0, i:i + 1].cpu(), want, big)
+        ref.assert_attention(b[0][0, i:i + 1].cpu(), want, big)
