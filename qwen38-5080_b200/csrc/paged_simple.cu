@@ -99,10 +99,6 @@ cudaError_t launch_simple(const PagedGeometry& g, const PagedAttnArgs& a, int n_
 
 }  // namespace
 
-size_t paged_decode_workspace_bytes(const PagedGeometry&, int) { return 0; }
-cudaError_t launch_paged_decode(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
-  return launch_simple(g, a, g.batch, nullptr, stream);
-}
 size_t paged_prefill_workspace_bytes(const PagedGeometry&, int, int) { return 0; }
 cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
   return launch_simple(g, a, a.n_tokens, a.q_start, stream);
