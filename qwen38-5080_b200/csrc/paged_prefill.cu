@@ -42,7 +42,7 @@ struct PrefillParams {
   const uint8_t* v_pages;
   const float *k_scale, *v_scale;
   const int *page_table, *seq_len, *q_start;
-  int n_tokens, causal, tiles, splits;     // tiles: upper bound of the query tiles of one layer
+  int n_tokens, causal, page_shift, tiles, splits;     // tiles: upper bound of the query tiles of one layer
   float score_scale;
   float* part;                             // [query tiles * heads * layers][splits][128 * (D + 2)]
   int* counters;
@@ -123,7 +123,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 6];
-  __shared__ __align__(16) float s_ks[kInfo][8];            // K scale of each 16 keys of a tile; -1: no such page
+  // each 16 keys of a tile: K scale (-1: no such page), V scale, page (-1: none)
+  __shared__ __align__(16) float s_ks[kInfo][8], s_vs[kInfo][8];
+  __shared__ __align__(16) int s_id[kInfo][8];
   __shared__ float s_red[4];
   __shared__ float s_ml[2][2][kRows];
   __shared__ int s_info[8];                                 // [0] sequence [1] tile of it [2] gave up [3] tensor memory [4] last
@@ -205,41 +207,58 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
 
   float r_v = 0.f;                                          // largest V scale of the block's keys (V and softmax warps)
   if (warp == kTma) {
-    // ================= K tiles, and the K scales of their keys =================
+    // ================= K tiles; pages and scales of their keys =================
+    // Lane i < 8 looks after the tile's keys 16 i .. 16 i + 15.  A page's number and then its scales are two dependent loads, so
+    // they run ahead: pages by four tiles, scales by three; they are published two tiles ahead of the K copy (the V warps
+    // start from them).  A slot of the ring of kInfo tiles is free by then: K tile j is copied after S(j - KST), i.e. after the
+    // softmax of tile j - KST - 2 and the V units of tile j - KST - 2, and j - KST - 2 >= j + 2 - kInfo.
+    static_assert(kInfo >= KST + 4, "info ring");
     int issued = 0;
+    auto page_at = [&](int j) -> int {
+      const int key = (j0 + j) * kKeys + lane * 16;
+      return lane < 8 && j < nt && key < key_end ? __ldg(p.page_table + (long long)b * g.max_pages + (key >> p.page_shift)) : -2;   // -2: no key
+    };
+    auto scales_at = [&](int id) -> float2 {
+      if (id == -2) return make_float2(0.f, 0.f);
+      if (id < 0 || id >= g.n_pages) return make_float2(-1.f, 0.f);
+      const long long si = ((long long)layer * g.n_pages + id) * g.h_kv + h;
+      return make_float2(__ldg(p.k_scale + si), __ldg(p.v_scale + si));
+    };
+    auto publish = [&](int j, int id, float2 sc) {
+      if (j >= nt) return;
+      if (lane < 8) {
+        const bool bad = id != -2 && (id < 0 || id >= g.n_pages);
+        if (bad) atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
+        s_ks[j % kInfo][lane] = sc.x;
+        s_vs[j % kInfo][lane] = sc.y;
+        s_id[j % kInfo][lane] = bad ? -1 : id;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kinfo + 8 * (j % kInfo));
+    };
+    int id0 = page_at(0), id1 = page_at(1), id2 = page_at(2), id3 = page_at(3);
+    float2 sc0 = scales_at(id0), sc1 = scales_at(id1), sc2 = scales_at(id2);
+    publish(0, id0, sc0);
+    publish(1, id1, sc1);
     for (int j = 0; j < nt; ++j) {
       const int st = j % KST;
+      const int id4 = page_at(j + 4);
+      const float2 sc3 = scales_at(id3);
       if (j >= KST && !mbar_wait_lean(kempty + 8 * st, ((j / KST) - 1) & 1, gave_up, p.status)) break;
-      const int key = (j0 + j) * kKeys + lane * 16;
-      int id = -1;
-      bool box = false;
-      if (lane < 8) {
-        float ks = -1.f;
-        if (key < key_end) {
-          id = p.page_table[(long long)b * g.max_pages + key / g.page_size];
-          if (id < 0 || id >= g.n_pages) {
-            id = -1;
-            atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
-          } else {
-            ks = p.k_scale[((long long)layer * g.n_pages + id) * g.h_kv + h];
-          }
-        }
-        s_ks[j % kInfo][lane] = key < key_end ? ks : 0.f;
-        box = id >= 0 && key % g.page_size == 0;            // the lane of a page's first key copies the page
-      }
+      // the lane of a page's first key copies the page
+      const bool box = id0 >= 0 && id0 < g.n_pages && ((lane * 16) & (g.page_size - 1)) == 0;
       const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, box));
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(kinfo + 8 * (j % kInfo));
-        mbar_arrive_expect_tx(kfull + 8 * st, boxes * g.page_size * D);
-      }
+      if (lane == 0) mbar_arrive_expect_tx(kfull + 8 * st, boxes * g.page_size * D);
       __syncwarp();
       if (box) {
 #pragma unroll
         for (int hf = 0; hf < DH; ++hf)
-          tma_load_3d(sK + st * P::KTILE + hf * kKeys * 128 + lane * 16 * 128, &kmap, hf * 128, (id * g.h_kv + h) * g.page_size, layer, kfull + 8 * st);
+          tma_load_3d(sK + st * P::KTILE + hf * kKeys * 128 + lane * 16 * 128, &kmap, hf * 128, (id0 * g.h_kv + h) << p.page_shift, layer, kfull + 8 * st);
       }
       ++issued;
+      publish(j + 2, id2, sc2);
+      id0 = id1; id1 = id2; id2 = id3; id3 = id4;
+      sc2 = sc3;
     }
     if (lane == 0) s_info[5] = issued;
   } else if (warp == kMma) {
@@ -312,7 +331,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
       asm volatile("bar.sync 2, 128;" ::: "memory");
       r_v = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     }
-    const float inv_r = r_v > 0.f ? 1.f / r_v : 0.f;
+    const float inv_r = r_v > 0.f ? kVUp / r_v : 0.f;
     const uint8_t* vbase = p.v_pages + (long long)layer * g.v_layer_stride;
     // a lane's 16 bytes: chunk k of 64-dim block blk of row ro; the mapping makes 8 lanes hit all banks when they store
     const int k4 = lane & 3, blk = D == 128 ? (lane >> 3) & 1 : lane >> 3;
@@ -321,31 +340,26 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
     constexpr int N = P::UNIT_KEYS / STEP;                  // loads per lane and unit: 8
     const int units = nt * P::UNITS;
     uint4 raw[2][N];
-    uint32_t mul[2][N];                                     // f16x2 scale ratio, leading part (low) and remainder (high)
-    auto load = [&](int u, uint4 (&rw)[N], uint32_t (&ml)[N]) {
-      const int key0 = j0 * kKeys + u * P::UNIT_KEYS + ro;
+    auto load = [&](int u, uint4 (&rw)[N]) {
+      const int key0 = j0 * kKeys + u * P::UNIT_KEYS + ro, c0 = (u % P::UNITS) * (P::UNIT_KEYS / 16);
+      const int* ids = s_id[(u / P::UNITS) % kInfo];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int key = key0 + i * STEP;
+        const int key = key0 + i * STEP, id = ids[c0 + i * STEP / 16];
         rw[i] = make_uint4(0, 0, 0, 0);
-        ml[i] = 0;
-        if (key < key_end) {
-          const int id = __ldg(p.page_table + (long long)b * g.max_pages + key / g.page_size);
-          if (id >= 0 && id < g.n_pages) {
-            rw[i] = __ldg(reinterpret_cast<const uint4*>(vbase + (((long long)id * g.h_kv + h) * g.page_size + key % g.page_size) * D + blk * 64 + k4 * 16));
-            const float ratio = __ldg(p.v_scale + ((long long)layer * g.n_pages + id) * g.h_kv + h) * inv_r * kVUp;
-            const __half hi = __float2half_rn(ratio), lo = __float2half_rn(ratio - __half2float(hi));
-            ml[i] = (uint32_t)__half_as_ushort(hi) | ((uint32_t)__half_as_ushort(lo) << 16);
-          }
-        }
+        if (key < key_end && id >= 0)
+          rw[i] = __ldg(reinterpret_cast<const uint4*>(vbase + (((((long long)id * g.h_kv + h) << p.page_shift) + (key & (g.page_size - 1))) * D + blk * 64 + k4 * 16)));
       }
     };
-    auto store = [&](int st, const uint4 (&rw)[N], const uint32_t (&ml)[N]) {
+    auto store = [&](int u, int st, const uint4 (&rw)[N]) {
       const uint32_t base = sV + st * kUnitBytes + blk * (P::UNIT_KEYS * 128);
+      const float* vs = s_vs[(u / P::UNITS) % kInfo] + (u % P::UNITS) * (P::UNIT_KEYS / 16);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int row = ro + i * STEP;
-        const __half2 hi = __half2half2(__ushort_as_half((unsigned short)(ml[i] & 0xFFFFu))), lo = __half2half2(__ushort_as_half((unsigned short)(ml[i] >> 16)));
+        // the page's scale relative to the largest, as leading part + remainder
+        const float ratio = vs[i * STEP / 16] * inv_r;
+        const __half2 hi = __float2half2_rn(ratio), lo = __float2half2_rn(ratio - __low2float(hi));
         const uint32_t w[4] = {rw[i].x, rw[i].y, rw[i].z, rw[i].w};
         uint32_t o[8];
 #pragma unroll
@@ -360,20 +374,27 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
         sts128(rowaddr + (((2 * k4 + 1) ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
       }
     };
-    load(0, raw[0], mul[0]);
+    bool alive = mbar_wait_lean(kinfo, 0, gave_up, p.status);
+    if (alive) load(0, raw[0]);
 #pragma unroll 1
-    for (int u = 0; u < units; u += 2) {
+    for (int u = 0; u < units && alive; u += 2) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int uu = u + half;
-        if (uu < units) {
-          if (uu + 1 < units) load(uu + 1, raw[half ^ 1], mul[half ^ 1]);
+        if (uu < units && alive) {
+          if (uu + 1 < units) {
+            const int t = (uu + 1) / P::UNITS;
+            if ((uu + 1) % P::UNITS == 0) alive = mbar_wait_lean(kinfo + 8 * (t % kInfo), (t / kInfo) & 1, gave_up, p.status);
+            if (alive) load(uu + 1, raw[half ^ 1]);
+          }
           const int st = uu % kVRing;
-          if (uu >= kVRing && !mbar_wait_lean(vempty + 8 * st, ((uu / kVRing) - 1) & 1, gave_up, p.status)) { u = units; break; }
-          store(st, raw[half], mul[half]);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(vfull + 8 * st);
+          if (alive && uu >= kVRing) alive = mbar_wait_lean(vempty + 8 * st, ((uu / kVRing) - 1) & 1, gave_up, p.status);
+          if (alive) {
+            store(uu, st, raw[half]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(vfull + 8 * st);
+          }
         }
       }
     }
@@ -449,23 +470,25 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
       }
       const bool mask = !__all_sync(0xffffffffu, vis >= base + kKeys) || bad;
       const uint32_t ts = tmem + lane_base + (uint32_t)(j & 1) * 128u;
-      // ---- maximum ----
+      // ---- maximum: the next 32 scores are on their way while these are looked at ----
       float tmax = -INFINITY;
-      uint32_t s[32];
+      uint32_t s[2][32];
+      tmem_ld32(ts, s[0]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        tmem_ld32(ts + 32 * c, s);
-        tmem_wait32(s);
+        uint32_t (&x)[32] = s[c & 1];
+        tmem_wait32(x);
+        tmem_ld32(ts + 32 * ((c + 1) & 3), s[(c + 1) & 1]);   // after the last: the first again, for the exponentials
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           float mx = -INFINITY;
           if (!mask) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(s[16 * hh + i]));
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(x[16 * hh + i]));
           } else {
             const int n = a[2 * c + hh] < 0.f ? 0 : vis - base - 32 * c - 16 * hh;   // keys of these 16 that the row sees
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, i < n ? __uint_as_float(s[16 * hh + i]) : -INFINITY);
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, i < n ? __uint_as_float(x[16 * hh + i]) : -INFINITY);
           }
           tmax = fmaxf(tmax, mx == -INFINITY ? -INFINITY : mx * (rowmul * a[2 * c + hh]));
         }
@@ -486,19 +509,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
         const uint32_t to = tmem + lane_base + 256u + (uint32_t)grp * 128u;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
-          tmem_ld32(to + 32 * c, s);
-          tmem_wait32(s);
+          tmem_ld32(to + 32 * c, s[1]);
+          tmem_wait32(s[1]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * alpha);
-          tmem_st32_nowait(to + 32 * c, s);
+          for (int i = 0; i < 32; ++i) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * alpha);
+          tmem_st32_nowait(to + 32 * c, s[1]);
         }
       }
       // ---- probabilities, into the columns that the scores leave ----
       const float mb = (m == -INFINITY ? 0.f : m) - kBitsP;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        tmem_ld32(ts + 32 * c, s);
-        tmem_wait32(s);
+        uint32_t (&x)[32] = s[c & 1];
+        tmem_wait32(x);
+        if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
         uint32_t pk[16];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -507,7 +531,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
           float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float p0 = ex2(fmaf(__uint_as_float(s[16 * hh + i]), f, -mb)), p1 = ex2(fmaf(__uint_as_float(s[16 * hh + i + 1]), f, -mb));
+            float p0 = ex2(fmaf(__uint_as_float(x[16 * hh + i]), f, -mb)), p1 = ex2(fmaf(__uint_as_float(x[16 * hh + i + 1]), f, -mb));
             if (mask) {
               p0 = i < n ? p0 : 0.f;
               p1 = i + 1 < n ? p1 : 0.f;
@@ -690,6 +714,7 @@ cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a,
   p.page_table = a.page_table; p.seq_len = a.seq_len; p.q_start = a.q_start;
   p.n_tokens = a.n_tokens;
   p.causal = a.causal;
+  p.page_shift = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
   p.tiles = (int)prefill_tiles(g, a.n_tokens);
   p.splits = prefill_splits(g, a.n_tokens, a.max_seq_len);
   p.score_scale = a.softmax_scale * kLog2e;
