@@ -10,8 +10,7 @@
 //   * V is widened to f16 by four warps on its way from global to shared memory (exact; times the page's scale relative to
 //     the largest scale of the block's keys), because P needs more than 8 bits: P is f16 in tensor memory, in the columns
 //     that its scores left, and O += P V is kind::f16 with P as the tensor-memory operand.
-//   * softmax: one thread per row; scores are read twice from tensor memory (maximum, then exponentials), which keeps the
-//     registers few.  The reference maximum moves only when a tile exceeds it by 2^4, so O is rarely rescaled.
+//   * softmax: one thread per row, which takes its 128 scores into registers (the other warps give theirs up for it).  The reference maximum moves only when a tile exceeds it by 2^4, so O is rarely rescaled.
 //   * heads of 128: two groups of softmax warps take alternate tiles, each with its own maximum, sum and O, joined at the
 //     end; heads of 256: one group (O fills the tensor memory, and the products take twice as long per tile).
 // Tensor memory: S0 S1 at columns 0 and 128, O at 256 (two of 128 columns, or one of 256).
@@ -31,7 +30,7 @@ namespace {
 constexpr int kRows = 128;                 // query rows of a tile
 constexpr int kKeys = 128;                 // keys of a tile
 constexpr int kInfo = 8;                   // tiles whose scales are in flight
-constexpr int kVRing = 3;                  // V units of 32 KB in f16
+constexpr int kVRing = 2;                  // V units of 32 KB in f16
 constexpr int kUnitBytes = 32768;
 constexpr float kTauP = 4.f, kBitsP = 11.f;   // p <= 2^4, held times 2^11 in f16
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
@@ -39,7 +38,6 @@ constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 6
 struct PrefillParams {
   PagedGeometry g;
   const uint16_t* q;
-  const uint8_t* v_pages;
   const float *k_scale, *v_scale;
   const int *page_table, *seq_len, *q_start;
   int n_tokens, causal, page_shift, tiles, splits;     // tiles: upper bound of the query tiles of one layer
@@ -58,10 +56,41 @@ struct PrefillPlan {
   static constexpr int KTILE = kKeys * D;
   static constexpr int UNIT_KEYS = kUnitBytes / (2 * D);   // keys of a V unit
   static constexpr int UNITS = kKeys / UNIT_KEYS;          // V units of a tile
-  static constexpr int WARPS = 4 * NS + 4 + 2;             // softmax, V, TMA, MMA
+  static constexpr int RAW = D == 128 ? 3 : 2;             // V units in flight as bytes
+  static constexpr int RAW_BYTES = kUnitBytes / 2;
+  static constexpr int WARPS = 4 * NS + 8;                 // softmax, V, and a group of TMA, MMA and two idle warps
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int SMEM = 1024 + 2 * kRows * D + KST * KTILE + kVRing * kUnitBytes;
+  static constexpr int SMEM = 1024 + 2 * kRows * D + KST * KTILE + kVRing * kUnitBytes + RAW * RAW_BYTES;
+  // Registers per thread after the roles part: softmax keeps a row's 128 scores.  The shares add up to what the block
+  // is launched with (512 x 128; 384 x 168): 256 x 184 + 256 x 72; 128 x 232 + 256 x 136.
+  static constexpr int REGS_SOFTMAX = D == 128 ? 184 : 232;
+  static constexpr int REGS_OTHER = D == 128 ? 72 : 136;
 };
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pair2(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split2(unsigned long long p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -85,20 +114,58 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {  
       : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : B200_R32(r)::"memory"); }
+// A row's 128 scores (loads and the wait for them in one statement: the registers are not touched before it is over).
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
+      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
+      "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 64u) : "memory");
+}
+// Bounded wait without a call: functions that are called would have to fit the registers of the warps that gave theirs up.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*gave_up) return false;
+    if (global_timer_ns() - t0 > kWaitBudgetNs) {
+      *gave_up = 1;
+      atomicOr(status, B200ATTN_STATUS_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
 __device__ __forceinline__ void tmem_st16_nowait(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
-}
-__device__ __forceinline__ void tmem_st32_nowait(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -111,7 +178,7 @@ __device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t addr, uint32_t lbo)
 
 template <int D>
 __global__ void __launch_bounds__(PrefillPlan<D>::THREADS, 1)
-paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillParams p) {
+paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefillParams p) {
   using P = PrefillPlan<D>;
   constexpr int DH = P::DH, NS = P::NS, KST = P::KST;
   constexpr int kSoftmaxWarps = 4 * NS, kFirstV = kSoftmaxWarps, kTma = kSoftmaxWarps + 4, kMma = kSoftmaxWarps + 5;
@@ -122,19 +189,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
   const int G = g.group;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 6];
+  __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 2 * P::RAW + 6];
   // each 16 keys of a tile: K scale (-1: no such page), V scale, page (-1: none)
   __shared__ __align__(16) float s_ks[kInfo][8], s_vs[kInfo][8];
   __shared__ __align__(16) int s_id[kInfo][8];
   __shared__ float s_red[4];
-  __shared__ float s_ml[2][2][kRows];
-  __shared__ int s_info[8];                                 // [0] sequence [1] tile of it [2] gave up [3] tensor memory [4] last
+  __shared__ float s_ml[2][2][kRows], s_amax[2][kRows];
+  __shared__ int s_info[8];                                 // [0] sequence [1] tile of it, later V units issued [2] gave up [3] tensor memory [4] last
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sQ = smem0, sK = sQ + 2 * kRows * D, sV = sK + KST * P::KTILE;
+  const uint32_t sQ = smem0, sK = sQ + 2 * kRows * D, sV = sK + KST * P::KTILE, sRaw = sV + kVRing * kUnitBytes;
   const uint32_t qready = smem_u32(bars), kfull = qready + 8, kempty = kfull + 8 * KST, kinfo = kempty + 8 * KST;
   const uint32_t vfull = kinfo + 8 * kInfo, vempty = vfull + 8 * kVRing;
   const uint32_t sfull = vempty + 8 * kVRing, pfull = sfull + 16, odone = pfull + 16;
+  const uint32_t rfull = odone + 16, rempty = rfull + 8 * P::RAW;
   volatile int* gave_up = s_info + 2;
 
   // ---- which tile: piece fastest, then head, layer, query tile from the last (most keys) to the first ----
@@ -172,6 +240,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
     for (int i = 0; i < KST; ++i) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, 1); }
     for (int i = 0; i < kInfo; ++i) mbar_init(kinfo + 8 * i, 1);
     for (int i = 0; i < kVRing; ++i) { mbar_init(vfull + 8 * i, 4); mbar_init(vempty + 8 * i, 1); }
+    for (int i = 0; i < P::RAW; ++i) { mbar_init(rfull + 8 * i, 1); mbar_init(rempty + 8 * i, 4); }
     for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(odone + 8 * i, 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -206,6 +275,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
   const uint32_t tmem = (uint32_t)s_info[3];
 
   float r_v = 0.f;                                          // largest V scale of the block's keys (V and softmax warps)
+  if (warp >= kTma) regs_down<P::REGS_OTHER>();
   if (warp == kTma) {
     // ================= K tiles; pages and scales of their keys =================
     // Lane i < 8 looks after the tile's keys 16 i .. 16 i + 15.  A page's number and then its scales are two dependent loads, so
@@ -213,10 +283,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
     // start from them).  A slot of the ring of kInfo tiles is free by then: K tile j is copied after S(j - KST), i.e. after the
     // softmax of tile j - KST - 2 and the V units of tile j - KST - 2, and j - KST - 2 >= j + 2 - kInfo.
     static_assert(kInfo >= KST + 4, "info ring");
-    int issued = 0;
+    int issued = 0, vissued = 0;
+    bool ok = true;
     auto page_at = [&](int j) -> int {
       const int key = (j0 + j) * kKeys + lane * 16;
-      return lane < 8 && j < nt && key < key_end ? __ldg(p.page_table + (long long)b * g.max_pages + (key >> p.page_shift)) : -2;   // -2: no key
+      if (lane >= 8 || j >= nt || key >= key_end) return -2;   // no key
+      return max(-1, __ldg(p.page_table + (long long)b * g.max_pages + (key >> p.page_shift)));
     };
     auto scales_at = [&](int id) -> float2 {
       if (id == -2) return make_float2(0.f, 0.f);
@@ -236,40 +308,72 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
       __syncwarp();
       if (lane == 0) mbar_arrive(kinfo + 8 * (j % kInfo));
     };
-    int id0 = page_at(0), id1 = page_at(1), id2 = page_at(2), id3 = page_at(3);
+    int idp = -2, id0 = page_at(0), id1 = page_at(1), id2 = page_at(2), id3 = page_at(3);
     float2 sc0 = scales_at(id0), sc1 = scales_at(id1), sc2 = scales_at(id2);
     publish(0, id0, sc0);
     publish(1, id1, sc1);
-    for (int j = 0; j < nt; ++j) {
-      const int st = j % KST;
-      const int id4 = page_at(j + 4);
-      const float2 sc3 = scales_at(id3);
-      if (j >= KST && !mbar_wait_lean(kempty + 8 * st, ((j / KST) - 1) & 1, gave_up, p.status)) break;
-      // the lane of a page's first key copies the page
-      const bool box = id0 >= 0 && id0 < g.n_pages && ((lane * 16) & (g.page_size - 1)) == 0;
-      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, box));
-      if (lane == 0) mbar_arrive_expect_tx(kfull + 8 * st, boxes * g.page_size * D);
-      __syncwarp();
-      if (box) {
+    for (int j = 0; j <= nt && ok; ++j) {                   // K tile j, then V tile j - 1
+      int id4_ = -2;
+      float2 sc3_ = make_float2(0.f, 0.f);
+      if (j < nt) {
+        const int st = j % KST;
+        const int id4 = page_at(j + 4);
+        const float2 sc3 = scales_at(id3);
+        if (j >= KST) ok = wait_for(kempty + 8 * st, ((j / KST) - 1) & 1, gave_up, p.status);
+        __syncwarp();
+        if (!ok) break;
+        // the lane of a page's first key copies the page
+        const bool box = id0 >= 0 && id0 < g.n_pages && ((lane * 16) & (g.page_size - 1)) == 0;
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, box));
+        if (lane == 0) mbar_arrive_expect_tx(kfull + 8 * st, boxes * g.page_size * D);
+        __syncwarp();
+        if (box) {
 #pragma unroll
-        for (int hf = 0; hf < DH; ++hf)
-          tma_load_3d(sK + st * P::KTILE + hf * kKeys * 128 + lane * 16 * 128, &kmap, hf * 128, (id0 * g.h_kv + h) << p.page_shift, layer, kfull + 8 * st);
+          for (int hf = 0; hf < DH; ++hf)
+            tma_load_3d(sK + st * P::KTILE + hf * kKeys * 128 + lane * 16 * 128, &kmap, hf * 128, (id0 * g.h_kv + h) << p.page_shift, layer, kfull + 8 * st);
+        }
+        ++issued;
+        publish(j + 2, id2, sc2);
+        id4_ = id4; sc3_ = sc3;
       }
-      ++issued;
-      publish(j + 2, id2, sc2);
-      id0 = id1; id1 = id2; id2 = id3; id3 = id4;
-      sc2 = sc3;
+      if (j > 0) {
+        // V bytes, a unit at a time; a page of 128 keys makes two boxes where the unit has 64
+        constexpr int UL = P::UNIT_KEYS / 16;               // lanes of a unit
+        const int vrows = min(g.page_size, P::UNIT_KEYS);
+#pragma unroll 1
+        for (int u = 0; u < P::UNITS && ok; ++u) {
+          const int vs = vissued % P::RAW;
+          if (vissued >= P::RAW) ok = wait_for(rempty + 8 * vs, ((vissued / P::RAW) - 1) & 1, gave_up, p.status);
+          __syncwarp();
+          if (!ok) break;
+          const bool vbox = lane / UL == u && idp >= 0 && idp < g.n_pages && ((lane * 16) & (vrows - 1)) == 0;
+          const uint32_t vboxes = __popc(__ballot_sync(0xffffffffu, vbox));
+          if (lane == 0) mbar_arrive_expect_tx(rfull + 8 * vs, vboxes * vrows * D);
+          __syncwarp();
+          if (vbox) {
+            const int row = ((idp * g.h_kv + h) << p.page_shift) + ((lane * 16) & (g.page_size - 1));
+#pragma unroll
+            for (int hf = 0; hf < DH; ++hf)
+              tma_load_3d(sRaw + vs * P::RAW_BYTES + hf * P::UNIT_KEYS * 128 + (lane % UL) * 16 * 128, &vmap, hf * 128, row, layer, rfull + 8 * vs);
+          }
+          ++vissued;
+        }
+      }
+      idp = id0; id0 = id1; id1 = id2; id2 = id3; id3 = id4_;
+      sc2 = sc3_;
     }
-    if (lane == 0) s_info[5] = issued;
+    if (lane == 0) { s_info[5] = issued; s_info[1] = vissued; }
+    __syncwarp();
+    asm volatile("bar.arrive 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
   } else if (warp == kMma) {
     // ================= products =================
     int s_issued = 0, o_issued = 0;
-    bool ok = mbar_wait_lean(qready, 0, gave_up, p.status);
+    bool ok = wait_for(qready, 0, gave_up, p.status);
     const uint64_t descQ = smem_desc_k128(sQ), descK = smem_desc_k128(sK);
     const uint64_t descV = smem_desc_mn128(sV, P::UNIT_KEYS * 128);
     auto issue_s = [&](int j) {
       const int st = j % KST;
-      if (!mbar_wait_lean(kfull + 8 * st, (j / KST) & 1, gave_up, p.status)) return false;
+      if (!wait_for(kfull + 8 * st, (j / KST) & 1, gave_up, p.status)) return false;
       tc_fence_after();
       if (lane == 0) {
         const uint32_t d = tmem + (uint32_t)(j & 1) * 128u;
@@ -292,11 +396,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
     if (nt > 1) ok = ok && issue_s(1);
     int vu = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      ok = mbar_wait_lean(pfull + 8 * (j & 1), (j >> 1) & 1, gave_up, p.status);
+      ok = wait_for(pfull + 8 * (j & 1), (j >> 1) & 1, gave_up, p.status);
 #pragma unroll 1
       for (int u = 0; u < P::UNITS && ok; ++u, ++vu) {
         const int st = vu % kVRing;
-        ok = mbar_wait_lean(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
+        ok = wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
@@ -313,9 +417,28 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
       if (ok) ++o_issued;
       if (ok && j + 2 < nt) ok = issue_s(j + 2);
     }
-    if (lane == 0) { s_info[6] = s_issued; s_info[7] = o_issued; }
-  } else if (warp >= kFirstV) {
-    // ================= V: widened to f16 between global and shared memory =================
+    // every softmax warp has read its output, and the TMA warp has said what it issued
+    asm volatile("bar.sync 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
+    if (*gave_up && lane == 0) {
+      // A wait ran out: wait (bounded) for what was issued into this block's shared and tensor memory.
+      auto drain = [&](uint32_t bar, int ring, int n) {
+        for (int s = 0; s < ring && s < n; ++s) {
+          const int last = ((n - 1 - s) / ring) * ring + s;
+          const unsigned long long t0 = global_timer_ns();
+          while (!mbar_try_wait(bar + 8 * s, (last / ring) & 1) && global_timer_ns() - t0 < kWaitBudgetNs) {}
+        }
+      };
+      drain(kfull, KST, s_info[5]);
+      drain(rfull, P::RAW, s_info[1]);
+      drain(sfull, 2, s_issued);
+      drain(odone, 2, o_issued);
+    }
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  } else if (warp >= kFirstV && warp < kTma) {
+    // ================= V: bytes to f16, shared memory to shared memory =================
+    regs_down<P::REGS_OTHER>();
     const int vw = warp - kFirstV, vt = tid - kFirstV * 32;
     // the largest V scale of the block's keys
     {
@@ -332,104 +455,110 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
       r_v = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     }
     const float inv_r = r_v > 0.f ? kVUp / r_v : 0.f;
-    const uint8_t* vbase = p.v_pages + (long long)layer * g.v_layer_stride;
-    // a lane's 16 bytes: chunk k of 64-dim block blk of row ro; the mapping makes 8 lanes hit all banks when they store
-    const int k4 = lane & 3, blk = D == 128 ? (lane >> 3) & 1 : lane >> 3;
-    const int ro = ((lane >> 2) & 1) + (D == 128 ? (lane >> 4) * 2 : 0) + vw * (D == 128 ? 4 : 2);
-    constexpr int STEP = D == 128 ? 16 : 8;                 // rows of one load of the four warps
-    constexpr int N = P::UNIT_KEYS / STEP;                  // loads per lane and unit: 8
+    // A lane's 16 bytes: chunk k4 of 64-dim block blk of a row.  Eight lanes that go together take 4 chunks of rows q and q ^ 5 of
+    // an 8-row group: with both layouts swizzled (16-byte chunk index xor row) neither their loads nor their stores share a bank.
+    const int k4 = lane & 3, rb = (lane >> 2) & 1, blk = D == 128 ? (lane >> 3) & 1 : lane >> 3;
+    const int pr = D == 128 ? vw * 2 + (lane >> 4) : vw;    // row pair of the first step: pair 4 g + q = rows 8 g + q, 8 g + (q ^ 5)
+    const int row0 = (pr >> 2) * 8 + ((pr & 3) ^ (rb ? 5 : 0));
+    constexpr int STEP = D == 128 ? 16 : 8;                 // rows of one step of the four warps
+    constexpr int N = P::UNIT_KEYS / STEP;                  // steps of a unit: 8
+    const uint32_t src = sRaw + (D == 128 ? 0 : (blk >> 1) * (P::UNIT_KEYS * 128)) + row0 * 128 + ((((D == 128 ? blk : blk & 1) * 4 + k4) ^ (row0 & 7)) << 4);
+    const uint32_t dst = sV + blk * (P::UNIT_KEYS * 128) + row0 * 128;
+    const uint32_t dst0 = dst + (((2 * k4) ^ (row0 & 7)) << 4), dst1 = dst + (((2 * k4 + 1) ^ (row0 & 7)) << 4);
     const int units = nt * P::UNITS;
-    uint4 raw[2][N];
-    auto load = [&](int u, uint4 (&rw)[N]) {
-      const int key0 = j0 * kKeys + u * P::UNIT_KEYS + ro, c0 = (u % P::UNITS) * (P::UNIT_KEYS / 16);
-      const int* ids = s_id[(u / P::UNITS) % kInfo];
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int key = key0 + i * STEP, id = ids[c0 + i * STEP / 16];
-        rw[i] = make_uint4(0, 0, 0, 0);
-        if (key < key_end && id >= 0)
-          rw[i] = __ldg(reinterpret_cast<const uint4*>(vbase + (((((long long)id * g.h_kv + h) << p.page_shift) + (key & (g.page_size - 1))) * D + blk * 64 + k4 * 16)));
-      }
-    };
-    auto store = [&](int u, int st, const uint4 (&rw)[N]) {
-      const uint32_t base = sV + st * kUnitBytes + blk * (P::UNIT_KEYS * 128);
-      const float* vs = s_vs[(u / P::UNITS) % kInfo] + (u % P::UNITS) * (P::UNIT_KEYS / 16);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int row = ro + i * STEP;
-        // the page's scale relative to the largest, as leading part + remainder
-        const float ratio = vs[i * STEP / 16] * inv_r;
-        const __half2 hi = __float2half2_rn(ratio), lo = __float2half2_rn(ratio - __low2float(hi));
-        const uint32_t w[4] = {rw[i].x, rw[i].y, rw[i].z, rw[i].w};
-        uint32_t o[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t h2 = e4m3x2_to_f16x2((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
-          const __half2 x = *reinterpret_cast<const __half2*>(&h2);
-          const __half2 y = __hfma2(x, hi, __hmul2(x, lo));
-          o[e] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-        const uint32_t rowaddr = base + row * 128;
-        sts128(rowaddr + (((2 * k4) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
-        sts128(rowaddr + (((2 * k4 + 1) ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
-      }
-    };
-    bool alive = mbar_wait_lean(kinfo, 0, gave_up, p.status);
-    if (alive) load(0, raw[0]);
+    bool alive = true;
 #pragma unroll 1
-    for (int u = 0; u < units && alive; u += 2) {
+    for (int u = 0; u < units && alive; ++u) {
+      const int t = u / P::UNITS, rs = u % P::RAW, st = u % kVRing;
+      alive = wait_for(kinfo + 8 * (t % kInfo), (t / kInfo) & 1, gave_up, p.status);
+      if (alive) alive = wait_for(rfull + 8 * rs, (u / P::RAW) & 1, gave_up, p.status);
+      if (alive && u >= kVRing) alive = wait_for(vempty + 8 * st, ((u / kVRing) - 1) & 1, gave_up, p.status);
+      if (!alive) break;
+      const float* vs = s_vs[t % kInfo] + (u % P::UNITS) * (P::UNIT_KEYS / 16);
+      const int* ids = s_id[t % kInfo] + (u % P::UNITS) * (P::UNIT_KEYS / 16);
+      const int left = key_end - (j0 * kKeys + u * P::UNIT_KEYS);   // keys of the unit that exist
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int uu = u + half;
-        if (uu < units && alive) {
-          if (uu + 1 < units) {
-            const int t = (uu + 1) / P::UNITS;
-            if ((uu + 1) % P::UNITS == 0) alive = mbar_wait_lean(kinfo + 8 * (t % kInfo), (t / kInfo) & 1, gave_up, p.status);
-            if (alive) load(uu + 1, raw[half ^ 1]);
+      for (int i0 = 0; i0 < N; i0 += 4) {
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = lds128(src + rs * P::RAW_BYTES + (i0 + i) * STEP * 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = row0 + (i0 + i) * STEP, c = (i0 + i) * STEP / 16;
+          // the page's scale relative to the largest, as leading part + remainder; nothing behind the last key (bytes there may be
+          // NaN patterns) and nothing of a page that does not exist
+          const float ratio = vs[c] * inv_r;
+          const __half2 hi = __float2half2_rn(ratio), lo = __float2half2_rn(ratio - __low2float(hi));
+          const bool there = row < left && ids[c] >= 0, exact = __low2float(lo) == 0.f;   // exact: powers of two
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t h2 = e4m3x2_to_f16x2((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
+            const __half2 x = *reinterpret_cast<const __half2*>(&h2);
+            const __half2 y = exact ? __hmul2(x, hi) : __hfma2(x, hi, __hmul2(x, lo));
+            o[e] = there ? *reinterpret_cast<const uint32_t*>(&y) : 0u;
           }
-          const int st = uu % kVRing;
-          if (alive && uu >= kVRing) alive = mbar_wait_lean(vempty + 8 * st, ((uu / kVRing) - 1) & 1, gave_up, p.status);
-          if (alive) {
-            store(uu, st, raw[half]);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(vfull + 8 * st);
-          }
+          const uint32_t off = st * kUnitBytes + (i0 + i) * STEP * 128;
+          sts128(dst0 + off, o[0], o[1], o[2], o[3]);
+          sts128(dst1 + off, o[4], o[5], o[6], o[7]);
         }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(vfull + 8 * st);
+        mbar_arrive(rempty + 8 * rs);
       }
     }
-  } else {
+  } else if (warp < kSoftmaxWarps) {
     // ================= softmax: one thread per query row =================
     const int grp = warp >> 2, row = tid & 127;
     const int tok = row / G, head = row % G;
     const bool real = tok < ntok;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint16_t* qrow = p.q + (out_row0 + (long long)tok * g.h_q + head) * D;
-    // the query row as two e4m3 rows; with two groups each writes half of the row's dims
+    regs_up<P::REGS_SOFTMAX>();
+    // the query row as two e4m3 rows; with two groups each takes half of the row's dims
+    constexpr int NQ = 8, ROUNDS = D / 8 / NS / NQ;          // 16-byte loads at a time
     float rowmul;
     {
-      float amax = 0.f;
-      if (real)
-#pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(qrow) + i);
-          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      uint4 raw[NQ];
+      auto load_q = [&](int round) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xFFFF0000u))));
+        for (int i = 0; i < NQ; ++i)
+          raw[i] = real ? __ldg(reinterpret_cast<const uint4*>(qrow) + (grp * ROUNDS + round) * NQ + i) : make_uint4(0, 0, 0, 0);
+      };
+      float amax = 0.f;
+#pragma unroll
+      for (int round = 0; round < ROUNDS; ++round) {
+        load_q(round);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) amax = max3(amax, fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xFFFF0000u)));
         }
+      }
+      if (NS == 2) {
+        s_amax[grp][row] = amax;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        amax = fmaxf(s_amax[0][row], s_amax[1][row]);
+      }
       int ex = (int)((__float_as_uint(amax) >> 23) & 0xFF);
       ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
       const float down = __uint_as_float((uint32_t)(261 - ex) << 23), up = __uint_as_float((uint32_t)(ex - 7) << 23);   // largest |q| in [128, 256)
       rowmul = up * p.score_scale;
-#pragma unroll 2
-      for (int c = grp * (D / 16 / NS); c < (grp + 1) * (D / 16 / NS); ++c) {   // 16 dims
+#pragma unroll 1
+      for (int round = 0; round < ROUNDS; ++round) {
+      if (ROUNDS > 1) load_q(round);                        // again, from the caches
+#pragma unroll
+      for (int ci = 0; ci < NQ / 2; ++ci) {                 // 16 dims
+        const int c = (grp * ROUNDS + round) * (NQ / 2) + ci;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint4 w4 = make_uint4(0, 0, 0, 0);
-          if (real) w4 = __ldg(reinterpret_cast<const uint4*>(qrow) + 2 * c + i);
-          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+          const uint32_t w[4] = {raw[2 * ci + i].x, raw[2 * ci + i].y, raw[2 * ci + i].z, raw[2 * ci + i].w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float x0 = __uint_as_float(w[2 * e] << 16) * down, x1 = __uint_as_float(w[2 * e] & 0xFFFF0000u) * down;
@@ -443,6 +572,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
         sts128(sQ + off, hi[0], hi[1], hi[2], hi[3]);
         sts128(sQ + DH * kRows * 128 + off, lo[0], lo[1], lo[2], lo[3]);
       }
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(qready);
@@ -454,44 +584,46 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
     bool alive = true;
     for (int j = grp; j < nt && alive; j += NS) {
       const int base = (j0 + j) * kKeys;
-      alive = mbar_wait_lean(kinfo + 8 * (j % kInfo), (j / kInfo) & 1, gave_up, p.status);
-      if (alive) alive = mbar_wait_lean(sfull + 8 * (j & 1), (j >> 1) & 1, gave_up, p.status);
+      alive = wait_for(kinfo + 8 * (j % kInfo), (j / kInfo) & 1, gave_up, p.status);
+      if (alive) alive = wait_for(sfull + 8 * (j & 1), (j >> 1) & 1, gave_up, p.status);
+      __syncwarp();
       if (!alive) break;
       tc_fence_after();
-      float a[8];
+      const uint32_t ts = tmem + lane_base + (uint32_t)(j & 1) * 128u;
+      uint32_t s[128];
+      tmem_ld128(ts, s);
+      float f[8];                                           // score multipliers of 16 keys each
       bool bad = false;
       {
         const float4 x = *reinterpret_cast<const float4*>(s_ks[j % kInfo]), y = *reinterpret_cast<const float4*>(s_ks[j % kInfo] + 4);
-        a[0] = x.x; a[1] = x.y; a[2] = x.z; a[3] = x.w; a[4] = y.x; a[5] = y.y; a[6] = y.z; a[7] = y.w;
+        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          bad |= a[c] < 0.f;
-        }
+        for (int c = 0; c < 8; ++c) bad |= f[c] < 0.f;
       }
       const bool mask = !__all_sync(0xffffffffu, vis >= base + kKeys) || bad;
-      const uint32_t ts = tmem + lane_base + (uint32_t)(j & 1) * 128u;
-      // ---- maximum: the next 32 scores are on their way while these are looked at ----
-      float tmax = -INFINITY;
-      uint32_t s[2][32];
-      tmem_ld32(ts, s[0]);
+      if (mask) {                                           // bytes behind the last key may be anything, NaN patterns included
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t (&x)[32] = s[c & 1];
-        tmem_wait32(x);
-        tmem_ld32(ts + 32 * ((c + 1) & 3), s[(c + 1) & 1]);   // after the last: the first again, for the exponentials
+        for (int c = 0; c < 8; ++c) {
+          const int n = f[c] < 0.f ? 0 : vis - base - 16 * c;   // keys of these 16 that the row sees
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          float mx = -INFINITY;
-          if (!mask) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(x[16 * hh + i]));
-          } else {
-            const int n = a[2 * c + hh] < 0.f ? 0 : vis - base - 32 * c - 16 * hh;   // keys of these 16 that the row sees
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, i < n ? __uint_as_float(x[16 * hh + i]) : -INFINITY);
-          }
-          tmax = fmaxf(tmax, mx == -INFINITY ? -INFINITY : mx * (rowmul * a[2 * c + hh]));
+          for (int i = 0; i < 16; ++i)
+            if (i >= n) s[16 * c + i] = 0xFF800000u;
         }
+      }
+      // ---- maximum ----
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        f[c] = fmaxf(f[c] * rowmul, 1e-37f);                // never 0: a hidden score times its multiplier stays -inf
+        const uint32_t* x = s + 16 * c;
+        float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
+#pragma unroll
+        for (int i = 2; i < 14; i += 4) {
+          m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+        }
+        m0 = max3(m0, __uint_as_float(x[14]), __uint_as_float(x[15]));
+        tmax = fmaxf(tmax, fmaxf(m0, m1) * f[c]);
       }
       // ---- the reference moves when a tile exceeds it by more than kTauP ----
       float alpha = 1.f;
@@ -502,48 +634,46 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
       }
       if (j >= NS && __any_sync(0xffffffffu, alpha != 1.f)) {
         if (NS == 1) {                                      // the product of the tile before (two groups: complete, since these scores are)
-          alive = mbar_wait_lean(odone + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1, gave_up, p.status);
+          alive = wait_for(odone + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1, gave_up, p.status);
           if (!alive) break;
           tc_fence_after();
         }
         const uint32_t to = tmem + lane_base + 256u + (uint32_t)grp * 128u;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          tmem_ld32(to + 32 * c, s[1]);
-          tmem_wait32(s[1]);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t x[16];
+          tmem_ld16(to + 16 * c, x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * alpha);
-          tmem_st32_nowait(to + 32 * c, s[1]);
+          for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+          tmem_st16_nowait(to + 16 * c, x);
         }
       }
       // ---- probabilities, into the columns that the scores leave ----
-      const float mb = (m == -INFINITY ? 0.f : m) - kBitsP;
+      const float mb = kBitsP - (m == -INFINITY ? 0.f : m);
+      const unsigned long long mb2 = pair2(mb, mb);
+      unsigned long long sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t (&x)[32] = s[c & 1];
-        tmem_wait32(x);
-        if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
         uint32_t pk[16];
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const float f = rowmul * a[2 * c + hh];
-          const int n = !mask ? 16 : a[2 * c + hh] < 0.f ? 0 : vis - base - 32 * c - 16 * hh;
-          float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float p0 = ex2(fmaf(__uint_as_float(x[16 * hh + i]), f, -mb)), p1 = ex2(fmaf(__uint_as_float(x[16 * hh + i + 1]), f, -mb));
-            if (mask) {
-              p0 = i < n ? p0 : 0.f;
-              p1 = i + 1 < n ? p1 : 0.f;
-            }
-            sum0 += p0;
-            sum1 += p1;
-            const __half2 h2 = __floats2half2_rn(p0, p1);
-            pk[8 * hh + i / 2] = *reinterpret_cast<const uint32_t*>(&h2);
-          }
-          l += sum0 + sum1;
+        for (int i = 0; i < 32; i += 4) {
+          const unsigned long long f2 = pair2(f[2 * c + (i >> 4)], f[2 * c + (i >> 4)]);
+          float x0, x1, x2, x3;
+          split2(fma2(pair2(__uint_as_float(s[32 * c + i]), __uint_as_float(s[32 * c + i + 1])), f2, mb2), x0, x1);
+          split2(fma2(pair2(__uint_as_float(s[32 * c + i + 2]), __uint_as_float(s[32 * c + i + 3])), f2, mb2), x2, x3);
+          x0 = ex2(x0); x1 = ex2(x1); x2 = ex2(x2); x3 = ex2(x3);
+          sum0 = add2(sum0, pair2(x0, x1));
+          sum1 = add2(sum1, pair2(x2, x3));
+          const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
+          pk[i / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+          pk[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
         tmem_st16_nowait(ts + 16 * c, pk);
+      }
+      {
+        float x, y;
+        split2(add2(sum0, sum1), x, y);
+        l += x + y;
       }
       tmem_wait_st();
       tc_fence_before();
@@ -555,7 +685,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
     const int mine = (nt - grp + NS - 1) / NS;              // tiles of this group
     if (alive && mine > 0) {
       const int jl = grp + (mine - 1) * NS;
-      alive = mbar_wait_lean(odone + 8 * (jl & 1), (jl >> 1) & 1, gave_up, p.status);
+      alive = wait_for(odone + 8 * (jl & 1), (jl >> 1) & 1, gave_up, p.status);
       tc_fence_after();
     }
     if (NS == 2) {
@@ -617,59 +747,40 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const PrefillPara
         part[kRows * D + kRows + row] = L;
       }
     }
-  }
+    tc_fence_before();
+    asm volatile("bar.arrive 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
+    if (pieces == 1) return;
 
-  tc_fence_before();
-  __syncthreads();
-  if (warp == kMma) {
-    if (*gave_up && lane == 0) {
-      // A wait ran out: wait (bounded) for what was issued into this block's shared and tensor memory.
-      auto drain = [&](uint32_t bar, int ring, int issued) {
-        for (int s = 0; s < ring && s < issued; ++s) {
-          const int last = ((issued - 1 - s) / ring) * ring + s;
-          const unsigned long long t0 = global_timer_ns();
-          while (!mbar_try_wait(bar + 8 * s, (last / ring) & 1) && global_timer_ns() - t0 < kWaitBudgetNs) {}
-        }
-      };
-      drain(kfull, KST, s_info[5]);
-      drain(sfull, 2, s_info[6]);
-      drain(odone, 2, s_info[7]);
-    }
-    __syncwarp();
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
-  }
-  if (pieces == 1) return;
-
-  // ---- the last piece to be finished joins all of them ----
-  const long long tile_id = blockIdx.x / p.splits;
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) s_info[4] = atomicAdd(p.counters + tile_id, 1) == pieces - 1;
-  __syncthreads();
-  if (!s_info[4]) return;
-  __threadfence();
-  if (tid == 0) p.counters[tile_id] = 0;
-  const float* part = p.part + tile_id * p.splits * (kRows * (D + 2));
-  constexpr long long stride = kRows * (D + 2);
-  for (int i = tid; i < ntok * G * (D / 4); i += P::THREADS) {
-    const int row = i / (D / 4);
-    float M = -INFINITY, L = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    // ---- the last piece to be finished joins all of them ----
+    const long long tile_id = blockIdx.x / p.splits;
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+    if (tid == 0) s_info[4] = atomicAdd(p.counters + tile_id, 1) == pieces - 1;
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+    if (!s_info[4]) return;
+    __threadfence();
+    if (tid == 0) p.counters[tile_id] = 0;
+    constexpr long long stride = kRows * (D + 2);
+    const float* all = p.part + tile_id * p.splits * stride;
+    for (int i = tid; i < ntok * G * (D / 4); i += kSoftmaxWarps * 32) {
+      const int r = i / (D / 4);
+      float Mx = -INFINITY, Ls = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = 0; s < pieces; ++s) M = fmaxf(M, __ldcg(part + s * stride + kRows * D + row));
+      for (int s = 0; s < pieces; ++s) Mx = fmaxf(Mx, __ldcg(all + s * stride + kRows * D + r));
 #pragma unroll 4
-    for (int s = 0; s < pieces; ++s) {
-      const float ms = __ldcg(part + s * stride + kRows * D + row);
-      const float f = ms == -INFINITY ? 0.f : ex2(ms - M);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(part + s * stride) + i);
-      L += __ldcg(part + s * stride + kRows * D + kRows + row) * f;
-      a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
+      for (int s = 0; s < pieces; ++s) {
+        const float ms = __ldcg(all + s * stride + kRows * D + r);
+        const float w = ms == -INFINITY ? 0.f : ex2(ms - Mx);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(all + s * stride) + i);
+        Ls += __ldcg(all + s * stride + kRows * D + kRows + r) * w;
+        acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
+      }
+      const float inv = Ls > 0.f ? 1.f / Ls : 0.f;
+      const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+      reinterpret_cast<uint2*>(p.out + (out_row0 + (long long)(r / G) * g.h_q + r % G) * D)[i % (D / 4)] =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-    reinterpret_cast<uint2*>(p.out + (out_row0 + (long long)(row / G) * g.h_q + row % G) * D)[i % (D / 4)] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
 }
 
@@ -704,12 +815,14 @@ size_t paged_prefill_workspace_bytes(const PagedGeometry& g, int n_tokens, int m
 cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
   Geometry cache{};
   cache.n_layers = g.n_layers; cache.batch = g.n_pages; cache.h_kv = g.h_kv; cache.capacity = g.page_size; cache.head_dim = g.head_dim;
-  CUtensorMap kmap;
-  if (!encode_cache_map(&kmap, a.k_pages, cache, g.k_layer_stride, g.page_size)) return cudaErrorInvalidValue;
+  CUtensorMap kmap, vmap;
+  const int unit_keys = g.head_dim == 128 ? PrefillPlan<128>::UNIT_KEYS : PrefillPlan<256>::UNIT_KEYS;
+  if (!encode_cache_map(&kmap, a.k_pages, cache, g.k_layer_stride, g.page_size) ||
+      !encode_cache_map(&vmap, a.v_pages, cache, g.v_layer_stride, g.page_size < unit_keys ? g.page_size : unit_keys))
+    return cudaErrorInvalidValue;
   PrefillParams p{};
   p.g = g;
   p.q = (const uint16_t*)a.q;
-  p.v_pages = (const uint8_t*)a.v_pages;
   p.k_scale = a.k_scale; p.v_scale = a.v_scale;
   p.page_table = a.page_table; p.seq_len = a.seq_len; p.q_start = a.q_start;
   p.n_tokens = a.n_tokens;
@@ -727,7 +840,7 @@ cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a,
   auto launch = [&](auto kernel, int threads, int smem) -> cudaError_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)grid, threads, smem, stream>>>(kmap, p);
+    kernel<<<(unsigned)grid, threads, smem, stream>>>(kmap, vmap, p);
     return cudaGetLastError();
   };
   return g.head_dim == 128 ? launch(paged_prefill_kernel<128>, PrefillPlan<128>::THREADS, PrefillPlan<128>::SMEM)
