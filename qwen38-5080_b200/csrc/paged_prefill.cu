@@ -40,7 +40,7 @@ struct PrefillParams {
   const uint16_t* q;
   const float *k_scale, *v_scale;
   const int *page_table, *seq_len, *q_start;
-  int n_tokens, causal, page_shift, tiles, splits;     // tiles: upper bound of the query tiles of one layer
+  int n_tokens, causal, page_shift, pair, tiles, splits;   // pair: a block takes two query tiles; tiles: upper bound of the query tiles of one layer
   float score_scale;
   float* part;                             // [query tiles * heads * layers][splits][128 * (D + 2)]
   int* counters;
@@ -56,11 +56,12 @@ struct PrefillPlan {
   static constexpr int KTILE = kKeys * D;
   static constexpr int UNIT_KEYS = kUnitBytes / (2 * D);   // keys of a V unit
   static constexpr int UNITS = kKeys / UNIT_KEYS;          // V units of a tile
-  static constexpr int RAW = D == 128 ? 3 : 2;             // V units in flight as bytes
+  static constexpr int RAW = 2;                            // V units in flight as bytes
+  static constexpr int QTILE = 2 * kRows * D;              // a query tile as two e4m3 terms
   static constexpr int RAW_BYTES = kUnitBytes / 2;
   static constexpr int WARPS = 4 * NS + 8;                 // softmax, V, and a group of TMA, MMA and two idle warps
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int SMEM = 1024 + 2 * kRows * D + KST * KTILE + kVRing * kUnitBytes + RAW * RAW_BYTES;
+  static constexpr int SMEM = 1024 + NS * QTILE + KST * KTILE + kVRing * kUnitBytes + RAW * RAW_BYTES;
   // Registers per thread after the roles part: softmax keeps a row's 128 scores.  The shares add up to what the block
   // is launched with (512 x 128; 384 x 168): 256 x 184 + 256 x 72; 128 x 232 + 256 x 136.
   static constexpr int REGS_SOFTMAX = D == 128 ? 184 : 232;
@@ -92,11 +93,28 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of the warp, as the compiler knows it: what it issues stays in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// Shared-memory operand descriptor from its low word: address / 16, and the leading offset / 16 in the upper half.  8-row groups
+// 1024 bytes apart, 128-byte swizzle, sm_100 descriptor version 1 (smem_desc_k128 with the words apart).
+__device__ __forceinline__ uint64_t desc_of(uint32_t low) {
+  return ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32) | low;
+}
+__device__ __forceinline__ void umma_s(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {   // e4m3 x e4m3
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d), "l"(desc_of(a)), "l"(desc_of(b)), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_o(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {   // f16 (tensor memory) x f16
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+      ::"r"(d), "r"(a), "l"(desc_of(b)), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
 #define B200_R32(r) \
   "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), \
@@ -171,11 +189,6 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// MN-major operand, 128-byte swizzle: rows (keys) of 128 bytes, 8-row groups 1024 bytes apart, the next 64 f16 dims `lbo` bytes on.
-__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-
 template <int D>
 __global__ void __launch_bounds__(PrefillPlan<D>::THREADS, 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefillParams p) {
@@ -198,7 +211,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   __shared__ int s_info[8];                                 // [0] sequence [1] tile of it, later V units issued [2] gave up [3] tensor memory [4] last
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sQ = smem0, sK = sQ + 2 * kRows * D, sV = sK + KST * P::KTILE, sRaw = sV + kVRing * kUnitBytes;
+  const uint32_t sQ = smem0, sK = sQ + NS * P::QTILE, sV = sK + KST * P::KTILE, sRaw = sV + kVRing * kUnitBytes;
   const uint32_t qready = smem_u32(bars), kfull = qready + 8, kempty = kfull + 8 * KST, kinfo = kempty + 8 * KST;
   const uint32_t vfull = kinfo + 8 * kInfo, vempty = vfull + 8 * kVRing;
   const uint32_t sfull = vempty + 8 * kVRing, pfull = sfull + 16, odone = pfull + 16;
@@ -211,7 +224,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int h = rest % g.h_kv;
   rest /= g.h_kv;
   const int layer = rest % g.n_layers, number = p.tiles - 1 - rest / g.n_layers;
-  const int per_tile = kRows / G;                           // query tokens of a tile
+  const int per_tile = kRows / G, per_block = per_tile << p.pair;   // query tokens of a tile, of a block
   if (warp == 0) {
     int before = 0;
     if (lane == 0) s_info[0] = -1;
@@ -221,7 +234,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       int n = 0;
       if (b < g.batch) {
         const int q0 = p.q_start[b], nq = p.q_start[b + 1] - q0;
-        if (nq > 0 && q0 >= 0 && q0 + nq <= p.n_tokens) n = (nq + per_tile - 1) / per_tile;
+        if (nq > 0 && q0 >= 0 && q0 + nq <= p.n_tokens) n = (nq + per_block - 1) / per_block;
       }
       int inc = n;
 #pragma unroll
@@ -250,7 +263,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int b = s_info[0];
   if (b < 0) return;                                        // the grid is an upper bound
   const int q0 = p.q_start[b], nq = p.q_start[b + 1] - q0;
-  const int first_tok = s_info[1] * per_tile, ntok = min(per_tile, nq - first_tok);
+  const int first_tok = s_info[1] * per_block, ntok = min(per_block, nq - first_tok);
+  const bool two = NS == 2 && ntok > per_tile;              // two query tiles, one for each softmax group; else they share one
   const int len = paged_len(g, p.seq_len[b], p.status, tid == 0 && layer == 0 && h == 0 && piece == 0);
   const int visible = p.causal ? min(len, max(0, len - nq + first_tok + ntok)) : len;   // of the tile's last token
   const int all_tiles = (visible + kKeys - 1) / kKeys;
@@ -272,7 +286,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = (uint32_t)s_info[3];
+  constexpr uint32_t tmem = 0;                              // all 512 columns are this block's: they begin at 0
 
   float r_v = 0.f;                                          // largest V scale of the block's keys (V and softmax warps)
   if (warp >= kTma) regs_down<P::REGS_OTHER>();
@@ -369,53 +383,56 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // ================= products =================
     int s_issued = 0, o_issued = 0;
     bool ok = wait_for(qready, 0, gave_up, p.status);
-    const uint64_t descQ = smem_desc_k128(sQ), descK = smem_desc_k128(sK);
-    const uint64_t descV = smem_desc_mn128(sV, P::UNIT_KEYS * 128);
-    auto issue_s = [&](int j) {
-      const int st = j % KST;
-      if (!wait_for(kfull + 8 * st, (j / KST) & 1, gave_up, p.status)) return false;
+    const uint32_t lowQ = (sQ >> 4) | (1u << 16), lowK = (sK >> 4) | (1u << 16), lowV = (sV >> 4) | ((uint32_t)(P::UNIT_KEYS * 128 >> 4) << 16);
+    // Products in the order of items: item i works in score buffer i & 1.  One query tile: item = key tile.  Two: items 2 t and
+    // 2 t + 1 are key tile t for the first and the second query tile.
+    const int items = two ? 2 * nt : nt, sh = two ? 1 : 0;
+    auto issue_s = [&](int i) {
+      const int t = i >> sh, st = t % KST;
+      if (!wait_for(kfull + 8 * st, (t / KST) & 1, gave_up, p.status)) return false;
+      __syncwarp();
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t d = tmem + (uint32_t)(j & 1) * 128u;
+      if (elect_one()) {
+        const uint32_t d = tmem + (uint32_t)(i & 1) * 128u;
+        const uint32_t qa = lowQ + (two ? (uint32_t)(i & 1) * (P::QTILE >> 4) : 0u), kb0 = lowK + (uint32_t)st * (P::KTILE >> 4);
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int hf = 0; hf < DH; ++hf)
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
-              umma_f8(d, descQ + (uint64_t)((term * DH + hf) * (kRows * 128 >> 4) + kb * 2), descK + (uint64_t)(st * (P::KTILE >> 4) + hf * (kKeys * 128 >> 4) + kb * 2),
-                      kIdescS, (term | hf | kb) ? 1u : 0u);
-        umma_commit(sfull + 8 * (j & 1));
-        umma_commit(kempty + 8 * st);
+              umma_s(d, qa + (term * DH + hf) * (kRows * 128 >> 4) + kb * 2, kb0 + hf * (kKeys * 128 >> 4) + kb * 2, kIdescS, (term | hf | kb) != 0);
+        umma_commit(sfull + 8 * (i & 1));
+        if (!two || (i & 1)) umma_commit(kempty + 8 * st);
       }
       __syncwarp();
       ++s_issued;
       return true;
     };
     ok = ok && issue_s(0);
-    if (nt > 1) ok = ok && issue_s(1);
-    int vu = 0;
-    for (int j = 0; j < nt && ok; ++j) {
-      ok = wait_for(pfull + 8 * (j & 1), (j >> 1) & 1, gave_up, p.status);
+    if (items > 1) ok = ok && issue_s(1);
+    for (int i = 0; i < items && ok; ++i) {
+      ok = wait_for(pfull + 8 * (i & 1), (i >> 1) & 1, gave_up, p.status);
+      int vu = (i >> sh) * P::UNITS;
 #pragma unroll 1
       for (int u = 0; u < P::UNITS && ok; ++u, ++vu) {
         const int st = vu % kVRing;
         ok = wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
+        __syncwarp();
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t d = tmem + 256u + (NS == 2 ? (uint32_t)(j & 1) * 128u : 0u);
-          const uint32_t a = tmem + (uint32_t)(j & 1) * 128u + (uint32_t)u * (P::UNIT_KEYS / 2);
+        if (elect_one()) {
+          const uint32_t d = tmem + 256u + (NS == 2 ? (uint32_t)(i & 1) * 128u : 0u);
+          const uint32_t a = tmem + (uint32_t)(i & 1) * 128u + (uint32_t)u * (P::UNIT_KEYS / 2), v0 = lowV + (uint32_t)st * (kUnitBytes >> 4);
 #pragma unroll
-          for (int kb = 0; kb < P::UNIT_KEYS / 16; ++kb)
-            umma_f16_ts(d, a + kb * 8, descV + (uint64_t)(st * (kUnitBytes >> 4) + kb * (2048 >> 4)), kIdescO, (j >= NS || u || kb) ? 1u : 0u);
-          umma_commit(vempty + 8 * st);
-          if (u == P::UNITS - 1) umma_commit(odone + 8 * (j & 1));
+          for (int kb = 0; kb < P::UNIT_KEYS / 16; ++kb) umma_o(d, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb ? true : i >= NS || u > 0);
+          if (!two || (i & 1)) umma_commit(vempty + 8 * st);
+          if (u == P::UNITS - 1) umma_commit(odone + 8 * (i & 1));
         }
         __syncwarp();
       }
       if (ok) ++o_issued;
-      if (ok && j + 2 < nt) ok = issue_s(j + 2);
+      if (ok && i + 2 < items) ok = issue_s(i + 2);
     }
     // every softmax warp has read its output, and the TMA warp has said what it issued
     asm volatile("bar.sync 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
@@ -514,24 +531,26 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   } else if (warp < kSoftmaxWarps) {
     // ================= softmax: one thread per query row =================
     const int grp = warp >> 2, row = tid & 127;
-    const int tok = row / G, head = row % G;
-    const bool real = tok < ntok;
+    const int tile_tok = two ? grp * per_tile : 0, tok = tile_tok + row / G, head = row % G;
+    const bool real = row / G < per_tile && tok < ntok;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint16_t* qrow = p.q + (out_row0 + (long long)tok * g.h_q + head) * D;
     regs_up<P::REGS_SOFTMAX>();
-    // the query row as two e4m3 rows; with two groups each takes half of the row's dims
-    constexpr int NQ = 8, ROUNDS = D / 8 / NS / NQ;          // 16-byte loads at a time
+    // the query row as two e4m3 rows; two groups that share a tile take half of the row's dims each
+    constexpr int NQ = 8, ROUNDS = D / 8 / NQ;              // 16-byte loads at a time
+    const bool halves = NS == 2 && !two;
+    const int round0 = halves ? grp : 0, round1 = halves ? grp + 1 : ROUNDS;
+    const uint32_t sq = sQ + (two ? grp * P::QTILE : 0);
     float rowmul;
     {
       uint4 raw[NQ];
       auto load_q = [&](int round) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-          raw[i] = real ? __ldg(reinterpret_cast<const uint4*>(qrow) + (grp * ROUNDS + round) * NQ + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < NQ; ++i) raw[i] = real ? __ldg(reinterpret_cast<const uint4*>(qrow) + round * NQ + i) : make_uint4(0, 0, 0, 0);
       };
       float amax = 0.f;
-#pragma unroll
-      for (int round = 0; round < ROUNDS; ++round) {
+#pragma unroll 1
+      for (int round = round0; round < round1; ++round) {
         load_q(round);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
@@ -540,7 +559,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           for (int e = 0; e < 4; ++e) amax = max3(amax, fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xFFFF0000u)));
         }
       }
-      if (NS == 2) {
+      if (halves) {
         s_amax[grp][row] = amax;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         amax = fmaxf(s_amax[0][row], s_amax[1][row]);
@@ -550,11 +569,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       const float down = __uint_as_float((uint32_t)(261 - ex) << 23), up = __uint_as_float((uint32_t)(ex - 7) << 23);   // largest |q| in [128, 256)
       rowmul = up * p.score_scale;
 #pragma unroll 1
-      for (int round = 0; round < ROUNDS; ++round) {
-      if (ROUNDS > 1) load_q(round);                        // again, from the caches
+      for (int round = round0; round < round1; ++round) {
+      if (!halves) load_q(round);                           // again, from the caches
 #pragma unroll
       for (int ci = 0; ci < NQ / 2; ++ci) {                 // 16 dims
-        const int c = (grp * ROUNDS + round) * (NQ / 2) + ci;
+        const int c = round * (NQ / 2) + ci;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -569,8 +588,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           }
         }
         const uint32_t off = (uint32_t)(c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        sts128(sQ + off, hi[0], hi[1], hi[2], hi[3]);
-        sts128(sQ + DH * kRows * 128 + off, lo[0], lo[1], lo[2], lo[3]);
+        sts128(sq + off, hi[0], hi[1], hi[2], hi[3]);
+        sts128(sq + DH * kRows * 128 + off, lo[0], lo[1], lo[2], lo[3]);
       }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -582,14 +601,15 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
     float m = -INFINITY, l = 0.f;
     bool alive = true;
-    for (int j = grp; j < nt && alive; j += NS) {
-      const int base = (j0 + j) * kKeys;
+    const int items = two ? 2 * nt : nt;
+    for (int i = grp; i < items && alive; i += NS) {
+      const int j = two ? i >> 1 : i, base = (j0 + j) * kKeys;
       alive = wait_for(kinfo + 8 * (j % kInfo), (j / kInfo) & 1, gave_up, p.status);
-      if (alive) alive = wait_for(sfull + 8 * (j & 1), (j >> 1) & 1, gave_up, p.status);
+      if (alive) alive = wait_for(sfull + 8 * (i & 1), (i >> 1) & 1, gave_up, p.status);
       __syncwarp();
       if (!alive) break;
       tc_fence_after();
-      const uint32_t ts = tmem + lane_base + (uint32_t)(j & 1) * 128u;
+      const uint32_t ts = tmem + lane_base + (uint32_t)(i & 1) * 128u;
       uint32_t s[128];
       tmem_ld128(ts, s);
       float f[8];                                           // score multipliers of 16 keys each
@@ -606,8 +626,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         for (int c = 0; c < 8; ++c) {
           const int n = f[c] < 0.f ? 0 : vis - base - 16 * c;   // keys of these 16 that the row sees
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i >= n) s[16 * c + i] = 0xFF800000u;
+          for (int e = 0; e < 16; ++e)
+            if (e >= n) s[16 * c + e] = 0xFF800000u;
         }
       }
       // ---- maximum ----
@@ -618,9 +638,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const uint32_t* x = s + 16 * c;
         float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
 #pragma unroll
-        for (int i = 2; i < 14; i += 4) {
-          m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-          m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+        for (int e = 2; e < 14; e += 4) {
+          m0 = max3(m0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          m1 = max3(m1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
         }
         m0 = max3(m0, __uint_as_float(x[14]), __uint_as_float(x[15]));
         tmax = fmaxf(tmax, fmaxf(m0, m1) * f[c]);
@@ -632,9 +652,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         m = tmax;
         l *= alpha;
       }
-      if (j >= NS && __any_sync(0xffffffffu, alpha != 1.f)) {
+      if (i >= NS && __any_sync(0xffffffffu, alpha != 1.f)) {
         if (NS == 1) {                                      // the product of the tile before (two groups: complete, since these scores are)
-          alive = wait_for(odone + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1, gave_up, p.status);
+          alive = wait_for(odone + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1, gave_up, p.status);
           if (!alive) break;
           tc_fence_after();
         }
@@ -644,7 +664,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           uint32_t x[16];
           tmem_ld16(to + 16 * c, x);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
           tmem_st16_nowait(to + 16 * c, x);
         }
       }
@@ -656,17 +676,17 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const unsigned long long f2 = pair2(f[2 * c + (i >> 4)], f[2 * c + (i >> 4)]);
+        for (int e = 0; e < 32; e += 4) {
+          const unsigned long long f2 = pair2(f[2 * c + (e >> 4)], f[2 * c + (e >> 4)]);
           float x0, x1, x2, x3;
-          split2(fma2(pair2(__uint_as_float(s[32 * c + i]), __uint_as_float(s[32 * c + i + 1])), f2, mb2), x0, x1);
-          split2(fma2(pair2(__uint_as_float(s[32 * c + i + 2]), __uint_as_float(s[32 * c + i + 3])), f2, mb2), x2, x3);
+          split2(fma2(pair2(__uint_as_float(s[32 * c + e]), __uint_as_float(s[32 * c + e + 1])), f2, mb2), x0, x1);
+          split2(fma2(pair2(__uint_as_float(s[32 * c + e + 2]), __uint_as_float(s[32 * c + e + 3])), f2, mb2), x2, x3);
           x0 = ex2(x0); x1 = ex2(x1); x2 = ex2(x2); x3 = ex2(x3);
           sum0 = add2(sum0, pair2(x0, x1));
           sum1 = add2(sum1, pair2(x2, x3));
           const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
-          pk[i / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-          pk[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          pk[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+          pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
         tmem_st16_nowait(ts + 16 * c, pk);
       }
@@ -678,17 +698,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pfull + 8 * (j & 1));
+      if (lane == 0) mbar_arrive(pfull + 8 * (i & 1));
     }
 
     // ---- the end: this group's last product ----
-    const int mine = (nt - grp + NS - 1) / NS;              // tiles of this group
+    const int mine = (items - grp + NS - 1) / NS;           // items of this group
     if (alive && mine > 0) {
-      const int jl = grp + (mine - 1) * NS;
-      alive = wait_for(odone + 8 * (jl & 1), (jl >> 1) & 1, gave_up, p.status);
+      const int il = grp + (mine - 1) * NS;
+      alive = wait_for(odone + 8 * (il & 1), (il >> 1) & 1, gave_up, p.status);
+      __syncwarp();
       tc_fence_after();
     }
-    if (NS == 2) {
+    if (halves) {
       s_ml[grp][0][row] = m;
       s_ml[grp][1][row] = l;
       tc_fence_before();
@@ -699,7 +720,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
     for (int i = 1; i < 4; ++i) r_v = fmaxf(r_v, s_red[i]); // written before the first V unit was
     float f0 = 1.f, f1 = 0.f, M = m, L = l;
-    if (NS == 2) {
+    if (halves) {
       const float m0 = s_ml[0][0][row], m1 = s_ml[1][0][row];
       M = fmaxf(m0, m1);
       f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M);
@@ -711,14 +732,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     float* part = p.part + ((long long)(blockIdx.x / p.splits) * p.splits + piece) * (kRows * (D + 2));
     if (alive && !*gave_up) {
 #pragma unroll 1
-      for (int c = grp * (D / 32 / NS); c < (grp + 1) * (D / 32 / NS); ++c) {
+      for (int c = halves ? grp * (D / 64) : 0; c < (halves ? (grp + 1) * (D / 64) : D / 32); ++c) {
         uint32_t x[32];
         float o[32];
-        tmem_ld32(tmem + lane_base + 256u + 32 * c, x);
+        tmem_ld32(tmem + lane_base + 256u + (two ? grp * 128u : 0u) + 32 * c, x);
         tmem_wait32(x);
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = f0 == 0.f ? 0.f : __uint_as_float(x[i]) * f0;
-        if (NS == 2 && nt > 1) {
+        if (halves && nt > 1) {
           tmem_ld32(tmem + lane_base + 384u + 32 * c, x);
           tmem_wait32(x);
 #pragma unroll
@@ -742,7 +763,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i] * scale, o[4 * i + 1] * scale, o[4 * i + 2] * scale, o[4 * i + 3] * scale);
         }
       }
-      if (pieces > 1 && real && grp == 0) {
+      if (pieces > 1 && real && (!halves || grp == 0)) {
         part[kRows * D + row] = M;
         part[kRows * D + kRows + row] = L;
       }
@@ -785,16 +806,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 }
 
 // Query tiles of a layer and head, at most: every sequence can have one that is not full, and has none without tokens.
-long long prefill_tiles(const PagedGeometry& g, int n_tokens) {
-  const int per_tile = kRows / g.group;
-  const long long most = (long long)n_tokens / per_tile + g.batch;
+long long prefill_tiles(const PagedGeometry& g, int n_tokens, int pair) {
+  const int per_block = (kRows / g.group) << pair;
+  const long long most = (long long)n_tokens / per_block + g.batch;
   return most < n_tokens ? most : n_tokens;
+}
+// Two query tiles in a block share its K copies, V conversion and V reads; where that leaves SMs without a block, one tile each.
+int prefill_pair(const PagedGeometry& g, int n_tokens) {
+  return g.head_dim == 128 && prefill_tiles(g, n_tokens, 1) * g.h_kv * g.n_layers >= device_sms() ? 1 : 0;
 }
 // Pieces of the keys: where the query tiles do not fill the GPU, as many as do, none under 4 tiles of keys.
 int prefill_splits(const PagedGeometry& g, int n_tokens, int max_seq_len) {
   const long long cap = (long long)g.max_pages * g.page_size;
   const long long most = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
-  const long long blocks = prefill_tiles(g, n_tokens) * g.h_kv * g.n_layers;
+  const long long blocks = prefill_tiles(g, n_tokens, prefill_pair(g, n_tokens)) * g.h_kv * g.n_layers;
   if (blocks < 1) return 1;
   long long want = device_sms() / blocks;
   const long long by_len = (most + 4 * kKeys - 1) / (4 * kKeys);
@@ -828,7 +853,8 @@ cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a,
   p.n_tokens = a.n_tokens;
   p.causal = a.causal;
   p.page_shift = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
-  p.tiles = (int)prefill_tiles(g, a.n_tokens);
+  p.pair = prefill_pair(g, a.n_tokens);
+  p.tiles = (int)prefill_tiles(g, a.n_tokens, p.pair);
   p.splits = prefill_splits(g, a.n_tokens, a.max_seq_len);
   p.score_scale = a.softmax_scale * kLog2e;
   p.counters = (int*)a.workspace;

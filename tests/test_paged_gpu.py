@@ -389,3 +389,11 @@ def test_other_stream_and_bits_stay_the_same(pkg, cuda_device):
         want, big = ref.attention(q[0, i:i + 1].cpu(), kb[0], vb[0], ks[0], vs[0], table[i], n)
         ref.assert_attention(a[0][0, i:i + 1].cpu(), want, big)
         ref.assert_attention(b[0][0, i:i + 1].cpu(), want, big)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_enough_rows_for_the_whole_gpu(pkg, cuda_device, causal):
+    """As many query tiles as make every thread block take two of them (heads of 128), with blocks that have one tile, a full
+    pair, or a pair whose second tile has one token."""
+    _run_attention(pkg, cuda_device, (1, (40, 8, 128), 64, [700, 1000, 26, 80, 25]), qlens=[700, 333, 26, 51, 25], causal=causal, seed=31)
+    _run_attention(pkg, cuda_device, (1, (16, 16, 128), 32, [600, 129]), qlens=[600, 129], causal=causal, seed=32)
