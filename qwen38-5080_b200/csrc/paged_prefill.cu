@@ -33,6 +33,7 @@ constexpr int kInfo = 8;                   // tiles whose scales are in flight
 constexpr int kVRing = 2;                  // V units of 32 KB in f16
 constexpr int kUnitBytes = 32768;
 constexpr float kTauP = 4.f, kBitsP = 11.f;   // p <= 2^4, held times 2^11 in f16
+constexpr int kPolyEvery = 2;              // of 8 exponentials, 2 by polynomial (of 4 kPolyEvery)
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
 
 struct PrefillParams {
@@ -189,6 +190,23 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// 2^x of two values without the special-function unit: x = n + f, n the nearest integer (from the low bits of x + 1.5 2^23), 2^f by
+// the degree-3 polynomial of least relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 = 2^-13.7, against the f16 rounding of
+// up to 2^-11 that follows), n added to its exponent.
+__device__ __forceinline__ void ex2_pair(float& x, float& y) {
+  const unsigned long long v = pair2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const unsigned long long t = add2(v, pair2(12582912.f, 12582912.f));
+  const unsigned long long f = add2(v, fma2(t, pair2(-1.f, -1.f), pair2(12582912.f, 12582912.f)));
+  unsigned long long q = fma2(f, pair2(0.0551716691f, 0.0551716691f), pair2(0.242611122f, 0.242611122f));
+  q = fma2(q, f, pair2(0.693260985f, 0.693260985f));
+  q = fma2(q, f, pair2(0.999928074f, 0.999928074f));
+  float t0, t1, q0, q1;
+  split2(t, t0, t1);
+  split2(q, q0, q1);
+  x = __uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(q0));
+  y = __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(q1));
+}
+
 template <int D>
 __global__ void __launch_bounds__(PrefillPlan<D>::THREADS, 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefillParams p) {
@@ -208,7 +226,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   __shared__ __align__(16) int s_id[kInfo][8];
   __shared__ float s_red[4];
   __shared__ float s_ml[2][2][kRows], s_amax[2][kRows];
-  __shared__ int s_info[8];                                 // [0] sequence [1] tile of it, later V units issued [2] gave up [3] tensor memory [4] last
+  __shared__ int s_info[10];   // [0] sequence [1] tile of it [2] gave up [3] tensor memory [4] last [5] first row [6] rows [7] length [8] K tiles, [9] V units issued
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = smem0, sK = sQ + NS * P::QTILE, sV = sK + KST * P::KTILE, sRaw = sV + kVRing * kUnitBytes;
@@ -231,9 +249,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     __syncwarp();
     for (int b0 = 0; b0 < g.batch; b0 += 32) {
       const int b = b0 + lane;
-      int n = 0;
+      int n = 0, q0 = 0, nq = 0, raw_len = 0;
       if (b < g.batch) {
-        const int q0 = p.q_start[b], nq = p.q_start[b + 1] - q0;
+        q0 = p.q_start[b];
+        nq = p.q_start[b + 1] - q0;
+        raw_len = p.seq_len[b];
         if (nq > 0 && q0 >= 0 && q0 + nq <= p.n_tokens) n = (nq + per_block - 1) / per_block;
       }
       int inc = n;
@@ -243,7 +263,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         if (lane >= off) inc += t;
       }
       const int start = before + inc - n;
-      if (n > 0 && number >= start && number < start + n) { s_info[0] = b; s_info[1] = number - start; }
+      if (n > 0 && number >= start && number < start + n) { s_info[0] = b; s_info[1] = number - start; s_info[5] = q0; s_info[6] = nq; s_info[7] = raw_len; }
       before += __shfl_sync(0xffffffffu, inc, 31);
       if (before > number) break;
     }
@@ -262,10 +282,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   __syncthreads();
   const int b = s_info[0];
   if (b < 0) return;                                        // the grid is an upper bound
-  const int q0 = p.q_start[b], nq = p.q_start[b + 1] - q0;
+  const int q0 = s_info[5], nq = s_info[6];
   const int first_tok = s_info[1] * per_block, ntok = min(per_block, nq - first_tok);
   const bool two = NS == 2 && ntok > per_tile;              // two query tiles, one for each softmax group; else they share one
-  const int len = paged_len(g, p.seq_len[b], p.status, tid == 0 && layer == 0 && h == 0 && piece == 0);
+  const int len = paged_len(g, s_info[7], p.status, tid == 0 && layer == 0 && h == 0 && piece == 0);
   const int visible = p.causal ? min(len, max(0, len - nq + first_tok + ntok)) : len;   // of the tile's last token
   const int all_tiles = (visible + kKeys - 1) / kKeys;
   const int per_piece = (all_tiles + p.splits - 1) / p.splits;
@@ -282,10 +302,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int j0 = piece * per_piece, nt = min(per_piece, all_tiles - j0);
   const int key_end = min(len, (j0 + nt) * kKeys);
 
-  if (warp == kMma) tmem_alloc(smem_u32(s_info + 3), 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   constexpr uint32_t tmem = 0;                              // all 512 columns are this block's: they begin at 0
 
   float r_v = 0.f;                                          // largest V scale of the block's keys (V and softmax warps)
@@ -324,8 +340,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     };
     int idp = -2, id0 = page_at(0), id1 = page_at(1), id2 = page_at(2), id3 = page_at(3);
     float2 sc0 = scales_at(id0), sc1 = scales_at(id1), sc2 = scales_at(id2);
-    publish(0, id0, sc0);
-    publish(1, id1, sc1);
     for (int j = 0; j <= nt && ok; ++j) {                   // K tile j, then V tile j - 1
       int id4_ = -2;
       float2 sc3_ = make_float2(0.f, 0.f);
@@ -347,6 +361,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             tma_load_3d(sK + st * P::KTILE + hf * kKeys * 128 + lane * 16 * 128, &kmap, hf * 128, (id0 * g.h_kv + h) << p.page_shift, layer, kfull + 8 * st);
         }
         ++issued;
+        if (j == 0) { publish(0, id0, sc0); publish(1, id1, sc1); }
         publish(j + 2, id2, sc2);
         id4_ = id4; sc3_ = sc3;
       }
@@ -376,11 +391,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       idp = id0; id0 = id1; id1 = id2; id2 = id3; id3 = id4_;
       sc2 = sc3_;
     }
-    if (lane == 0) { s_info[5] = issued; s_info[1] = vissued; }
+    if (lane == 0) { s_info[8] = issued; s_info[9] = vissued; }
     __syncwarp();
     asm volatile("bar.arrive 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
   } else if (warp == kMma) {
     // ================= products =================
+    tmem_alloc(smem_u32(s_info + 3), 512);                  // used by others only after this warp's first product
     int s_issued = 0, o_issued = 0;
     bool ok = wait_for(qready, 0, gave_up, p.status);
     const uint32_t lowQ = (sQ >> 4) | (1u << 16), lowK = (sK >> 4) | (1u << 16), lowV = (sV >> 4) | ((uint32_t)(P::UNIT_KEYS * 128 >> 4) << 16);
@@ -445,8 +461,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           while (!mbar_try_wait(bar + 8 * s, (last / ring) & 1) && global_timer_ns() - t0 < kWaitBudgetNs) {}
         }
       };
-      drain(kfull, KST, s_info[5]);
-      drain(rfull, P::RAW, s_info[1]);
+      drain(kfull, KST, s_info[8]);
+      drain(rfull, P::RAW, s_info[9]);
       drain(sfull, 2, s_issued);
       drain(odone, 2, o_issued);
     }
@@ -491,9 +507,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       if (alive) alive = wait_for(rfull + 8 * rs, (u / P::RAW) & 1, gave_up, p.status);
       if (alive && u >= kVRing) alive = wait_for(vempty + 8 * st, ((u / kVRing) - 1) & 1, gave_up, p.status);
       if (!alive) break;
-      const float* vs = s_vs[t % kInfo] + (u % P::UNITS) * (P::UNIT_KEYS / 16);
-      const int* ids = s_id[t % kInfo] + (u % P::UNITS) * (P::UNIT_KEYS / 16);
+      // Lane c holds the multiplier of the unit's keys 16 c ..: the page's scale relative to the largest, as an f16, and what that
+      // rounds away.  Nothing is rounded where scales are powers of two (the append's): then one product per pair of values.
+      const int c0 = (u % P::UNITS) * (P::UNIT_KEYS / 16), cl = c0 + lane % (P::UNIT_KEYS / 16);
+      const float ratio = s_vs[t % kInfo][cl] * inv_r;
+      const __half2 hi2 = __float2half2_rn(ratio), lo2 = __float2half2_rn(ratio - __low2float(hi2));
+      const uint32_t hi_bits = *reinterpret_cast<const uint32_t*>(&hi2), lo_bits = *reinterpret_cast<const uint32_t*>(&lo2);
+      const bool page_ok = s_id[t % kInfo][cl] >= 0;
       const int left = key_end - (j0 * kKeys + u * P::UNIT_KEYS);   // keys of the unit that exist
+      const bool plain = __all_sync(0xffffffffu, page_ok && __low2float(lo2) == 0.f) && left >= P::UNIT_KEYS;
+      const uint32_t pages_ok = __ballot_sync(0xffffffffu, page_ok);
 #pragma unroll
       for (int i0 = 0; i0 < N; i0 += 4) {
         uint4 raw[4];
@@ -501,20 +524,30 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         for (int i = 0; i < 4; ++i) raw[i] = lds128(src + rs * P::RAW_BYTES + (i0 + i) * STEP * 128);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = row0 + (i0 + i) * STEP, c = (i0 + i) * STEP / 16;
-          // the page's scale relative to the largest, as leading part + remainder; nothing behind the last key (bytes there may be
-          // NaN patterns) and nothing of a page that does not exist
-          const float ratio = vs[c] * inv_r;
-          const __half2 hi = __float2half2_rn(ratio), lo = __float2half2_rn(ratio - __low2float(hi));
-          const bool there = row < left && ids[c] >= 0, exact = __low2float(lo) == 0.f;   // exact: powers of two
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          const int c = (i0 + i) * STEP / 16;
+          const uint32_t mh = __shfl_sync(0xffffffffu, hi_bits, c);
+          const __half2 hi = *reinterpret_cast<const __half2*>(&mh);
           uint32_t o[8];
+          if (plain) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t h2 = e4m3x2_to_f16x2((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
-            const __half2 x = *reinterpret_cast<const __half2*>(&h2);
-            const __half2 y = exact ? __hmul2(x, hi) : __hfma2(x, hi, __hmul2(x, lo));
-            o[e] = there ? *reinterpret_cast<const uint32_t*>(&y) : 0u;
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t h2 = e4m3x2_to_f16x2((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h2), hi);
+              o[e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+          } else {   // nothing behind the last key (bytes there may be NaN patterns), nothing of a page that does not exist
+            const uint32_t ml = __shfl_sync(0xffffffffu, lo_bits, c);
+            const __half2 lo = *reinterpret_cast<const __half2*>(&ml);
+            const bool there = row0 + (i0 + i) * STEP < left && ((pages_ok >> c) & 1u);
+            const uint32_t w[4] = {there ? raw[i].x : 0u, there ? raw[i].y : 0u, there ? raw[i].z : 0u, there ? raw[i].w : 0u};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t h2 = e4m3x2_to_f16x2((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
+              const __half2 x = *reinterpret_cast<const __half2*>(&h2);
+              const __half2 y = there ? __hfma2(x, hi, __hmul2(x, lo)) : x;
+              o[e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
           }
           const uint32_t off = st * kUnitBytes + (i0 + i) * STEP * 128;
           sts128(dst0 + off, o[0], o[1], o[2], o[3]);
@@ -537,20 +570,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     const uint16_t* qrow = p.q + (out_row0 + (long long)tok * g.h_q + head) * D;
     regs_up<P::REGS_SOFTMAX>();
     // the query row as two e4m3 rows; two groups that share a tile take half of the row's dims each
-    constexpr int NQ = 8, ROUNDS = D / 8 / NQ;              // 16-byte loads at a time
+    constexpr int NQ = 16, ROUNDS = D / 8 / NQ;             // 16-byte loads at a time
     const bool halves = NS == 2 && !two;
-    const int round0 = halves ? grp : 0, round1 = halves ? grp + 1 : ROUNDS;
+    const int first = halves ? grp * (NQ / 2) : 0, count = halves ? NQ / 2 : NQ;   // of a round
     const uint32_t sq = sQ + (two ? grp * P::QTILE : 0);
     float rowmul;
     {
       uint4 raw[NQ];
       auto load_q = [&](int round) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) raw[i] = real ? __ldg(reinterpret_cast<const uint4*>(qrow) + round * NQ + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < NQ; ++i) raw[i] = real && i < count ? __ldg(reinterpret_cast<const uint4*>(qrow) + round * NQ + first + i) : make_uint4(0, 0, 0, 0);
       };
       float amax = 0.f;
 #pragma unroll 1
-      for (int round = round0; round < round1; ++round) {
+      for (int round = 0; round < ROUNDS; ++round) {
         load_q(round);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
@@ -569,11 +602,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       const float down = __uint_as_float((uint32_t)(261 - ex) << 23), up = __uint_as_float((uint32_t)(ex - 7) << 23);   // largest |q| in [128, 256)
       rowmul = up * p.score_scale;
 #pragma unroll 1
-      for (int round = round0; round < round1; ++round) {
-      if (!halves) load_q(round);                           // again, from the caches
+      for (int round = 0; round < ROUNDS; ++round) {
+      if (ROUNDS > 1) load_q(round);                        // again, from the caches
 #pragma unroll
       for (int ci = 0; ci < NQ / 2; ++ci) {                 // 16 dims
-        const int c = round * (NQ / 2) + ci;
+        if (2 * ci >= count) break;
+        const int c = (round * NQ + first) / 2 + ci;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -681,7 +715,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           float x0, x1, x2, x3;
           split2(fma2(pair2(__uint_as_float(s[32 * c + e]), __uint_as_float(s[32 * c + e + 1])), f2, mb2), x0, x1);
           split2(fma2(pair2(__uint_as_float(s[32 * c + e + 2]), __uint_as_float(s[32 * c + e + 3])), f2, mb2), x2, x3);
-          x0 = ex2(x0); x1 = ex2(x1); x2 = ex2(x2); x3 = ex2(x3);
+          x0 = ex2(x0); x1 = ex2(x1);
+          if ((e / 4) % kPolyEvery == kPolyEvery - 1) {     // a share of them on the FMA pipe
+            ex2_pair(x2, x3);
+          } else {
+            x2 = ex2(x2); x3 = ex2(x3);
+          }
           sum0 = add2(sum0, pair2(x0, x1));
           sum1 = add2(sum1, pair2(x2, x3));
           const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
