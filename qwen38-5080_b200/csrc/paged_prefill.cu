@@ -10,9 +10,15 @@
 //   * V is widened to f16 by four warps on its way from global to shared memory (exact; times the page's scale relative to
 //     the largest scale of the block's keys), because P needs more than 8 bits: P is f16 in tensor memory, in the columns
 //     that its scores left, and O += P V is kind::f16 with P as the tensor-memory operand.
-//   * softmax: one thread per row, which takes its 128 scores into registers (the other warps give theirs up for it).  The reference maximum moves only when a tile exceeds it by 2^4, so O is rarely rescaled.
-//   * heads of 128: two groups of softmax warps take alternate tiles, each with its own maximum, sum and O, joined at the
-//     end; heads of 256: one group (O fills the tensor memory, and the products take twice as long per tile).
+//   * softmax: one thread per row, which takes its 128 scores into registers (the other warps give theirs up for it).  The
+//     exponentials are taken against the reference maximum as it stands, without looking for the tile's maximum first; a
+//     p far beyond it shows in the sum, and only then the reference moves and O is rescaled.  f16 holds 2^12 above the
+//     reference and 2^28 below it, sums and O are fp32: nothing is lost by a reference that is not the maximum.
+//   * a tile's P is handed over in halves, so that the first is multiplied while the second's exponentials are taken.
+//   * heads of 128: two groups of softmax warps, each with its own S, P and O.  With rows enough a block takes two query tiles,
+//     one for each group, which share the K copies and the V conversion; otherwise the groups take alternate key tiles of
+//     one query tile, joined at the end.  Heads of 256: one group (O fills the tensor memory, and the products take twice as
+//     long per tile).
 // Tensor memory: S0 S1 at columns 0 and 128, O at 256 (two of 128 columns, or one of 256).
 //
 // Bound: the tensor cores (4 D flops per row, key and head), and as much the exponentials, one per row and key:
@@ -32,7 +38,7 @@ constexpr int kKeys = 128;                 // keys of a tile
 constexpr int kInfo = 8;                   // tiles whose scales are in flight
 constexpr int kVRing = 2;                  // V units of 32 KB in f16
 constexpr int kUnitBytes = 32768;
-constexpr float kTauP = 4.f, kBitsP = 11.f;   // p <= 2^4, held times 2^11 in f16
+constexpr float kBitsP = 4.f, kMostP = 61440.f;   // p is held times 2^4 in f16; what 64 keys may add up to before the reference moves
 constexpr int kPolyEvery = 2;              // of 8 exponentials, 2 by polynomial (of 4 kPolyEvery)
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
 
@@ -220,7 +226,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int G = g.group;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 2 * P::RAW + 6];
+  __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 2 * P::RAW + 10];
   // each 16 keys of a tile: K scale (-1: no such page), V scale, page (-1: none)
   __shared__ __align__(16) float s_ks[kInfo][8], s_vs[kInfo][8];
   __shared__ __align__(16) int s_id[kInfo][8];
@@ -232,8 +238,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const uint32_t sQ = smem0, sK = sQ + NS * P::QTILE, sV = sK + KST * P::KTILE, sRaw = sV + kVRing * kUnitBytes;
   const uint32_t qready = smem_u32(bars), kfull = qready + 8, kempty = kfull + 8 * KST, kinfo = kempty + 8 * KST;
   const uint32_t vfull = kinfo + 8 * kInfo, vempty = vfull + 8 * kVRing;
-  const uint32_t sfull = vempty + 8 * kVRing, pfull = sfull + 16, odone = pfull + 16;
-  const uint32_t rfull = odone + 16, rempty = rfull + 8 * P::RAW;
+  const uint32_t sfull = vempty + 8 * kVRing, pfull = sfull + 16, odone = pfull + 32;   // of both halves of both buffers
+  const uint32_t rfull = odone + 32, rempty = rfull + 8 * P::RAW;
   volatile int* gave_up = s_info + 2;
 
   // ---- which tile: piece fastest, then head, layer, query tile from the last (most keys) to the first ----
@@ -274,7 +280,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     for (int i = 0; i < kInfo; ++i) mbar_init(kinfo + 8 * i, 1);
     for (int i = 0; i < kVRing; ++i) { mbar_init(vfull + 8 * i, 4); mbar_init(vempty + 8 * i, 1); }
     for (int i = 0; i < P::RAW; ++i) { mbar_init(rfull + 8 * i, 1); mbar_init(rempty + 8 * i, 4); }
-    for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(odone + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(sfull + 8 * i, 1);
+    for (int i = 0; i < 4; ++i) { mbar_init(pfull + 8 * i, 4); mbar_init(odone + 8 * i, 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     s_info[2] = 0;
@@ -428,22 +435,23 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     ok = ok && issue_s(0);
     if (items > 1) ok = ok && issue_s(1);
     for (int i = 0; i < items && ok; ++i) {
-      ok = wait_for(pfull + 8 * (i & 1), (i >> 1) & 1, gave_up, p.status);
-      int vu = (i >> sh) * P::UNITS;
+      // keys 0..63 of the tile, then 64..127: the first half is multiplied while the second half's exponentials are taken
 #pragma unroll 1
-      for (int u = 0; u < P::UNITS && ok; ++u, ++vu) {
-        const int st = vu % kVRing;
+      for (int half = 0; half < 2 && ok; ++half) {
+        const int bar = 2 * (i & 1) + half, vu = (i >> sh) * P::UNITS + (P::UNITS == 2 ? half : 0), st = vu % kVRing;
         ok = wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
+        if (ok) ok = wait_for(pfull + 8 * bar, (i >> 1) & 1, gave_up, p.status);
         __syncwarp();
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t d = tmem + 256u + (NS == 2 ? (uint32_t)(i & 1) * 128u : 0u);
-          const uint32_t a = tmem + (uint32_t)(i & 1) * 128u + (uint32_t)u * (P::UNIT_KEYS / 2), v0 = lowV + (uint32_t)st * (kUnitBytes >> 4);
+          const uint32_t a = tmem + (uint32_t)(i & 1) * 128u + (uint32_t)half * 32u;
+          const uint32_t v0 = lowV + (uint32_t)st * (kUnitBytes >> 4) + (P::UNITS == 2 ? 0u : (uint32_t)half * (8192 >> 4));
 #pragma unroll
-          for (int kb = 0; kb < P::UNIT_KEYS / 16; ++kb) umma_o(d, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb ? true : i >= NS || u > 0);
-          if (!two || (i & 1)) umma_commit(vempty + 8 * st);
-          if (u == P::UNITS - 1) umma_commit(odone + 8 * (i & 1));
+          for (int kb = 0; kb < 4; ++kb) umma_o(d, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb ? true : i >= NS || half > 0);
+          if ((!two || (i & 1)) && (P::UNITS == 2 || half == 1)) umma_commit(vempty + 8 * st);
+          umma_commit(odone + 8 * bar);
         }
         __syncwarp();
       }
@@ -464,7 +472,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       drain(kfull, KST, s_info[8]);
       drain(rfull, P::RAW, s_info[9]);
       drain(sfull, 2, s_issued);
-      drain(odone, 2, o_issued);
+      if (o_issued > 0) drain(odone + 8 * (2 * ((o_issued - 1) & 1) + 1), 1, (o_issued + 1) / 2);
     }
     __syncwarp();
     tc_fence_after();
@@ -655,96 +663,109 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         for (int c = 0; c < 8; ++c) bad |= f[c] < 0.f;
       }
       const bool mask = !__all_sync(0xffffffffu, vis >= base + kKeys) || bad;
-      if (mask) {                                           // bytes behind the last key may be anything, NaN patterns included
+      // One half of the tile's keys (64 scores x with multipliers f of 16 each): probabilities into the columns that the scores
+      // leave.  The exponentials are taken against the reference as it stands; only where they add up to more than f16 may hold
+      // is the half's maximum looked for, the reference moved, O rescaled and the half done again.
+      auto half_tile = [&](uint32_t* x, float* fx, int half) -> bool {
+        if (mask) {                                         // bytes behind the last key may be anything, NaN patterns included
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int n = f[c] < 0.f ? 0 : vis - base - 16 * c;   // keys of these 16 that the row sees
+          for (int c = 0; c < 4; ++c) {
+            const int n = fx[c] < 0.f ? 0 : vis - base - 64 * half - 16 * c;   // keys of these 16 that the row sees
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (e >= n) s[16 * c + e] = 0xFF800000u;
-        }
-      }
-      // ---- maximum ----
-      float tmax = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        f[c] = fmaxf(f[c] * rowmul, 1e-37f);                // never 0: a hidden score times its multiplier stays -inf
-        const uint32_t* x = s + 16 * c;
-        float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
-#pragma unroll
-        for (int e = 2; e < 14; e += 4) {
-          m0 = max3(m0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          m1 = max3(m1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-        }
-        m0 = max3(m0, __uint_as_float(x[14]), __uint_as_float(x[15]));
-        tmax = fmaxf(tmax, fmaxf(m0, m1) * f[c]);
-      }
-      // ---- the reference moves when a tile exceeds it by more than kTauP ----
-      float alpha = 1.f;
-      if (tmax > m + kTauP || m == -INFINITY) {
-        alpha = m == -INFINITY ? 0.f : ex2(m - tmax);
-        m = tmax;
-        l *= alpha;
-      }
-      if (i >= NS && __any_sync(0xffffffffu, alpha != 1.f)) {
-        if (NS == 1) {                                      // the product of the tile before (two groups: complete, since these scores are)
-          alive = wait_for(odone + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1, gave_up, p.status);
-          if (!alive) break;
-          tc_fence_after();
-        }
-        const uint32_t to = tmem + lane_base + 256u + (uint32_t)grp * 128u;
-#pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t x[16];
-          tmem_ld16(to + 16 * c, x);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-          tmem_st16_nowait(to + 16 * c, x);
-        }
-      }
-      // ---- probabilities, into the columns that the scores leave ----
-      const float mb = kBitsP - (m == -INFINITY ? 0.f : m);
-      const unsigned long long mb2 = pair2(mb, mb);
-      unsigned long long sum0 = 0ull, sum1 = 0ull;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const unsigned long long f2 = pair2(f[2 * c + (e >> 4)], f[2 * c + (e >> 4)]);
-          float x0, x1, x2, x3;
-          split2(fma2(pair2(__uint_as_float(s[32 * c + e]), __uint_as_float(s[32 * c + e + 1])), f2, mb2), x0, x1);
-          split2(fma2(pair2(__uint_as_float(s[32 * c + e + 2]), __uint_as_float(s[32 * c + e + 3])), f2, mb2), x2, x3);
-          x0 = ex2(x0); x1 = ex2(x1);
-          if ((e / 4) % kPolyEvery == kPolyEvery - 1) {     // a share of them on the FMA pipe
-            ex2_pair(x2, x3);
-          } else {
-            x2 = ex2(x2); x3 = ex2(x3);
+            for (int e = 0; e < 16; ++e)
+              if (e >= n) x[16 * c + e] = 0xFF800000u;
           }
-          sum0 = add2(sum0, pair2(x0, x1));
-          sum1 = add2(sum1, pair2(x2, x3));
-          const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
-          pk[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-          pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
-        tmem_st16_nowait(ts + 16 * c, pk);
-      }
-      {
-        float x, y;
-        split2(add2(sum0, sum1), x, y);
-        l += x + y;
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pfull + 8 * (i & 1));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) fx[c] = fmaxf(fx[c] * rowmul, 1e-37f);   // never 0: a hidden score times its multiplier stays -inf
+        bool move = __any_sync(0xffffffffu, m == -INFINITY);
+        for (;;) {
+          if (move) {
+            float tmax = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float mx = __uint_as_float(x[16 * c]);
+#pragma unroll
+              for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(x[16 * c + e]), __uint_as_float(x[16 * c + e + 1]));
+              tmax = fmaxf(tmax, fmaxf(mx, __uint_as_float(x[16 * c + 15])) * fx[c]);
+            }
+            float alpha = 1.f;
+            if (tmax > m) {
+              alpha = m == -INFINITY ? 0.f : ex2(m - tmax);
+              m = tmax;
+              l *= alpha;
+            }
+            if (i >= NS || half) {                          // O has something in it: its last product has to be over
+              if (half) {
+                if (!wait_for(odone + 8 * (2 * (i & 1)), (i >> 1) & 1, gave_up, p.status)) return false;
+              } else if (NS == 1) {                         // (two groups: over, since these scores are there)
+                if (!wait_for(odone + 8 * (2 * ((i - 1) & 1) + 1), ((i - 1) >> 1) & 1, gave_up, p.status)) return false;
+              }
+              __syncwarp();
+              tc_fence_after();
+              const uint32_t to = tmem + lane_base + 256u + (uint32_t)grp * 128u;
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(to + 16 * c, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st16_nowait(to + 16 * c, o);
+              }
+            }
+          }
+          const float mb = kBitsP - (m == -INFINITY ? 0.f : m);
+          const unsigned long long mb2 = pair2(mb, mb);
+          unsigned long long sum0 = 0ull, sum1 = 0ull;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float fe = fx[2 * c + (e >> 4)];
+              const unsigned long long f2 = pair2(fe, fe);
+              float x0, x1, x2, x3;
+              split2(fma2(pair2(__uint_as_float(x[32 * c + e]), __uint_as_float(x[32 * c + e + 1])), f2, mb2), x0, x1);
+              split2(fma2(pair2(__uint_as_float(x[32 * c + e + 2]), __uint_as_float(x[32 * c + e + 3])), f2, mb2), x2, x3);
+              x0 = ex2(x0); x1 = ex2(x1);
+              if ((e / 4) % kPolyEvery == kPolyEvery - 1) { // a share of them on the FMA pipe
+                ex2_pair(x2, x3);
+              } else {
+                x2 = ex2(x2); x3 = ex2(x3);
+              }
+              sum0 = add2(sum0, pair2(x0, x1));
+              sum1 = add2(sum1, pair2(x2, x3));
+              const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
+              pk[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+              pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+            }
+            tmem_st16_nowait(ts + 32 * half + 16 * c, pk);
+          }
+          float u, w;
+          split2(add2(sum0, sum1), u, w);
+          u += w;
+          if (!move && __any_sync(0xffffffffu, u > kMostP)) {
+            move = true;
+            continue;
+          }
+          l += u;
+          break;
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull + 8 * (2 * (i & 1) + half));
+        return true;
+      };
+      alive = half_tile(s, f, 0);
+      if (alive) alive = half_tile(s + 64, f + 4, 1);
     }
 
     // ---- the end: this group's last product ----
     const int mine = (items - grp + NS - 1) / NS;           // items of this group
     if (alive && mine > 0) {
       const int il = grp + (mine - 1) * NS;
-      alive = wait_for(odone + 8 * (il & 1), (il >> 1) & 1, gave_up, p.status);
+      alive = wait_for(odone + 8 * (2 * (il & 1) + 1), (il >> 1) & 1, gave_up, p.status);
       __syncwarp();
       tc_fence_after();
     }
