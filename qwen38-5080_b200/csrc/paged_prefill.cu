@@ -39,7 +39,7 @@ constexpr int kInfo = 8;                   // tiles whose scales are in flight
 constexpr int kVRing = 2;                  // V units of 32 KB in f16
 constexpr int kUnitBytes = 32768;
 constexpr float kBitsP = 4.f, kMostP = 61440.f;   // p is held times 2^4 in f16; what 64 keys may add up to before the reference moves
-constexpr int kPolyEvery = 2;              // of 8 exponentials, 2 by polynomial (of 4 kPolyEvery)
+constexpr int kPolyEvery = 2;              // of every 4 * kPolyEvery exponentials, two by polynomial
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
 
 struct PrefillParams {
@@ -139,19 +139,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {  
       : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : B200_R32(r)::"memory"); }
-// A row's 128 scores (loads and the wait for them in one statement: the registers are not touched before it is over).
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+// 64 scores of a row (the load and the wait for it in one statement: the registers are not touched before it is over).
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
       "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%128];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
-      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
-      "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
-      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129];\n\t"
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -160,23 +155,39 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
         "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
         "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
         "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-      : "r"(taddr), "r"(taddr + 64u) : "memory");
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32_nowait(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// 32 bytes, one full sector, in one store.
+__device__ __forceinline__ void stg256(void* dst, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+// try_wait that may suspend the warp for up to a millisecond: a waiting warp that polls takes issue slots from the others.
+__device__ __forceinline__ bool try_wait_long(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
+  return ok != 0;
 }
 // Bounded wait without a call: functions that are called would have to fit the registers of the warps that gave theirs up.
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
 #pragma unroll 1
-  while (!mbar_try_wait(bar, parity)) {
+  while (!try_wait_long(bar, parity)) {
     if (*gave_up) return false;
     if (global_timer_ns() - t0 > kWaitBudgetNs) {
       *gave_up = 1;
@@ -224,14 +235,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
   const PagedGeometry& g = p.g;
   const int G = g.group;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  // Through a shuffle, so that the compiler knows that it is the same in all lanes: roles branch without divergence, and what
+  // they compute for all lanes (loop counters, descriptors) stays in uniform registers.
+  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+  const int warp = uniform(tid >> 5);
 
   __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 2 * P::RAW + 10];
   // each 16 keys of a tile: K scale (-1: no such page), V scale, page (-1: none)
   __shared__ __align__(16) float s_ks[kInfo][8], s_vs[kInfo][8];
   __shared__ __align__(16) int s_id[kInfo][8];
   __shared__ float s_red[4];
-  __shared__ float s_ml[2][2][kRows], s_amax[2][kRows];
+  __shared__ float s_ml[2][2][kRows], s_rowmul[NS][kRows];
   __shared__ int s_info[10];   // [0] sequence [1] tile of it [2] gave up [3] tensor memory [4] last [5] first row [6] rows [7] length [8] K tiles, [9] V units issued
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -287,12 +302,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     s_info[2] = 0;
   }
   __syncthreads();
-  const int b = s_info[0];
+  const int b = uniform(s_info[0]);
   if (b < 0) return;                                        // the grid is an upper bound
-  const int q0 = s_info[5], nq = s_info[6];
-  const int first_tok = s_info[1] * per_block, ntok = min(per_block, nq - first_tok);
+  const int q0 = uniform(s_info[5]), nq = uniform(s_info[6]);
+  const int first_tok = uniform(s_info[1]) * per_block, ntok = min(per_block, nq - first_tok);
   const bool two = NS == 2 && ntok > per_tile;              // two query tiles, one for each softmax group; else they share one
-  const int len = paged_len(g, s_info[7], p.status, tid == 0 && layer == 0 && h == 0 && piece == 0);
+  const int len = paged_len(g, uniform(s_info[7]), p.status, tid == 0 && layer == 0 && h == 0 && piece == 0);
   const int visible = p.causal ? min(len, max(0, len - nq + first_tok + ntok)) : len;   // of the tile's last token
   const int all_tiles = (visible + kKeys - 1) / kKeys;
   const int per_piece = (all_tiles + p.splits - 1) / p.splits;
@@ -404,60 +419,74 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   } else if (warp == kMma) {
     // ================= products =================
     tmem_alloc(smem_u32(s_info + 3), 512);                  // used by others only after this warp's first product
-    int s_issued = 0, o_issued = 0;
-    bool ok = wait_for(qready, 0, gave_up, p.status);
+    wait_for(qready, 0, gave_up, p.status);
+    __syncwarp();
     const uint32_t lowQ = (sQ >> 4) | (1u << 16), lowK = (sK >> 4) | (1u << 16), lowV = (sV >> 4) | ((uint32_t)(P::UNIT_KEYS * 128 >> 4) << 16);
-    // Products in the order of items: item i works in score buffer i & 1.  One query tile: item = key tile.  Two: items 2 t and
-    // 2 t + 1 are key tile t for the first and the second query tile.
-    const int items = two ? 2 * nt : nt, sh = two ? 1 : 0;
-    auto issue_s = [&](int i) {
-      const int t = i >> sh, st = t % KST;
-      if (!wait_for(kfull + 8 * st, (t / KST) & 1, gave_up, p.status)) return false;
-      __syncwarp();
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t d = tmem + (uint32_t)(i & 1) * 128u;
-        const uint32_t qa = lowQ + (two ? (uint32_t)(i & 1) * (P::QTILE >> 4) : 0u), kb0 = lowK + (uint32_t)st * (P::KTILE >> 4);
+    // One lane runs the whole loop.  What stands between two products leaves the tensor cores idle, so nothing is waited for twice
+    // and a wait that ran out is only looked at by the waits that follow (they return at once; the results go nowhere).
+    // Item n of a group is its n-th key tile: with two query tiles every key tile is one of both groups, with one the groups take
+    // them in turn; heads of 256 have one group and use the two score buffers in turn.
+    if (elect_one()) {
+      auto issue_s = [&](int t, int buf, uint32_t qa, bool wait_k, bool last) {
+        const int st = t % KST;
+        if (wait_k) wait_for(kfull + 8 * st, (t / KST) & 1, gave_up, p.status);
+        tc_fence_after();
+        const uint32_t kb0 = lowK + (uint32_t)st * (P::KTILE >> 4);
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int hf = 0; hf < DH; ++hf)
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
-              umma_s(d, qa + (term * DH + hf) * (kRows * 128 >> 4) + kb * 2, kb0 + hf * (kKeys * 128 >> 4) + kb * 2, kIdescS, (term | hf | kb) != 0);
-        umma_commit(sfull + 8 * (i & 1));
-        if (!two || (i & 1)) umma_commit(kempty + 8 * st);
-      }
-      __syncwarp();
-      ++s_issued;
-      return true;
-    };
-    ok = ok && issue_s(0);
-    if (items > 1) ok = ok && issue_s(1);
-    for (int i = 0; i < items && ok; ++i) {
-      // keys 0..63 of the tile, then 64..127: the first half is multiplied while the second half's exponentials are taken
-#pragma unroll 1
-      for (int half = 0; half < 2 && ok; ++half) {
-        const int bar = 2 * (i & 1) + half, vu = (i >> sh) * P::UNITS + (P::UNITS == 2 ? half : 0), st = vu % kVRing;
-        ok = wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
-        if (ok) ok = wait_for(pfull + 8 * bar, (i >> 1) & 1, gave_up, p.status);
-        __syncwarp();
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t d = tmem + 256u + (NS == 2 ? (uint32_t)(i & 1) * 128u : 0u);
-          const uint32_t a = tmem + (uint32_t)(i & 1) * 128u + (uint32_t)half * 32u;
+              umma_s(tmem + (uint32_t)buf * 128u, qa + (term * DH + hf) * (kRows * 128 >> 4) + kb * 2, kb0 + hf * (kKeys * 128 >> 4) + kb * 2, kIdescS, (term | hf | kb) != 0);
+        umma_commit(sfull + 8 * buf);
+        if (last) umma_commit(kempty + 8 * st);
+      };
+      auto issue_o = [&](int t, int buf, uint32_t parity, uint32_t d, bool fresh, bool wait_v, bool last) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {              // keys 0..63 of the tile, then 64..127
+          const int vu = t * P::UNITS + (P::UNITS == 2 ? half : 0), st = vu % kVRing;
+          if (wait_v && (P::UNITS == 2 || half == 0)) wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
+          wait_for(pfull + 8 * (2 * buf + half), parity, gave_up, p.status);
+          tc_fence_after();
+          const uint32_t a = tmem + (uint32_t)buf * 128u + (uint32_t)half * 32u;
           const uint32_t v0 = lowV + (uint32_t)st * (kUnitBytes >> 4) + (P::UNITS == 2 ? 0u : (uint32_t)half * (8192 >> 4));
 #pragma unroll
-          for (int kb = 0; kb < 4; ++kb) umma_o(d, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb ? true : i >= NS || half > 0);
-          if ((!two || (i & 1)) && (P::UNITS == 2 || half == 1)) umma_commit(vempty + 8 * st);
-          umma_commit(odone + 8 * bar);
+          for (int kb = 0; kb < 4; ++kb) umma_o(d, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb || half ? true : !fresh);
+          umma_commit(odone + 8 * (2 * buf + half));
+          if (last && (P::UNITS == 2 || half == 1)) umma_commit(vempty + 8 * st);
         }
-        __syncwarp();
+      };
+      const uint32_t q1 = lowQ + (two ? (uint32_t)(P::QTILE >> 4) : 0u);
+      if (NS == 1) {
+        issue_s(0, 0, lowQ, true, true);
+        if (nt > 1) issue_s(1, 1, lowQ, true, true);
+#pragma unroll 1
+        for (int t = 0; t < nt; ++t) {
+          issue_o(t, t & 1, (t >> 1) & 1, tmem + 256u, t == 0, true, true);
+          if (t + 2 < nt) issue_s(t + 2, t & 1, lowQ, true, true);
+        }
+      } else if (two) {
+        issue_s(0, 0, lowQ, true, false);
+        issue_s(0, 1, q1, false, true);
+#pragma unroll 1
+        for (int t = 0; t < nt; ++t) {
+          issue_o(t, 0, t & 1, tmem + 256u, t == 0, true, false);
+          if (t + 1 < nt) issue_s(t + 1, 0, lowQ, true, false);
+          issue_o(t, 1, t & 1, tmem + 384u, t == 0, false, true);
+          if (t + 1 < nt) issue_s(t + 1, 1, q1, false, true);
+        }
+      } else {
+        issue_s(0, 0, lowQ, true, true);
+        if (nt > 1) issue_s(1, 1, lowQ, true, true);
+#pragma unroll 1
+        for (int t = 0; t < nt; ++t) {
+          issue_o(t, t & 1, (t >> 1) & 1, tmem + 256u + (uint32_t)(t & 1) * 128u, t < 2, true, true);
+          if (t + 2 < nt) issue_s(t + 2, t & 1, lowQ, true, true);
+        }
       }
-      if (ok) ++o_issued;
-      if (ok && i + 2 < items) ok = issue_s(i + 2);
     }
+    __syncwarp();
     // every softmax warp has read its output, and the TMA warp has said what it issued
     asm volatile("bar.sync 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
     if (*gave_up && lane == 0) {
@@ -471,8 +500,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       };
       drain(kfull, KST, s_info[8]);
       drain(rfull, P::RAW, s_info[9]);
-      drain(sfull, 2, s_issued);
-      if (o_issued > 0) drain(odone + 8 * (2 * ((o_issued - 1) & 1) + 1), 1, (o_issued + 1) / 2);
+      for (int buf = 0; buf < 2; ++buf) {                   // every product was issued
+        const int n = two ? nt : (nt - buf + 1) >> 1;
+        drain(sfull + 8 * buf, 1, n);
+        drain(odone + 8 * (2 * buf + 1), 1, n);
+      }
     }
     __syncwarp();
     tc_fence_after();
@@ -575,68 +607,66 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     const int tile_tok = two ? grp * per_tile : 0, tok = tile_tok + row / G, head = row % G;
     const bool real = row / G < per_tile && tok < ntok;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint16_t* qrow = p.q + (out_row0 + (long long)tok * g.h_q + head) * D;
     regs_up<P::REGS_SOFTMAX>();
-    // the query row as two e4m3 rows; two groups that share a tile take half of the row's dims each
-    constexpr int NQ = 16, ROUNDS = D / 8 / NQ;             // 16-byte loads at a time
+    regs_up<P::REGS_SOFTMAX>();
+    // The query rows as two e4m3 rows each.  A warp takes 32 rows (16 where two groups share a tile), D / 8 lanes per row, and has
+    // all its loads in flight before it looks at the first; every thread then picks up the multiplier of its own row.
     const bool halves = NS == 2 && !two;
-    const int first = halves ? grp * (NQ / 2) : 0, count = halves ? NQ / 2 : NQ;   // of a round
-    const uint32_t sq = sQ + (two ? grp * P::QTILE : 0);
     float rowmul;
     {
-      uint4 raw[NQ];
-      auto load_q = [&](int round) {
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) raw[i] = real && i < count ? __ldg(reinterpret_cast<const uint4*>(qrow) + round * NQ + first + i) : make_uint4(0, 0, 0, 0);
-      };
-      float amax = 0.f;
+      constexpr int LPR = D / 8, RPL = 32 / LPR, BATCH = 16;  // lanes per row, rows per load, loads in flight
+      const uint32_t sq = sQ + (two ? grp * P::QTILE : 0);
+      float* s_mul = s_rowmul[two ? grp : 0];
+      const int first = halves ? warp * 16 : (warp & 3) * 32, loads = (halves ? 16 : 32) / RPL;
+      const int sub = lane / LPR, c8 = lane % LPR;            // row of the load, 8 dims of it
 #pragma unroll 1
-      for (int round = 0; round < ROUNDS; ++round) {
-        load_q(round);
+      for (int i0 = 0; i0 < loads; i0 += BATCH) {
+        uint4 raw[BATCH];
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) amax = max3(amax, fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xFFFF0000u)));
+        for (int i = 0; i < BATCH; ++i) {
+          const int r = first + (i0 + i) * RPL + sub, t = tile_tok + r / G;
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (i0 + i < loads && r / G < per_tile && t < ntok)
+            raw[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (out_row0 + (long long)t * g.h_q + r % G) * D) + c8);
         }
-      }
-      if (halves) {
-        s_amax[grp][row] = amax;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        amax = fmaxf(s_amax[0][row], s_amax[1][row]);
-      }
-      int ex = (int)((__float_as_uint(amax) >> 23) & 0xFF);
-      ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
-      const float down = __uint_as_float((uint32_t)(261 - ex) << 23), up = __uint_as_float((uint32_t)(ex - 7) << 23);   // largest |q| in [128, 256)
-      rowmul = up * p.score_scale;
-#pragma unroll 1
-      for (int round = 0; round < ROUNDS; ++round) {
-      if (ROUNDS > 1) load_q(round);                        // again, from the caches
 #pragma unroll
-      for (int ci = 0; ci < NQ / 2; ++ci) {                 // 16 dims
-        if (2 * ci >= count) break;
-        const int c = (round * NQ + first) / 2 + ci;
-        uint32_t hi[4], lo[4];
+        for (int i = 0; i < BATCH; ++i) {
+          if (i0 + i < loads) {
+            const int r = first + (i0 + i) * RPL + sub;
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float x[8], amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t w[4] = {raw[2 * ci + i].x, raw[2 * ci + i].y, raw[2 * ci + i].z, raw[2 * ci + i].w};
+            for (int e = 0; e < 4; ++e) {
+              x[2 * e] = __uint_as_float(w[e] << 16);
+              x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+              amax = max3(amax, fabsf(x[2 * e]), fabsf(x[2 * e + 1]));
+            }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x0 = __uint_as_float(w[2 * e] << 16) * down, x1 = __uint_as_float(w[2 * e] & 0xFFFF0000u) * down;
-            const float x2 = __uint_as_float(w[2 * e + 1] << 16) * down, x3 = __uint_as_float(w[2 * e + 1] & 0xFFFF0000u) * down;
-            const float h0 = e4m3_head(x0), h1 = e4m3_head(x1), h2 = e4m3_head(x2), h3 = e4m3_head(x3);
-            hi[2 * i + e] = pack_e4m3x2(h0, h1) | (pack_e4m3x2(h2, h3) << 16);
-            lo[2 * i + e] = pack_e4m3x2(x0 - h0, x1 - h1) | (pack_e4m3x2(x2 - h2, x3 - h3) << 16);
+            for (int off = LPR / 2; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+            int ex = (int)((__float_as_uint(amax) >> 23) & 0xFF);
+            ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
+            const float down = __uint_as_float((uint32_t)(261 - ex) << 23);   // brings the largest |q| into [128, 256)
+            if (c8 == 0) s_mul[r] = __uint_as_float((uint32_t)(ex - 7) << 23) * p.score_scale;
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float x0 = x[4 * e] * down, x1 = x[4 * e + 1] * down, x2 = x[4 * e + 2] * down, x3 = x[4 * e + 3] * down;
+              const float h0 = e4m3_head(x0), h1 = e4m3_head(x1), h2 = e4m3_head(x2), h3 = e4m3_head(x3);
+              hi[e] = pack_e4m3x2(h0, h1) | (pack_e4m3x2(h2, h3) << 16);
+              lo[e] = pack_e4m3x2(x0 - h0, x1 - h1) | (pack_e4m3x2(x2 - h2, x3 - h3) << 16);
+            }
+            const int c = c8 >> 1;                            // 16-byte chunk of the row
+            const uint32_t off = (uint32_t)(c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c8 & 1) * 8;
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(sq + off), "r"(hi[0]), "r"(hi[1]) : "memory");
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(sq + DH * kRows * 128 + off), "r"(lo[0]), "r"(lo[1]) : "memory");
           }
         }
-        const uint32_t off = (uint32_t)(c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        sts128(sq + off, hi[0], hi[1], hi[2], hi[3]);
-        sts128(sq + DH * kRows * 128 + off, lo[0], lo[1], lo[2], lo[3]);
-      }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(qready);
+      if (halves) asm volatile("bar.sync 1, 256;" ::: "memory");
+      rowmul = s_mul[row];
     }
     // keys this row sees; rows of no token see all of them (their results go nowhere, and they need no mask)
     const int vis = !real ? 0x7fffffff : p.causal ? min(len, max(0, len - nq + first_tok + tok + 1)) : len;
@@ -652,113 +682,98 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       if (!alive) break;
       tc_fence_after();
       const uint32_t ts = tmem + lane_base + (uint32_t)(i & 1) * 128u;
-      uint32_t s[128];
-      tmem_ld128(ts, s);
-      float f[8];                                           // score multipliers of 16 keys each
-      bool bad = false;
-      {
-        const float4 x = *reinterpret_cast<const float4*>(s_ks[j % kInfo]), y = *reinterpret_cast<const float4*>(s_ks[j % kInfo] + 4);
-        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) bad |= f[c] < 0.f;
-      }
-      const bool mask = !__all_sync(0xffffffffu, vis >= base + kKeys) || bad;
-      // One half of the tile's keys (64 scores x with multipliers f of 16 each): probabilities into the columns that the scores
-      // leave.  The exponentials are taken against the reference as it stands; only where they add up to more than f16 may hold
-      // is the half's maximum looked for, the reference moved, O rescaled and the half done again.
-      auto half_tile = [&](uint32_t* x, float* fx, int half) -> bool {
-        if (mask) {                                         // bytes behind the last key may be anything, NaN patterns included
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int n = fx[c] < 0.f ? 0 : vis - base - 64 * half - 16 * c;   // keys of these 16 that the row sees
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (e >= n) x[16 * c + e] = 0xFF800000u;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) fx[c] = fmaxf(fx[c] * rowmul, 1e-37f);   // never 0: a hidden score times its multiplier stays -inf
-        bool move = __any_sync(0xffffffffu, m == -INFINITY);
-        for (;;) {
-          if (move) {
-            float tmax = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float mx = __uint_as_float(x[16 * c]);
-#pragma unroll
-              for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(x[16 * c + e]), __uint_as_float(x[16 * c + e + 1]));
-              tmax = fmaxf(tmax, fmaxf(mx, __uint_as_float(x[16 * c + 15])) * fx[c]);
-            }
-            float alpha = 1.f;
-            if (tmax > m) {
-              alpha = m == -INFINITY ? 0.f : ex2(m - tmax);
-              m = tmax;
-              l *= alpha;
-            }
-            if (i >= NS || half) {                          // O has something in it: its last product has to be over
-              if (half) {
-                if (!wait_for(odone + 8 * (2 * (i & 1)), (i >> 1) & 1, gave_up, p.status)) return false;
-              } else if (NS == 1) {                         // (two groups: over, since these scores are there)
-                if (!wait_for(odone + 8 * (2 * ((i - 1) & 1) + 1), ((i - 1) >> 1) & 1, gave_up, p.status)) return false;
-              }
-              __syncwarp();
-              tc_fence_after();
-              const uint32_t to = tmem + lane_base + 256u + (uint32_t)grp * 128u;
+      const bool open = __all_sync(0xffffffffu, vis >= base + kKeys);   // no row of the warp has a hidden key in the tile
 #pragma unroll 1
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t o[16];
-                tmem_ld16(to + 16 * c, o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                tmem_st16_nowait(to + 16 * c, o);
-              }
-            }
-          }
+      for (int part = 0; part < 2; ++part) {                // 64 keys at a time
+        const float4 ks = *reinterpret_cast<const float4*>(s_ks[j % kInfo] + 4 * part);
+        const bool bad = fminf(fminf(ks.x, ks.y), fminf(ks.z, ks.w)) < 0.f;   // a page that does not exist
+        // multipliers of 16 scores each; never 0: a hidden score (-inf) times its multiplier stays -inf
+        const float f[4] = {fmaxf(ks.x * rowmul, 1e-37f), fmaxf(ks.y * rowmul, 1e-37f), fmaxf(ks.z * rowmul, 1e-37f), fmaxf(ks.w * rowmul, 1e-37f)};
+        const uint32_t ss = ts + 64u * part;
+        uint32_t x[64], pk[32];
+        float u;
+        // Exponentials against the reference as it stands; their sum tells whether f16 can hold them.
+        auto exponentials = [&]() {
           const float mb = kBitsP - (m == -INFINITY ? 0.f : m);
           const unsigned long long mb2 = pair2(mb, mb);
           unsigned long long sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float fe = fx[2 * c + (e >> 4)];
-              const unsigned long long f2 = pair2(fe, fe);
-              float x0, x1, x2, x3;
-              split2(fma2(pair2(__uint_as_float(x[32 * c + e]), __uint_as_float(x[32 * c + e + 1])), f2, mb2), x0, x1);
-              split2(fma2(pair2(__uint_as_float(x[32 * c + e + 2]), __uint_as_float(x[32 * c + e + 3])), f2, mb2), x2, x3);
-              x0 = ex2(x0); x1 = ex2(x1);
-              if ((e / 4) % kPolyEvery == kPolyEvery - 1) { // a share of them on the FMA pipe
-                ex2_pair(x2, x3);
-              } else {
-                x2 = ex2(x2); x3 = ex2(x3);
-              }
-              sum0 = add2(sum0, pair2(x0, x1));
-              sum1 = add2(sum1, pair2(x2, x3));
-              const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
-              pk[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-              pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          for (int e = 0; e < 64; e += 4) {
+            const unsigned long long f2 = pair2(f[e >> 4], f[e >> 4]);
+            float x0, x1, x2, x3;
+            split2(fma2(pair2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, mb2), x0, x1);
+            split2(fma2(pair2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), f2, mb2), x2, x3);
+            x0 = ex2(x0); x1 = ex2(x1);
+            if ((e / 4) % kPolyEvery == kPolyEvery - 1) {     // a share of them on the FMA pipe
+              ex2_pair(x2, x3);
+            } else {
+              x2 = ex2(x2); x3 = ex2(x3);
             }
-            tmem_st16_nowait(ts + 32 * half + 16 * c, pk);
+            sum0 = add2(sum0, pair2(x0, x1));
+            sum1 = add2(sum1, pair2(x2, x3));
+            const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
+            pk[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+            pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
           }
-          float u, w;
-          split2(add2(sum0, sum1), u, w);
-          u += w;
-          if (!move && __any_sync(0xffffffffu, u > kMostP)) {
-            move = true;
-            continue;
-          }
-          l += u;
-          break;
+          float v, w;
+          split2(add2(sum0, sum1), v, w);
+          u = v + w;
+        };
+        bool fits = open && !bad && !__any_sync(0xffffffffu, m == -INFINITY);
+        if (fits) {
+          tmem_ld64(ss, x);
+          exponentials();
+          fits = !__any_sync(0xffffffffu, u > kMostP);
         }
+        if (!fits) {
+          // Hidden keys, no reference yet, or exponentials too large: the scores again, hidden ones out, the reference to their
+          // maximum if that is larger, and what O and the sum hold so far rescaled to it.
+          tmem_ld64(ss, x);
+          float tmax = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float kc = c == 0 ? ks.x : c == 1 ? ks.y : c == 2 ? ks.z : ks.w;
+            const int seen = kc < 0.f ? 0 : vis - base - 64 * part - 16 * c;   // keys of these 16 that the row sees
+            float mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              if (e >= seen) x[16 * c + e] = 0xFF800000u;   // whatever the bytes there gave, NaN included
+              mx = fmaxf(mx, __uint_as_float(x[16 * c + e]));
+            }
+            tmax = fmaxf(tmax, mx * f[c]);
+          }
+          float alpha = 1.f;
+          if (tmax > m) {
+            alpha = m == -INFINITY ? 0.f : ex2(m - tmax);
+            m = tmax;
+            l *= alpha;
+          }
+          if ((i >= NS || part) && __any_sync(0xffffffffu, alpha != 1.f)) {   // O has something in it: its last product has to be over
+            if (part) alive = wait_for(odone + 8 * (2 * (i & 1)), (i >> 1) & 1, gave_up, p.status);
+            else if (NS == 1) alive = wait_for(odone + 8 * (2 * ((i - 1) & 1) + 1), ((i - 1) >> 1) & 1, gave_up, p.status);   // (two groups: over, since these scores are there)
+            __syncwarp();
+            if (!alive) break;
+            tc_fence_after();
+            const uint32_t to = tmem + lane_base + 256u + (uint32_t)grp * 128u;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(to + 16 * c, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16_nowait(to + 16 * c, o);
+            }
+          }
+          exponentials();
+        }
+        l += u;
+        // into the columns that the scores leave
+        tmem_st32_nowait(ts + 32u * part, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pfull + 8 * (2 * (i & 1) + half));
-        return true;
-      };
-      alive = half_tile(s, f, 0);
-      if (alive) alive = half_tile(s + 64, f + 4, 1);
+        if (lane == 0) mbar_arrive(pfull + 8 * (2 * (i & 1) + part));
+      }
     }
 
     // ---- the end: this group's last product ----
@@ -806,16 +821,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           for (int i = 0; i < 32; ++i) o[i] += f1 == 0.f ? 0.f : __uint_as_float(x[i]) * f1;
         }
         if (real && pieces == 1) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + (out_row0 + (long long)tok * g.h_q + head) * D + 32 * c);
+          uint16_t* dst = p.out + (out_row0 + (long long)tok * g.h_q + head) * D + 32 * c;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+          for (int i = 0; i < 2; ++i) {
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 v2 = __floats2bfloat162_rn(o[8 * i + 2 * e] * scale, o[8 * i + 2 * e + 1] * scale);
+            for (int e = 0; e < 8; ++e) {
+              const __nv_bfloat162 v2 = __floats2bfloat162_rn(o[16 * i + 2 * e] * scale, o[16 * i + 2 * e + 1] * scale);
               w[e] = *reinterpret_cast<const uint32_t*>(&v2);
             }
-            dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            stg256(dst + 16 * i, w);
           }
         } else if (real) {
           float4* dst = reinterpret_cast<float4*>(part + (long long)row * D + 32 * c);
