@@ -14,12 +14,13 @@
 //     exponentials are taken against the reference maximum as it stands, without looking for the tile's maximum first; a
 //     p far beyond it shows in the sum, and only then the reference moves and O is rescaled.  f16 holds 2^12 above the
 //     reference and 2^28 below it, sums and O are fp32: nothing is lost by a reference that is not the maximum.
-//   * a tile's P is handed over in halves, so that the first is multiplied while the second's exponentials are taken.
+//   * P is handed over 64 keys at a time, so that they are multiplied while the next exponentials are taken; with heads of 128
+//     each 64 keys' scores have a buffer of their own, refilled as soon as their P is multiplied.
 //   * heads of 128: two groups of softmax warps, each with its own S, P and O.  With rows enough a block takes two query tiles,
 //     one for each group, which share the K copies and the V conversion; otherwise the groups take alternate key tiles of
 //     one query tile, joined at the end.  Heads of 256: one group (O fills the tensor memory, and the products take twice as
 //     long per tile).
-// Tensor memory: S0 S1 at columns 0 and 128, O at 256 (two of 128 columns, or one of 256).
+// Tensor memory: S at columns 0..255 (two of 128, or four of 64), O at 256 (one of 256 columns, or two of 128).
 //
 // Bound: the tensor cores (4 D flops per row, key and head), and as much the exponentials, one per row and key:
 // 16 a cycle per SM make 1024 cycles a tile, the products of a 128-wide head 1048.
@@ -39,7 +40,7 @@ constexpr int kInfo = 8;                   // tiles whose scales are in flight
 constexpr int kVRing = 2;                  // V units of 32 KB in f16
 constexpr int kUnitBytes = 32768;
 constexpr float kBitsP = 4.f, kMostP = 61440.f;   // p is held times 2^4 in f16; what 64 keys may add up to before the reference moves
-constexpr int kPolyEvery = 2;              // of every 4 * kPolyEvery exponentials, two by polynomial
+constexpr int kPolyEvery = 4;              // of every 4 * kPolyEvery exponentials, two by polynomial
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
 
 struct PrefillParams {
@@ -61,6 +62,7 @@ struct PrefillPlan {
   static constexpr int NS = D == 128 ? 2 : 1;              // softmax groups
   static constexpr int KST = D == 128 ? 3 : 2;             // K tiles in flight
   static constexpr int KTILE = kKeys * D;
+  static constexpr int SK = D == 128 ? 64 : 128;           // keys of a score buffer; every group has two buffers
   static constexpr int UNIT_KEYS = kUnitBytes / (2 * D);   // keys of a V unit
   static constexpr int UNITS = kKeys / UNIT_KEYS;          // V units of a tile
   static constexpr int RAW = 2;                            // V units in flight as bytes
@@ -231,7 +233,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   constexpr int DH = P::DH, NS = P::NS, KST = P::KST;
   constexpr int kSoftmaxWarps = 4 * NS, kFirstV = kSoftmaxWarps, kTma = kSoftmaxWarps + 4, kMma = kSoftmaxWarps + 5;
   // D f32, A and B e4m3, both K-major, N = 128 keys, M = 128;   D f32, A f16 in tensor memory, B f16 MN-major, N = D, M = 128
-  constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  constexpr uint32_t kIdescS = (1u << 4) | (((uint32_t)P::SK >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
   const PagedGeometry& g = p.g;
   const int G = g.group;
@@ -241,7 +243,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
   const int warp = uniform(tid >> 5);
 
-  __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 2 * P::RAW + 10];
+  __shared__ __align__(8) uint64_t bars[1 + 2 * KST + kInfo + 2 * kVRing + 2 * P::RAW + 2 * NS + 8];
   // each 16 keys of a tile: K scale (-1: no such page), V scale, page (-1: none)
   __shared__ __align__(16) float s_ks[kInfo][8], s_vs[kInfo][8];
   __shared__ __align__(16) int s_id[kInfo][8];
@@ -253,7 +255,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const uint32_t sQ = smem0, sK = sQ + NS * P::QTILE, sV = sK + KST * P::KTILE, sRaw = sV + kVRing * kUnitBytes;
   const uint32_t qready = smem_u32(bars), kfull = qready + 8, kempty = kfull + 8 * KST, kinfo = kempty + 8 * KST;
   const uint32_t vfull = kinfo + 8 * kInfo, vempty = vfull + 8 * kVRing;
-  const uint32_t sfull = vempty + 8 * kVRing, pfull = sfull + 16, odone = pfull + 32;   // of both halves of both buffers
+  const uint32_t sfull = vempty + 8 * kVRing, pfull = sfull + 16 * NS, odone = pfull + 32;   // of both halves of both buffers
   const uint32_t rfull = odone + 32, rempty = rfull + 8 * P::RAW;
   volatile int* gave_up = s_info + 2;
 
@@ -295,7 +297,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     for (int i = 0; i < kInfo; ++i) mbar_init(kinfo + 8 * i, 1);
     for (int i = 0; i < kVRing; ++i) { mbar_init(vfull + 8 * i, 4); mbar_init(vempty + 8 * i, 1); }
     for (int i = 0; i < P::RAW; ++i) { mbar_init(rfull + 8 * i, 1); mbar_init(rempty + 8 * i, 4); }
-    for (int i = 0; i < 2; ++i) mbar_init(sfull + 8 * i, 1);
+    for (int i = 0; i < 2 * NS; ++i) mbar_init(sfull + 8 * i, 1);
     for (int i = 0; i < 4; ++i) { mbar_init(pfull + 8 * i, 4); mbar_init(odone + 8 * i, 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -427,62 +429,72 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // Item n of a group is its n-th key tile: with two query tiles every key tile is one of both groups, with one the groups take
     // them in turn; heads of 256 have one group and use the two score buffers in turn.
     if (elect_one()) {
-      auto issue_s = [&](int t, int buf, uint32_t qa, bool wait_k, bool last) {
+      // keys [64 sub, 64 sub + 64) of tile t (heads of 128) or all of it
+      auto issue_s = [&](int t, int sub, int grp, int buf, uint32_t qa, bool wait_k, bool last) {
         const int st = t % KST;
         if (wait_k) wait_for(kfull + 8 * st, (t / KST) & 1, gave_up, p.status);
         tc_fence_after();
-        const uint32_t kb0 = lowK + (uint32_t)st * (P::KTILE >> 4);
+        const uint32_t kb0 = lowK + (uint32_t)st * (P::KTILE >> 4) + (uint32_t)sub * (8192 >> 4);
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int hf = 0; hf < DH; ++hf)
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
-              umma_s(tmem + (uint32_t)buf * 128u, qa + (term * DH + hf) * (kRows * 128 >> 4) + kb * 2, kb0 + hf * (kKeys * 128 >> 4) + kb * 2, kIdescS, (term | hf | kb) != 0);
-        umma_commit(sfull + 8 * buf);
+              umma_s(tmem + (uint32_t)(grp * 128 + buf * P::SK), qa + (term * DH + hf) * (kRows * 128 >> 4) + kb * 2, kb0 + hf * (kKeys * 128 >> 4) + kb * 2, kIdescS, (term | hf | kb) != 0);
+        umma_commit(sfull + 8 * (2 * grp + buf));
         if (last) umma_commit(kempty + 8 * st);
       };
-      auto issue_o = [&](int t, int buf, uint32_t parity, uint32_t d, bool fresh, bool wait_v, bool last) {
+      auto issue_o = [&](int t, int half, int grp, uint32_t a, int bar, uint32_t parity, bool fresh, bool wait_v, bool last) {
+        const int vu = t * P::UNITS + (P::UNITS == 2 ? half : 0), st = vu % kVRing;
+        if (wait_v) wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
+        wait_for(pfull + 8 * bar, parity, gave_up, p.status);
+        tc_fence_after();
+        const uint32_t v0 = lowV + (uint32_t)st * (kUnitBytes >> 4) + (P::UNITS == 2 ? 0u : (uint32_t)half * (8192 >> 4));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {              // keys 0..63 of the tile, then 64..127
-          const int vu = t * P::UNITS + (P::UNITS == 2 ? half : 0), st = vu % kVRing;
-          if (wait_v && (P::UNITS == 2 || half == 0)) wait_for(vfull + 8 * st, (vu / kVRing) & 1, gave_up, p.status);
-          wait_for(pfull + 8 * (2 * buf + half), parity, gave_up, p.status);
-          tc_fence_after();
-          const uint32_t a = tmem + (uint32_t)buf * 128u + (uint32_t)half * 32u;
-          const uint32_t v0 = lowV + (uint32_t)st * (kUnitBytes >> 4) + (P::UNITS == 2 ? 0u : (uint32_t)half * (8192 >> 4));
-#pragma unroll
-          for (int kb = 0; kb < 4; ++kb) umma_o(d, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb || half ? true : !fresh);
-          umma_commit(odone + 8 * (2 * buf + half));
-          if (last && (P::UNITS == 2 || half == 1)) umma_commit(vempty + 8 * st);
-        }
+        for (int kb = 0; kb < 4; ++kb) umma_o(tmem + 256u + (uint32_t)grp * 128u, a + kb * 8, v0 + kb * (2048 >> 4), kIdescO, kb ? true : !fresh);
+        umma_commit(odone + 8 * bar);
+        if (last) umma_commit(vempty + 8 * st);
       };
       const uint32_t q1 = lowQ + (two ? (uint32_t)(P::QTILE >> 4) : 0u);
       if (NS == 1) {
-        issue_s(0, 0, lowQ, true, true);
-        if (nt > 1) issue_s(1, 1, lowQ, true, true);
+        issue_s(0, 0, 0, 0, lowQ, true, true);
+        if (nt > 1) issue_s(1, 0, 0, 1, lowQ, true, true);
 #pragma unroll 1
         for (int t = 0; t < nt; ++t) {
-          issue_o(t, t & 1, (t >> 1) & 1, tmem + 256u, t == 0, true, true);
-          if (t + 2 < nt) issue_s(t + 2, t & 1, lowQ, true, true);
+          const int buf = t & 1;
+          issue_o(t, 0, 0, tmem + buf * 128u, 2 * buf, (t >> 1) & 1, t == 0, true, true);
+          issue_o(t, 1, 0, tmem + buf * 128u + 32u, 2 * buf + 1, (t >> 1) & 1, false, true, true);
+          if (t + 2 < nt) issue_s(t + 2, 0, 0, buf, lowQ, true, true);
         }
       } else if (two) {
-        issue_s(0, 0, lowQ, true, false);
-        issue_s(0, 1, q1, false, true);
+        issue_s(0, 0, 0, 0, lowQ, true, false);
+        issue_s(0, 0, 1, 0, q1, false, false);
+        issue_s(0, 1, 0, 1, lowQ, false, false);
+        issue_s(0, 1, 1, 1, q1, false, true);
 #pragma unroll 1
         for (int t = 0; t < nt; ++t) {
-          issue_o(t, 0, t & 1, tmem + 256u, t == 0, true, false);
-          if (t + 1 < nt) issue_s(t + 1, 0, lowQ, true, false);
-          issue_o(t, 1, t & 1, tmem + 384u, t == 0, false, true);
-          if (t + 1 < nt) issue_s(t + 1, 1, q1, false, true);
+          const bool more = t + 1 < nt;
+          issue_o(t, 0, 0, tmem, 0, t & 1, t == 0, true, false);
+          if (more) issue_s(t + 1, 0, 0, 0, lowQ, true, false);
+          issue_o(t, 0, 1, tmem + 128u, 2, t & 1, t == 0, false, false);
+          if (more) issue_s(t + 1, 0, 1, 0, q1, false, false);
+          issue_o(t, 1, 0, tmem + 64u, 1, t & 1, false, false, false);
+          if (more) issue_s(t + 1, 1, 0, 1, lowQ, false, false);
+          issue_o(t, 1, 1, tmem + 192u, 3, t & 1, false, false, true);
+          if (more) issue_s(t + 1, 1, 1, 1, q1, false, true);
         }
       } else {
-        issue_s(0, 0, lowQ, true, true);
-        if (nt > 1) issue_s(1, 1, lowQ, true, true);
+        for (int grp = 0; grp < 2; ++grp)
+          if (grp < nt) { issue_s(grp, 0, grp, 0, lowQ, true, false); issue_s(grp, 1, grp, 1, lowQ, false, true); }
 #pragma unroll 1
         for (int t = 0; t < nt; ++t) {
-          issue_o(t, t & 1, (t >> 1) & 1, tmem + 256u + (uint32_t)(t & 1) * 128u, t < 2, true, true);
-          if (t + 2 < nt) issue_s(t + 2, t & 1, lowQ, true, true);
+          const int grp = t & 1;
+          const bool more = t + 2 < nt;
+          issue_o(t, 0, grp, tmem + grp * 128u, 2 * grp, (t >> 1) & 1, t < 2, true, false);
+          if (more) issue_s(t + 2, 0, grp, 0, lowQ, true, false);
+          issue_o(t, 1, grp, tmem + grp * 128u + 64u, 2 * grp + 1, (t >> 1) & 1, false, false, true);
+          if (more) issue_s(t + 2, 1, grp, 1, lowQ, false, true);
         }
       }
     }
@@ -502,7 +514,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       drain(rfull, P::RAW, s_info[9]);
       for (int buf = 0; buf < 2; ++buf) {                   // every product was issued
         const int n = two ? nt : (nt - buf + 1) >> 1;
-        drain(sfull + 8 * buf, 1, n);
+        for (int sub = 0; sub < NS; ++sub) drain(sfull + 8 * (NS == 2 ? 2 * buf + sub : buf), 1, n);
         drain(odone + 8 * (2 * buf + 1), 1, n);
       }
     }
@@ -608,7 +620,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     const bool real = row / G < per_tile && tok < ntok;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     regs_up<P::REGS_SOFTMAX>();
-    regs_up<P::REGS_SOFTMAX>();
     // The query rows as two e4m3 rows each.  A warp takes 32 rows (16 where two groups share a tile), D / 8 lanes per row, and has
     // all its loads in flight before it looks at the first; every thread then picks up the multiplier of its own row.
     const bool halves = NS == 2 && !two;
@@ -677,7 +688,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     for (int i = grp; i < items && alive; i += NS) {
       const int j = two ? i >> 1 : i, base = (j0 + j) * kKeys;
       alive = wait_for(kinfo + 8 * (j % kInfo), (j / kInfo) & 1, gave_up, p.status);
-      if (alive) alive = wait_for(sfull + 8 * (i & 1), (i >> 1) & 1, gave_up, p.status);
+      if (NS == 1 && alive) alive = wait_for(sfull + 8 * (i & 1), (i >> 1) & 1, gave_up, p.status);
       __syncwarp();
       if (!alive) break;
       tc_fence_after();
@@ -690,6 +701,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         // multipliers of 16 scores each; never 0: a hidden score (-inf) times its multiplier stays -inf
         const float f[4] = {fmaxf(ks.x * rowmul, 1e-37f), fmaxf(ks.y * rowmul, 1e-37f), fmaxf(ks.z * rowmul, 1e-37f), fmaxf(ks.w * rowmul, 1e-37f)};
         const uint32_t ss = ts + 64u * part;
+        if (NS == 2) {
+          alive = wait_for(sfull + 8 * (2 * grp + part), (i >> 1) & 1, gave_up, p.status);
+          __syncwarp();
+          if (!alive) break;
+          tc_fence_after();
+        }
         uint32_t x[64], pk[32];
         float u;
         // Exponentials against the reference as it stands; their sum tells whether f16 can hold them.
@@ -750,7 +767,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           }
           if ((i >= NS || part) && __any_sync(0xffffffffu, alpha != 1.f)) {   // O has something in it: its last product has to be over
             if (part) alive = wait_for(odone + 8 * (2 * (i & 1)), (i >> 1) & 1, gave_up, p.status);
-            else if (NS == 1) alive = wait_for(odone + 8 * (2 * ((i - 1) & 1) + 1), ((i - 1) >> 1) & 1, gave_up, p.status);   // (two groups: over, since these scores are there)
+            else alive = wait_for(odone + 8 * (2 * ((i - NS) & 1) + 1), ((i - NS) >> 1) & 1, gave_up, p.status);
             __syncwarp();
             if (!alive) break;
             tc_fence_after();
@@ -768,7 +785,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         l += u;
         // into the columns that the scores leave
-        tmem_st32_nowait(ts + 32u * part, pk);
+        tmem_st32_nowait(NS == 2 ? ss : ts + 32u * part, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
