@@ -34,7 +34,7 @@ int check_rope(const B200AttnRope* r, const PagedGeometry& g) {
   if (!r->cos || !r->sin) return B200ATTN_ERR_NULL;
   if (r->rotary_dim < 16 || r->rotary_dim > g.head_dim || r->rotary_dim % 16) return B200ATTN_ERR_SHAPE;
   if (r->n_positions < 1 || r->n_axes < 1 || r->n_axes > 4 || (!r->positions && r->n_axes != 1)) return B200ATTN_ERR_SHAPE;
-  if (!aligned16(r->cos) || !aligned16(r->sin)) return B200ATTN_ERR_ALIGN;
+  if (!aligned16(r->cos) || !aligned16(r->sin) || !aligned16(r->pair_axis)) return B200ATTN_ERR_ALIGN;
   return B200ATTN_OK;
 }
 

@@ -33,7 +33,8 @@ struct AppendParams {
   const float *cos, *sin;
   const int *positions, *pair_axis;
   int n_positions, n_axes, rot;
-  int kv_blocks;
+  uint32_t q_units;       // warps' shares of the queries
+  int kv_blocks, heads;   // pages that the call touches, at most; kv heads that a block takes in turn
 };
 
 // Smallest power of two s with amax / s <= 448 = 1.75 * 2^8, at least 2^-126; amax is finite and >= 0.
@@ -48,98 +49,97 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;   // NaN and infinities do not take part in the maximum
 }
 
-// 8 bf16 -> floats
-__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+// A lane's share of a head row: four dims at `a` and four at `b`.  In the rotated part b = a + R / 2: a lane holds both halves of
+// its four pairs, so that the rotation needs no other lane (16 contiguous bytes per lane instead made 8 shuffles and twice the
+// cosines and sines: 170 instructions per 8 values, and the kernels were bound by issue).  Beyond it, 8 dims in a row.
+template <int D>
+struct Share {
+  static constexpr int TPR = D / 8;   // lanes per head row
+  int a, b;
+  bool on;                            // rotated
+  __device__ __forceinline__ Share(int lane, int rot) {
+    const int l = lane % TPR;
+    on = 8 * l < rot;
+    a = on ? 4 * l : 8 * l;
+    b = a + (on ? rot >> 1 : 4);
+  }
+};
+struct Raw { uint2 a, b; };
+// Read once: not worth a line of L1.
+__device__ __forceinline__ uint2 ldg_once(const uint16_t* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+template <int D>
+__device__ __forceinline__ Raw load_row(const uint16_t* row, const Share<D>& sh) { return Raw{ldg_once(row + sh.a), ldg_once(row + sh.b)}; }
+__device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = __uint_as_float(w[i] << 16);
     x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
 }
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&b);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ uint2 pack4(const float* x) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(x[0], x[1]), q = __floats2bfloat162_rn(x[2], x[3]);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
 }
-// 8 floats -> 8 e4m3 bytes: nearest even, saturating at 448; NaN -> 0x7F
-__device__ __forceinline__ uint2 quant8(const float (&x)[8], float inv) {
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(x[2 * i + 1] * inv), "f"(x[2 * i] * inv));
-    h[i] = r;
-  }
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+// 4 floats -> 4 e4m3 bytes: nearest even, saturating at 448; NaN -> 0x7F
+__device__ __forceinline__ uint32_t quant4(const float* x, float inv) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1] * inv), "f"(x[0] * inv));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3] * inv), "f"(x[2] * inv));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 // 16 e4m3 bytes re-expressed in a larger power-of-two scale: value * ratio, ratio = old / new < 1
 __device__ __forceinline__ uint4 rescale16(const uint4& raw, float ratio) {
   float f[16];
   e4m3x16_to_float(raw, f);
-  float a[8], b[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { a[i] = f[i]; b[i] = f[8 + i]; }
-  const uint2 lo = quant8(a, ratio), hi = quant8(b, ratio);
-  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  return make_uint4(quant4(f, ratio), quant4(f + 4, ratio), quant4(f + 8, ratio), quant4(f + 12, ratio));
 }
 
-// What a lane needs to rotate its 8 dims of a head: cosines, sines (0 / identity beyond rot) for one token.
-template <int D>
+// The cosines and sines of a lane's four pairs for one token (lanes beyond the rotated dims load those of pair 0 and do not use
+// them, so that no load stands behind a branch).
 struct Rotation {
-  static constexpr int TPR = D / 8;   // lanes per head row
-  float c[8], s[8];
-  int partner;                        // lane that holds the other half of the pairs
-  bool on, low;
+  float4 c, s;
 
-  __device__ __forceinline__ void load(const AppendParams& p, int lane, int token, int slot) {
-    const int lr = lane % TPR, i0 = lr * 8, half = p.rot >> 1;
-    on = i0 < p.rot;
-    low = i0 < half;
-    partner = lane + (on ? (low ? half / 8 : -(half / 8)) : 0);
-    if (!on) return;
-    const int j0 = low ? i0 : i0 - half;
+  __device__ __forceinline__ int clamped(const AppendParams& p, int pos, bool bad, bool on) const {
+    bad |= pos < 0 || pos >= p.n_positions;
+    if (bad && on) atomicOr(p.status, B200ATTN_STATUS_BAD_POSITION);
+    return min(max(pos, 0), p.n_positions - 1);
+  }
+  template <int D>
+  __device__ __forceinline__ void load(const AppendParams& p, const Share<D>& sh, int token, int slot) {
+    if (p.rot == 0) return;
+    const int half = p.rot >> 1, j0 = sh.on ? sh.a : 0;
     if (p.pair_axis == nullptr) {
-      int pos = p.positions ? p.positions[token] : slot;
-      if (pos < 0 || pos >= p.n_positions) {
-        atomicOr(p.status, B200ATTN_STATUS_BAD_POSITION);
-        pos = pos < 0 ? 0 : p.n_positions - 1;
-      }
-      const float4* cp = reinterpret_cast<const float4*>(p.cos + (long long)pos * half + j0);
-      const float4* sp = reinterpret_cast<const float4*>(p.sin + (long long)pos * half + j0);
-      const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-      c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
-      s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w; s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
+      const int pos = clamped(p, p.positions ? __ldg(p.positions + token) : slot, false, sh.on);
+      c = __ldg(reinterpret_cast<const float4*>(p.cos + (long long)pos * half + j0));
+      s = __ldg(reinterpret_cast<const float4*>(p.sin + (long long)pos * half + j0));
     } else {
+      const int4 ax = __ldg(reinterpret_cast<const int4*>(p.pair_axis + j0));
+      int at[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        int ax = __ldg(p.pair_axis + j0 + e);
-        bool bad = ax < 0 || ax >= p.n_axes;
-        ax = bad ? 0 : ax;
-        int pos = p.positions ? p.positions[(long long)ax * p.n_tokens + token] : slot;
-        bad |= pos < 0 || pos >= p.n_positions;
-        if (bad) atomicOr(p.status, B200ATTN_STATUS_BAD_POSITION);
-        pos = pos < 0 ? 0 : (pos >= p.n_positions ? p.n_positions - 1 : pos);
-        c[e] = __ldg(p.cos + (long long)pos * half + j0 + e);
-        s[e] = __ldg(p.sin + (long long)pos * half + j0 + e);
-      }
+      for (int a = 0; a < 4; ++a) at[a] = !p.positions ? slot : a < p.n_axes ? __ldg(p.positions + (long long)a * p.n_tokens + token) : 0;
+      auto pick = [&](int a) { return (long long)clamped(p, a == 1 ? at[1] : a == 2 ? at[2] : a == 3 ? at[3] : at[0], a < 0 || a >= p.n_axes, sh.on) * half + j0; };
+      const long long i0 = pick(ax.x), i1 = pick(ax.y) + 1, i2 = pick(ax.z) + 2, i3 = pick(ax.w) + 3;
+      c = make_float4(__ldg(p.cos + i0), __ldg(p.cos + i1), __ldg(p.cos + i2), __ldg(p.cos + i3));
+      s = make_float4(__ldg(p.sin + i0), __ldg(p.sin + i1), __ldg(p.sin + i2), __ldg(p.sin + i3));
     }
   }
-  // Every lane of the warp calls it (lanes of absent rows with zeros).
   __device__ __forceinline__ void turn(float (&x)[8]) const {
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_sync(0xffffffffu, x[e], partner & 31);
-      if (on) x[e] = low ? x[e] * c[e] - other * s[e] : x[e] * c[e] + other * s[e];
+    for (int e = 0; e < 4; ++e) {
+      const float u = x[e], v = x[4 + e];
+      x[e] = u * cc[e] - v * ss[e];
+      x[4 + e] = v * cc[e] + u * ss[e];
     }
   }
 };
 
-// RMS norm over the head's TPR lanes; every lane of the warp calls it.
+// RMS norm over the head's lanes; every lane of the warp calls it.
 template <int D>
 __device__ __forceinline__ void rms_norm(float (&x)[8], const float (&w1)[8], float eps) {
   float ss = 0.f;
@@ -152,11 +152,12 @@ __device__ __forceinline__ void rms_norm(float (&x)[8], const float (&w1)[8], fl
   for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w1[e];
 }
 template <int D>
-__device__ __forceinline__ void load_norm(const uint16_t* w, int layer, int lane, float (&w1)[8]) {
-  float t[8];
-  unpack8(__ldg(reinterpret_cast<const uint4*>(w + (long long)layer * D) + lane % (D / 8)), t);
+__device__ __forceinline__ void load_norm(const uint16_t* w, int layer, const Share<D>& sh, float (&w1)[8]) {
+  const uint16_t* row = w + (long long)layer * D;
+  const Raw r{__ldg(reinterpret_cast<const uint2*>(row + sh.a)), __ldg(reinterpret_cast<const uint2*>(row + sh.b))};
+  unpack(r, w1);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w1[e] = 1.f + t[e];
+  for (int e = 0; e < 8; ++e) w1[e] += 1.f;
 }
 
 // Sequence that owns packed token t (largest b with q_start[b] <= t; empty sequences share their start).
@@ -164,7 +165,7 @@ __device__ __forceinline__ int sequence_of(const int* q_start, int batch, int t)
   int lo = 0, hi = batch - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (q_start[mid] <= t) lo = mid; else hi = mid - 1;
+    if (__ldg(q_start + mid) <= t) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -174,138 +175,154 @@ __device__ __forceinline__ int page_of(const AppendParams& p, int b, int page_in
   return id >= 0 && id < p.g.n_pages ? id : -1;
 }
 
-// Query rows: one warp per token, its heads in turn; the rotation is loaded once per token.
+// Query rows: a warp takes kQLoads loads' worth of a token's heads, all in flight together, and rotates them with one set of
+// cosines and sines.  (One warp per token, head after head, waited for every load: 445 us for a 32768-token prompt of 40 / 8
+// heads against 160 us for its keys and values alone.)
+constexpr int kQLoads = 4;
 template <int D>
-__device__ __forceinline__ void rotate_queries(const AppendParams& p, long long first_warp, long long n_warps) {
-  constexpr int TPR = D / 8, RPW = 32 / TPR;   // head rows per warp step
+__host__ __device__ constexpr int q_heads() { return kQLoads * 32 / (D / 8); }   // heads of a warp: 8 or 4
+template <int D>
+__device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t unit) {
+  constexpr int TPR = D / 8, RPW = 32 / TPR;   // lanes per head row, rows per load
   const int lane = threadIdx.x & 31;
-  const long long rows = (long long)p.g.n_layers * p.n_tokens;
-  for (long long r = first_warp; r < rows; r += n_warps) {
-    const int layer = (int)(r / p.n_tokens), token = (int)(r % p.n_tokens);
-    int b = token, slot;
-    if (p.q_start) {
-      if (token >= p.q_start[p.g.batch] || token < p.q_start[0]) continue;   // a row that belongs to nobody
-      b = sequence_of(p.q_start, p.g.batch, token);
-      slot = p.seq_pos[b] + token - p.q_start[b];
-    } else {
-      slot = p.seq_pos[b];
-    }
-    Rotation<D> rot;
-    rot.load(p, lane, token, slot);
-    float w1[8];
-    if (p.wq) load_norm<D>(p.wq, layer, lane, w1);
-    const uint4* src = reinterpret_cast<const uint4*>(p.q) + r * p.g.h_q * TPR;
-    uint4* dst = reinterpret_cast<uint4*>(p.q_out) + r * p.g.h_q * TPR;
-    for (int h0 = 0; h0 < p.g.h_q; h0 += RPW) {
-      const int h = h0 + lane / TPR;
-      float x[8] = {};
-      if (h < p.g.h_q) unpack8(src[h * TPR + lane % TPR], x);
-      if (p.wq) rms_norm<D>(x, w1, p.eps);
-      rot.turn(x);
-      if (h < p.g.h_q) dst[h * TPR + lane % TPR] = pack8(x);
+  const uint32_t groups = (uint32_t)(p.g.h_q + q_heads<D>() - 1) / q_heads<D>();
+  const uint32_t r = unit / groups;            // (layer, token)
+  const int h0 = (int)(unit - r * groups) * q_heads<D>() + lane / TPR;
+  const int layer = (int)(r / (uint32_t)p.n_tokens), token = (int)(r - (uint32_t)layer * p.n_tokens);
+  const Share<D> sh(lane, p.rot);
+  const long long row0 = (long long)r * p.g.h_q + h0;
+  Raw raw[kQLoads];
+#pragma unroll
+  for (int i = 0; i < kQLoads; ++i)
+    if (h0 + i * RPW < p.g.h_q) raw[i] = load_row<D>(p.q + (row0 + i * RPW) * D, sh);
+  int b = token, slot;
+  if (p.q_start) {
+    if (token >= __ldg(p.q_start + p.g.batch) || token < __ldg(p.q_start)) return;   // a row that belongs to nobody
+    b = sequence_of(p.q_start, p.g.batch, token);
+    slot = __ldg(p.seq_pos + b) + token - __ldg(p.q_start + b);
+  } else {
+    slot = __ldg(p.seq_pos + b);
+  }
+  Rotation rot;
+  rot.load<D>(p, sh, token, slot);
+  float w1[8];
+  if (p.wq) load_norm<D>(p.wq, layer, sh, w1);
+#pragma unroll
+  for (int i = 0; i < kQLoads; ++i) {
+    float x[8];
+    unpack(raw[i], x);
+    if (p.wq) rms_norm<D>(x, w1, p.eps);
+    if (sh.on) rot.turn(x);
+    if (h0 + i * RPW < p.g.h_q) {
+      uint16_t* dst = p.q_out + (row0 + i * RPW) * D;
+      *reinterpret_cast<uint2*>(dst + sh.a) = pack4(x);
+      *reinterpret_cast<uint2*>(dst + sh.b) = pack4(x + 4);
     }
   }
 }
 
-// One token per sequence.  One warp per key or value row (its first TPR lanes hold the row; all 32 re-express the page's
-// earlier rows when the scale grows), the warps behind them rotate the queries.
+// One token per sequence.  D / 8 lanes hold a key or value row: half a warp the key and half the value of a head (heads of
+// 128), or a warp one of them (256).  The same lanes re-express the page's earlier rows when the scale grows.  The warps behind
+// those rotate the queries.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 paged_append_token_kernel(const AppendParams p) {
-  constexpr int TPR = D / 8;
+  constexpr int TPR = D / 8, RPW = 32 / TPR;
   const PagedGeometry& g = p.g;
-  const int lane = threadIdx.x & 31;
-  const long long warp = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const long long kv_rows = (long long)g.n_layers * g.batch * g.h_kv * 2;
-  if (warp >= kv_rows) {
-    if (p.q) rotate_queries<D>(p, warp - kv_rows, (long long)gridDim.x * 8 - kv_rows);
+  const int lane = threadIdx.x & 31, lr = lane % TPR;
+  const uint32_t warp = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const uint32_t rows = (uint32_t)g.n_layers * g.batch * g.h_kv * 2, kv_warps = (rows + RPW - 1) / RPW;   // rows is even
+  if (warp >= kv_warps) {
+    if (warp - kv_warps < p.q_units) rotate_queries<D>(p, warp - kv_warps);
     return;
   }
-  const int which = (int)(warp & 1);                 // 0 key, 1 value
-  const long long row = warp >> 1;                   // (layer, sequence, head)
+  const uint32_t r2 = warp * RPW + lane / TPR;       // (layer, sequence, head, key or value)
+  const int which = (int)(r2 & 1);                   // 0 key, 1 value
+  const uint32_t row = r2 >> 1;
   const int h = (int)(row % g.h_kv);
-  const long long lb = row / g.h_kv;
+  const uint32_t lb = row / g.h_kv;
   const int b = (int)(lb % g.batch), layer = (int)(lb / g.batch);
-  const int pos = p.seq_pos[b];
-  if (pos < 0 || pos >= (long long)g.max_pages * g.page_size) {
-    if (lane == 0) atomicOr(p.status, B200ATTN_STATUS_POS_AT_CAPACITY);
-    return;
-  }
-  const int fill = pos % g.page_size, page = page_of(p, b, pos / g.page_size);
-  if (page < 0) {
-    if (lane == 0) atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
-    return;
-  }
-  float x[8] = {};
-  if (lane < TPR) unpack8(reinterpret_cast<const uint4*>(which ? p.v : p.k)[row * TPR + lane], x);
-  if (!which) {
+  const Share<D> sh(lane, p.rot);
+  const Raw raw = load_row<D>((which ? p.v : p.k) + (long long)row * D, sh);
+  const int pos = __ldg(p.seq_pos + b);
+  const bool fits = pos >= 0 && pos < (long long)g.max_pages * g.page_size;
+  const int page = fits ? page_of(p, b, pos / g.page_size) : -1, fill = fits ? pos % g.page_size : 0;
+  if (page < 0 && lr == 0) atomicOr(p.status, fits ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);
+  float* sp = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv + h;
+  const float old = page >= 0 && fill > 0 ? *sp : 0.f;
+  float x[8];
+  unpack(raw, x);
+  if (RPW == 2 || !which) {                          // uniform over the warp: it holds a key and a value, or one of them
     if (p.wk) {
-      float w1[8];
-      load_norm<D>(p.wk, layer, lane, w1);
-      rms_norm<D>(x, w1, p.eps);
+      float w1[8], k[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[e] = x[e];
+      load_norm<D>(p.wk, layer, sh, w1);
+      rms_norm<D>(k, w1, p.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = which ? x[e] : k[e];
     }
-    Rotation<D> rot;
-    rot.load(p, lane, b, pos);
-    rot.turn(x);
+    Rotation rot;
+    rot.load<D>(p, sh, b, fits ? pos : 0);
+    if (!which && sh.on) rot.turn(x);
   }
   float amax = 0.f;
-  if (lane < TPR)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[e]));
+  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[e]));
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  for (int off = TPR / 2; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  if (page < 0) return;
   float s = pow2_scale(amax);
-  float* sp = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv + h;
   uint8_t* base = (which ? p.v_pages : p.k_pages) + (long long)layer * (which ? g.v_layer_stride : g.k_layer_stride) +
                   ((long long)page * g.h_kv + h) * g.page_size * D;
   if (fill > 0) {
-    const float old = *sp;
     if (s > old) {
       const float ratio = old / s;
       uint4* rows16 = reinterpret_cast<uint4*>(base);
       const int n = fill * (D / 16);
 #pragma unroll 4
-      for (int i = lane; i < n; i += 32) rows16[i] = rescale16(rows16[i], ratio);
+      for (int i = lr; i < n; i += TPR) rows16[i] = rescale16(rows16[i], ratio);
     } else {
       s = old;
     }
   }
-  __syncwarp();
-  if (lane == 0) *sp = s;
-  if (lane < TPR) reinterpret_cast<uint2*>(base + (long long)fill * D)[lane] = quant8(x, __fdiv_rn(1.f, s));
+  if (lr == 0) *sp = s;
+  const float inv = __fdiv_rn(1.f, s);
+  uint8_t* dst = base + (long long)fill * D;
+  *reinterpret_cast<uint32_t*>(dst + sh.a) = quant4(x, inv);
+  *reinterpret_cast<uint32_t*>(dst + sh.b) = quant4(x + 4, inv);
 }
 
-// Prompts.  A thread block holds the new tokens of one (layer, page, kv head) of keys or of values: rotates them, finds
-// their scale, writes them.  The blocks behind those rotate the queries.  NP: passes of THREADS / TPR rows over a page.
+// Prompts.  A thread block holds the new tokens of one page for `heads` kv heads in turn, of keys or of values: it rotates
+// them, finds the page's scale, writes them; the next head's rows are on their way meanwhile.  THREADS x NP rows' shares cover a
+// page.
 template <int D, int NP, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 paged_append_prompt_kernel(const AppendParams p) {
   constexpr int TPR = D / 8, RPP = THREADS / TPR;
   const PagedGeometry& g = p.g;
   const int tid = threadIdx.x, lane = tid & 31;
-  const long long units = (long long)p.kv_blocks * g.h_kv * 2 * g.n_layers;
-  if (blockIdx.x >= units) {
-    if (p.q) rotate_queries<D>(p, ((long long)blockIdx.x - units) * (THREADS / 32) + (tid >> 5), ((long long)gridDim.x - units) * (THREADS / 32));
-    return;
-  }
+  const int groups = (g.h_kv + p.heads - 1) / p.heads;
   const int which = (int)(blockIdx.x & 1);
-  long long u = blockIdx.x >> 1;
-  const int h = (int)(u % g.h_kv);
-  u /= g.h_kv;
+  uint32_t u = blockIdx.x >> 1;
+  const int h_first = (int)(u % groups) * p.heads, h_end = min(h_first + p.heads, g.h_kv);
+  u /= groups;
   const int chunk = (int)(u % p.kv_blocks), layer = (int)(u / p.kv_blocks);
 
   // the sequence and page that chunk number `chunk` of the call is: a scan over the sequences' touched pages
-  __shared__ int s_seq, s_page;
-  __shared__ float s_max[THREADS / 32];
+  __shared__ int s_at[5];                                // sequence, page of it, first packed token, tokens, tokens before
+  __shared__ float s_max[2][THREADS / 32];
   if (tid < 32) {
     int before = 0;
-    if (tid == 0) s_seq = -1;
+    if (tid == 0) s_at[0] = -1;
     __syncwarp();
     for (int b0 = 0; b0 < g.batch; b0 += 32) {
       const int b = b0 + lane;
-      int n = 0, first = 0;
+      int n = 0, first = 0, q0 = 0, nt = 0, pos = 0;
       if (b < g.batch) {
-        const int q0 = p.q_start[b], nt = p.q_start[b + 1] - q0, pos = p.seq_pos[b];
+        q0 = p.q_start[b];
+        nt = p.q_start[b + 1] - q0;
+        pos = p.seq_pos[b];
         if (nt > 0 && pos >= 0 && q0 >= 0 && q0 + nt <= p.n_tokens) {
           first = pos / g.page_size;
           n = (int)(((long long)pos + nt - 1) / g.page_size) - first + 1;
@@ -318,83 +335,103 @@ paged_append_prompt_kernel(const AppendParams p) {
         if (lane >= off) inc += t;
       }
       const int start = before + inc - n;
-      if (n > 0 && chunk >= start && chunk < start + n) { s_seq = b; s_page = first + chunk - start; }
+      if (n > 0 && chunk >= start && chunk < start + n) { s_at[0] = b; s_at[1] = first + chunk - start; s_at[2] = q0; s_at[3] = nt; s_at[4] = pos; }
       before += __shfl_sync(0xffffffffu, inc, 31);
       if (before > chunk) break;
     }
   }
   __syncthreads();
-  const int b = s_seq;
+  const int b = s_at[0];
   if (b < 0) return;                                     // the grid is an upper bound
-  const int page_index = s_page;
-  const int q0 = p.q_start[b], nt = p.q_start[b + 1] - q0, pos = p.seq_pos[b];
+  const int page_index = s_at[1], q0 = s_at[2], nt = s_at[3], pos = s_at[4];
+  const int slot0 = page_index * g.page_size;
+  const int lo = max(pos - slot0, 0);                                                   // rows [lo, hi) are new
+  const int hi = (int)min((long long)g.page_size, (long long)pos + nt - slot0);
+  const Share<D> sh(lane, p.rot);
+  const uint16_t* src = (which ? p.v : p.k) + ((long long)layer * p.n_tokens + q0 + slot0 - pos) * g.h_kv * D;
+  Raw raw[NP];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = i * RPP + tid / TPR;
+      raw[i] = Raw{make_uint2(0, 0), make_uint2(0, 0)};
+      if (row >= lo && row < hi) raw[i] = load_row<D>(src + ((long long)row * g.h_kv + h) * D, sh);
+    }
+  };
+  load(h_first);
   const int page = page_index < g.max_pages ? page_of(p, b, page_index) : -1;
   if (page < 0) {
     if (tid == 0) atomicOr(p.status, page_index < g.max_pages ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);
     return;
   }
-  const int slot0 = page_index * g.page_size;
-  const int lo = max(pos - slot0, 0);                                                   // rows [lo, hi) are new
-  const int hi = (int)min((long long)g.page_size, (long long)pos + nt - slot0);
+  Rotation rot[NP];                                      // of this thread's rows, for all heads
+  if (!which)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = min(max(i * RPP + tid / TPR, lo), hi - 1);
+      rot[i].load<D>(p, sh, q0 + slot0 + row - pos, slot0 + row);
+    }
+  float* scales = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv;
+  uint8_t* pages = (which ? p.v_pages : p.k_pages) + (long long)layer * (which ? g.v_layer_stride : g.k_layer_stride) +
+                   (long long)page * g.h_kv * g.page_size * D;
+#pragma unroll 1
+  for (int h = h_first; h < h_end; ++h) {
+    float x[NP][8];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) unpack(raw[i], x[i]);
+    const float old = lo > 0 ? scales[h] : 0.f;
+    if (h + 1 < h_end) load(h + 1);
+    if (!which && p.wk) {
+      float w1[8];
+      load_norm<D>(p.wk, layer, sh, w1);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) rms_norm<D>(x[i], w1, p.eps);
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (!which && sh.on) rot[i].turn(x[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[i][e]));   // rows that are not new are zero
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    if (lane == 0) s_max[h & 1][tid >> 5] = amax;
+    __syncthreads();                                      // maxima are in; every thread has read the old scale
+    amax = lane < THREADS / 32 ? s_max[h & 1][lane] : 0.f;
+#pragma unroll
+    for (int off = THREADS / 64; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    amax = __shfl_sync(0xffffffffu, amax, 0);
+    float s = pow2_scale(amax);
+    uint8_t* base = pages + (long long)h * g.page_size * D;
+    if (lo > 0) {
+      if (s > old) {
+        const float ratio = old / s;
+        uint4* rows16 = reinterpret_cast<uint4*>(base);
+        for (int i = tid; i < lo * (D / 16); i += THREADS) rows16[i] = rescale16(rows16[i], ratio);
+      } else {
+        s = old;
+      }
+    }
+    if (tid == 0) scales[h] = s;
+    const float inv = __fdiv_rn(1.f, s);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = i * RPP + tid / TPR;
+      if (row >= lo && row < hi) {
+        uint8_t* dst = base + (long long)row * D;
+        *reinterpret_cast<uint32_t*>(dst + sh.a) = quant4(x[i], inv);
+        *reinterpret_cast<uint32_t*>(dst + sh.b) = quant4(x[i] + 4, inv);
+      }
+    }
+  }
+}
 
-  float x[NP][8];
-  float w1[8];
-  const bool norm = !which && p.wk != nullptr;
-  if (norm) load_norm<D>(p.wk, layer, lane, w1);
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int row = i * RPP + tid / TPR;
-    const bool mine = row >= lo && row < hi;
-    const int token = q0 + slot0 + row - pos;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-    if (mine)
-      unpack8(reinterpret_cast<const uint4*>(which ? p.v : p.k)[(((long long)layer * p.n_tokens + token) * g.h_kv + h) * TPR + tid % TPR], x[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int row = i * RPP + tid / TPR;
-    const bool mine = row >= lo && row < hi;
-    if (!which) {
-      if (norm) rms_norm<D>(x[i], w1, p.eps);
-      Rotation<D> rot;
-      const int safe = min(max(row, lo), hi - 1);
-      rot.load(p, lane, q0 + slot0 + safe - pos, slot0 + safe);
-      rot.turn(x[i]);
-    }
-    if (mine)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[i][e]));
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  if (lane == 0) s_max[tid >> 5] = amax;
-  float* sp = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv + h;
-  const float old = lo > 0 ? *sp : 0.f;
-  __syncthreads();                                        // maxima are in; every thread has read the old scale
-  amax = s_max[0];
-#pragma unroll
-  for (int i = 1; i < THREADS / 32; ++i) amax = fmaxf(amax, s_max[i]);
-  float s = pow2_scale(amax);
-  uint8_t* base = (which ? p.v_pages : p.k_pages) + (long long)layer * (which ? g.v_layer_stride : g.k_layer_stride) +
-                  ((long long)page * g.h_kv + h) * g.page_size * D;
-  if (lo > 0) {
-    if (s > old) {
-      const float ratio = old / s;
-      uint4* rows16 = reinterpret_cast<uint4*>(base);
-      for (int i = tid; i < lo * (D / 16); i += THREADS) rows16[i] = rescale16(rows16[i], ratio);
-    } else {
-      s = old;
-    }
-  }
-  if (tid == 0) *sp = s;
-  const float inv = __fdiv_rn(1.f, s);
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int row = i * RPP + tid / TPR;
-    if (row >= lo && row < hi) reinterpret_cast<uint2*>(base + (long long)row * D)[tid % TPR] = quant8(x[i], inv);
-  }
+// The queries of prompts: a kernel of their own, with more warps on an SM than the one above has.
+template <int D>
+__global__ void __launch_bounds__(256) paged_rotate_queries_kernel(const AppendParams p) {
+  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit < p.q_units) rotate_queries<D>(p, unit);
 }
 
 __global__ void paged_advance_kernel(PagedGeometry g, const int* q_start, int* seq_pos) {
@@ -425,34 +462,44 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
     p.positions = a.rope->positions; p.pair_axis = a.rope->pair_axis;
     p.n_positions = a.rope->n_positions; p.n_axes = a.rope->n_axes; p.rot = a.rope->rotary_dim;
   }
-  const long long q_rows = a.q ? (long long)g.n_layers * a.n_tokens : 0;
+  const int q_heads_ = g.head_dim == 128 ? q_heads<128>() : q_heads<256>();
+  const long long q_warps = a.q ? (long long)g.n_layers * a.n_tokens * ((g.h_q + q_heads_ - 1) / q_heads_) : 0;
+  const long long kv_rows = (long long)g.n_layers * g.batch * g.h_kv * 2;
+  if (q_warps > 0x7fffffffLL || kv_rows > 0x7fffffffLL) return cudaErrorInvalidConfiguration;   // indices are 32-bit
+  p.q_units = (uint32_t)q_warps;
   if (!a.q_start) {
-    const long long warps = (long long)g.n_layers * g.batch * g.h_kv * 2 + q_rows;
-    const long long grid = (warps + 7) / 8;
-    if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    if (g.head_dim == 128) paged_append_token_kernel<128><<<(unsigned)grid, 256, 0, stream>>>(p);
-    else paged_append_token_kernel<256><<<(unsigned)grid, 256, 0, stream>>>(p);
+    const long long rpw = g.head_dim == 128 ? 2 : 1, grid = ((kv_rows + rpw - 1) / rpw + q_warps + 3) / 4;
+    if (g.head_dim == 128) paged_append_token_kernel<128><<<(unsigned)grid, 128, 0, stream>>>(p);
+    else paged_append_token_kernel<256><<<(unsigned)grid, 128, 0, stream>>>(p);
   } else if (a.n_tokens > 0) {
     // pages that the call touches: n tokens touch at most n pages, and at most n / page_size + 2 (an open first and last page)
     const long long most = (long long)a.n_tokens / g.page_size + 2LL * g.batch;
     p.kv_blocks = (int)(most < a.n_tokens ? most : a.n_tokens);
-    const int threads = g.page_size * g.head_dim == 128 * 256 ? 512 : 256;
-    const long long grid = (long long)p.kv_blocks * g.h_kv * 2 * g.n_layers + (q_rows + threads / 32 - 1) / (threads / 32);
+    // two loads of 16 bytes per thread and page (four for the largest pages); of its heads a block takes as many in turn as leave every SM a few blocks
+    const int threads = g.page_size * g.head_dim / 16 < 1024 ? g.page_size * g.head_dim / 16 : 1024;
+    const long long pages = (long long)p.kv_blocks * 2 * g.n_layers, blocks = 2LL * device_sms() * (1024 / threads);
+    long long heads = pages * g.h_kv / blocks;
+    p.heads = (int)(heads < 1 ? 1 : heads > g.h_kv ? g.h_kv : heads);
+    const long long grid = pages * ((g.h_kv + p.heads - 1) / p.heads), q_grid = (q_warps + 7) / 8;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    if (q_grid) {
+      if (g.head_dim == 128) paged_rotate_queries_kernel<128><<<(unsigned)q_grid, 256, 0, stream>>>(p);
+      else paged_rotate_queries_kernel<256><<<(unsigned)q_grid, 256, 0, stream>>>(p);
+    }
     auto launch = [&](auto kernel) { kernel<<<(unsigned)grid, threads, 0, stream>>>(p); };
     if (g.head_dim == 128) {
       switch (g.page_size) {
-        case 16: launch(paged_append_prompt_kernel<128, 1, 256>); break;
+        case 16: launch(paged_append_prompt_kernel<128, 2, 128>); break;
         case 32: launch(paged_append_prompt_kernel<128, 2, 256>); break;
-        case 64: launch(paged_append_prompt_kernel<128, 4, 256>); break;
-        default: launch(paged_append_prompt_kernel<128, 8, 256>); break;
+        case 64: launch(paged_append_prompt_kernel<128, 2, 512>); break;
+        default: launch(paged_append_prompt_kernel<128, 2, 1024>); break;
       }
     } else {
       switch (g.page_size) {
         case 16: launch(paged_append_prompt_kernel<256, 2, 256>); break;
-        case 32: launch(paged_append_prompt_kernel<256, 4, 256>); break;
-        case 64: launch(paged_append_prompt_kernel<256, 8, 256>); break;
-        default: launch(paged_append_prompt_kernel<256, 8, 512>); break;
+        case 32: launch(paged_append_prompt_kernel<256, 2, 512>); break;
+        case 64: launch(paged_append_prompt_kernel<256, 2, 1024>); break;
+        default: launch(paged_append_prompt_kernel<256, 4, 1024>); break;
       }
     }
   }
