@@ -462,6 +462,7 @@ __device__ __noinline__ void combine_deferred(CombineArgs a, DeferredCombine dc,
 #pragma unroll
       for (int i = 0; i < CH; ++i)
         if (c0 + i < n) pending |= ((1u << (2 * UR + 2)) - 1u) << (i * (2 * UR + 2));
+      bool gave_up = false;
       for (int tries = 0; pending; ++tries) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -487,9 +488,13 @@ __device__ __noinline__ void combine_deferred(CombineArgs a, DeferredCombine dc,
         }
         if (pending && (tries & 63) == 63 && global_timer_ns() - t0 > kWaitBudgetNs) {
           atomicOr(a.status, B200ATTN_STATUS_WAIT_TIMEOUT);
-          return;
+          gave_up = true;
+          break;
         }
       }
+      // Every lane polls m and l, and lane 0 zeroes them below: not before the others have read them.  (Lanes leave the loop
+      // above one by one.)
+      if (__any_sync(0xffffffffu, gave_up)) return;
       float Mn = M;
 #pragma unroll
       for (int i = 0; i < CH; ++i)
