@@ -24,57 +24,45 @@ from . import _lib
 from ._lib import B200AttnPagedShape, B200AttnRope, check
 
 _BYTE_TYPES = (torch.uint8, torch.float8_e4m3fn)
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _need(device: torch.device, dtype, **tensors) -> None:
-    """Every given tensor: on `device`, contiguous, of type `dtype`."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if t.device != device or device.type != "cuda":
-            raise ValueError(f"{name} must be on the cache's CUDA device ({device}): there is no CPU path")
-        if t.dtype != dtype:
-            raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+def _need(idx: int, dtype, names: str, *tensors) -> None:
+    """Every given tensor (None = not given): on CUDA device `idx`, contiguous, of type `dtype`.  `names` in the same order."""
+    for t in tensors:
+        if t is not None and (t.get_device() != idx or t.dtype is not dtype or not t.is_contiguous() or idx < 0):
+            name = names.split()[[x is t for x in tensors].index(True)]
+            if idx < 0 or t.get_device() != idx:
+                raise ValueError(f"{name} must be on the cache's CUDA device: there is no CPU path")
+            raise ValueError(f"{name} must be contiguous {dtype}, not {'' if t.is_contiguous() else 'strided '}{t.dtype}")
 
 
-class _on:
-    """The tensors' device, made current for the call if it is not; gives its current stream."""
-
-    __slots__ = ("device", "guard")
-
-    def __init__(self, device: torch.device):
-        self.device, self.guard = device, None
-
-    def __enter__(self) -> int:
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(idx: int, fn, *args) -> int:
+    """fn(*args, stream) on device `idx`, which is made current for the call if it is not, and its current stream."""
+    if torch._C._cuda_getDevice() == idx:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    with torch.cuda.device(idx):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(idx))
 
 
 def make_paged_shape(h_q: int, k_pages, v_pages, k_scale, page_table) -> B200AttnPagedShape:
     """Geometry from the cache handles.  A 5-d pool may be strided over layers (dim 0) only."""
-    if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
+    dims = k_pages.shape
+    if v_pages.shape != dims or len(dims) not in (4, 5):
         raise ValueError("k_pages and v_pages must have the same shape [n_layers, n_pages, h_kv, page_size, head_dim]")
-    n = 1 if k_pages.dim() == 4 else k_pages.shape[0]
-    n_pages, h_kv, page, d = k_pages.shape[-4:]
-    for c in (k_pages, v_pages):
-        if c.dtype not in _BYTE_TYPES:
-            raise ValueError("the cache must be uint8 / float8_e4m3fn")
-        if c.stride()[-4:] != (h_kv * page * d, page * d, d, 1):
-            raise ValueError("the cache must be dense within a layer")
+    n = 1 if len(dims) == 4 else dims[0]
+    n_pages, h_kv, page, d = dims[-4:]
+    if k_pages.dtype not in _BYTE_TYPES or v_pages.dtype not in _BYTE_TYPES:
+        raise ValueError("the cache must be uint8 / float8_e4m3fn")
+    k_stride, v_stride, dense = k_pages.stride(), v_pages.stride(), (h_kv * page * d, page * d, d, 1)
+    if k_stride[-4:] != dense or v_stride[-4:] != dense:
+        raise ValueError("the cache must be dense within a layer")
     if k_scale.numel() != n * n_pages * h_kv:
         raise ValueError("scales must be [n_layers, n_pages, h_kv]")
-    if page_table.dim() != 2:
+    table = page_table.shape
+    if len(table) != 2:
         raise ValueError("page_table must be [batch, max_pages]")
-    return B200AttnPagedShape(n, page_table.shape[0], h_q, h_kv, d, page, n_pages, page_table.shape[1],
-                              k_pages.stride(0) if n > 1 else 0, v_pages.stride(0) if n > 1 else 0, 0, 0)
+    return B200AttnPagedShape(n, table[0], h_q, h_kv, d, page, n_pages, table[1], k_stride[0] if n > 1 else 0, v_stride[0] if n > 1 else 0, 0, 0)
 
 
 class PagedWorkspace:
@@ -86,26 +74,27 @@ class PagedWorkspace:
         self.max_seq_len = int(max_seq_len or 0)
         self.q_tokens = int(q_tokens or 0)
         out = ctypes.c_size_t(0)
-        with _on(torch.device(device)) as stream:
+        with torch.cuda.device(device):
             check(_lib.lib().b200attn_paged_workspace_bytes(ctypes.byref(shape), self.q_tokens, self.max_seq_len, ctypes.byref(out)),
                   "b200attn_paged_workspace_bytes")
             self.nbytes = max(256, out.value)
             self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
             self.status = torch.zeros(1, dtype=torch.int32, device=device)
-            check(_lib.lib().b200attn_workspace_init(self.buf.data_ptr(), self.nbytes, stream), "b200attn_workspace_init")
+            check(_lib.lib().b200attn_workspace_init(self.buf.data_ptr(), self.nbytes, torch.cuda.current_stream().cuda_stream),
+                  "b200attn_workspace_init")
 
     def read_status(self) -> int:
         """Device status bits (synchronises; not for use inside a captured step)."""
         return int(self.status.item())
 
 
-def _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table):
-    dev = k_pages.device
-    _need(dev, torch.float32, k_scale=k_scale, v_scale=v_scale)
-    _need(dev, torch.int32, page_table=page_table)
-    if v_pages.device != dev or v_scale.numel() != k_scale.numel():
+def _cache_device(k_pages, v_pages, k_scale, v_scale, page_table) -> int:
+    idx = k_pages.get_device()
+    _need(idx, _F32, "k_scale v_scale", k_scale, v_scale)
+    _need(idx, _I32, "page_table", page_table)
+    if v_pages.get_device() != idx or v_scale.numel() != k_scale.numel():
         raise ValueError("k_pages / v_pages and k_scale / v_scale must match")
-    return dev
+    return idx
 
 
 def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, seq_pos, *, q_start=None,
@@ -119,16 +108,16 @@ def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, pag
     [rotary_dim / 2] saying which axis turns which pair.  Norm weights bf16 [n_layers, head_dim]: RMS norm with weight 1 + w
     before the rotation.  `seq_pos`: tokens cached before the call, advanced afterwards if `advance`.  Capacity, bad pages
     and bad positions are reported in `status`."""
-    h_kv, d = k_pages.shape[-3], k_pages.shape[-1]
-    h_q = q.shape[-2] if q is not None else h_kv
+    h_q = q.shape[-2] if q is not None else k_pages.shape[-3]
     shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
-    dev = _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table)
-    _need(dev, torch.bfloat16, q=q, k=k, v=v, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, q_out=q_out)
-    _need(dev, torch.int32, seq_pos=seq_pos, q_start=q_start, positions=positions, pair_axis=pair_axis, status=status)
-    _need(dev, torch.float32, cos=cos, sin=sin)
+    h_kv, d = shape.h_kv, shape.head_dim
+    idx = _cache_device(k_pages, v_pages, k_scale, v_scale, page_table)
+    _need(idx, _BF16, "q k v q_norm_weight k_norm_weight q_out", q, k, v, q_norm_weight, k_norm_weight, q_out)
+    _need(idx, _I32, "seq_pos q_start positions pair_axis status", seq_pos, q_start, positions, pair_axis, status)
+    _need(idx, _F32, "cos sin", cos, sin)
     n_layers = shape.n_layers
     n_tokens = k.numel() // (n_layers * h_kv * d)
-    if k.numel() != n_layers * n_tokens * h_kv * d or k.shape[-2:] != (h_kv, d) or v.shape != k.shape:
+    if k.numel() != n_layers * n_tokens * h_kv * d or v.shape != k.shape or k.shape[-2:] != (h_kv, d):
         raise ValueError("k and v must be [n_layers, n_tokens, h_kv, head_dim]")
     if q is not None and (q.numel() != n_layers * n_tokens * h_q * d or q.shape[-1] != d):
         raise ValueError("q must be [n_layers, n_tokens, h_q, head_dim]")
@@ -161,14 +150,12 @@ def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, pag
             raise ValueError("q_out must have q's shape")
     if n_tokens == 0:
         return q_out if q is not None else None
-    with _on(dev) as stream:
-        rc = _lib.lib().b200attn_paged_rope_append(
-            ctypes.byref(shape), ctypes.byref(rope) if rope is not None else None, n_tokens,
-            q_start.data_ptr() if q_start is not None else None, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
-            q_norm_weight.data_ptr() if q_norm_weight is not None else None,
-            k_norm_weight.data_ptr() if k_norm_weight is not None else None, eps, q_out.data_ptr() if q is not None else None,
-            k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
-            seq_pos.data_ptr(), int(advance), status.data_ptr(), stream)
+    rc = _call(idx, _lib.lib().b200attn_paged_rope_append, ctypes.byref(shape), ctypes.byref(rope) if rope is not None else None, n_tokens,
+               q_start.data_ptr() if q_start is not None else None, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
+               q_norm_weight.data_ptr() if q_norm_weight is not None else None,
+               k_norm_weight.data_ptr() if k_norm_weight is not None else None, eps, q_out.data_ptr() if q is not None else None,
+               k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
+               seq_pos.data_ptr(), int(advance), status.data_ptr())
     check(rc, "b200attn_paged_rope_append")
     return q_out if q is not None else None
 
@@ -177,27 +164,25 @@ def paged_decode_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, se
                            softmax_scale: float | None = None, seq_len_offset: int = 0, out: torch.Tensor | None = None):
     """Attention of one query token per sequence (q bf16 [n_layers, batch, h_q, head_dim]) over the first
     seq_len[b] + seq_len_offset tokens of its pages; bf16 with q's shape.  A sequence without tokens gives zeros."""
-    h_q, d = q.shape[-2], q.shape[-1]
+    h_q, d = q.shape[-2:]
     shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
-    dev = _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table)
-    _need(dev, torch.bfloat16, q=q, out=out)
-    _need(dev, torch.int32, seq_len=seq_len)
+    idx = _cache_device(k_pages, v_pages, k_scale, v_scale, page_table)
+    _need(idx, _BF16, "q out", q, out)
+    _need(idx, _I32, "seq_len", seq_len)
     if d != shape.head_dim or q.numel() != shape.n_layers * shape.batch * h_q * d:
         raise ValueError("q must be [n_layers, batch, h_q, head_dim]")
     if seq_len.numel() != shape.batch:
         raise ValueError("seq_len must be int32 [batch]")
-    if workspace.q_tokens or workspace.buf.device != dev:
+    if workspace.q_tokens or workspace.buf.get_device() != idx:
         raise ValueError("the workspace must be one for decode, on the cache's device")
     if out is None:
         out = torch.empty_like(q)
     elif out.numel() != q.numel():
         raise ValueError("out must have q's shape")
-    with _on(dev) as stream:
-        rc = _lib.lib().b200attn_paged_decode(
-            ctypes.byref(shape), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            page_table.data_ptr(), seq_len.data_ptr(), seq_len_offset, workspace.max_seq_len,
-            d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(), workspace.nbytes, out.data_ptr(),
-            workspace.status.data_ptr(), stream)
+    rc = _call(idx, _lib.lib().b200attn_paged_decode, ctypes.byref(shape), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+               k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(), seq_len_offset, workspace.max_seq_len,
+               d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(), workspace.nbytes, out.data_ptr(),
+               workspace.status.data_ptr())
     check(rc, "b200attn_paged_decode")
     return out
 
@@ -207,17 +192,17 @@ def paged_prefill_attention(q, q_start, k_pages, v_pages, k_scale, v_scale, page
     """Attention of many query tokens per sequence (q bf16 [n_layers, n_tokens, h_q, head_dim], packed by `q_start`) over the
     first seq_len[b] tokens of its pages.  causal: a sequence's queries are its last tokens, each sees those up to itself;
     not causal: all (cross attention).  Rows that see nothing are zero; rows behind q_start[batch] are left as they were."""
-    h_q, d = q.shape[-2], q.shape[-1]
+    h_q, d = q.shape[-2:]
     shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
-    dev = _cache_args(shape, k_pages, v_pages, k_scale, v_scale, page_table)
-    _need(dev, torch.bfloat16, q=q, out=out)
-    _need(dev, torch.int32, seq_len=seq_len, q_start=q_start)
+    idx = _cache_device(k_pages, v_pages, k_scale, v_scale, page_table)
+    _need(idx, _BF16, "q out", q, out)
+    _need(idx, _I32, "seq_len q_start", seq_len, q_start)
     n_tokens = q.numel() // (shape.n_layers * h_q * d)
     if d != shape.head_dim or q.numel() != shape.n_layers * n_tokens * h_q * d:
         raise ValueError("q must be [n_layers, n_tokens, h_q, head_dim]")
     if seq_len.numel() != shape.batch or q_start.numel() != shape.batch + 1:
         raise ValueError("seq_len must be int32 [batch], q_start int32 [batch + 1]")
-    if workspace.q_tokens < n_tokens or workspace.buf.device != dev:
+    if workspace.q_tokens < n_tokens or workspace.buf.get_device() != idx:
         raise ValueError(f"the workspace must be one for {n_tokens} query tokens, on the cache's device")
     if out is None:
         out = torch.empty_like(q)
@@ -225,12 +210,10 @@ def paged_prefill_attention(q, q_start, k_pages, v_pages, k_scale, v_scale, page
         raise ValueError("out must have q's shape")
     if n_tokens == 0:
         return out
-    with _on(dev) as stream:
-        rc = _lib.lib().b200attn_paged_prefill(
-            ctypes.byref(shape), n_tokens, q.data_ptr(), q_start.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(), workspace.max_seq_len, int(causal),
-            d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(), workspace.nbytes, out.data_ptr(),
-            workspace.status.data_ptr(), stream)
+    rc = _call(idx, _lib.lib().b200attn_paged_prefill, ctypes.byref(shape), n_tokens, q.data_ptr(), q_start.data_ptr(), k_pages.data_ptr(),
+               v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(),
+               workspace.max_seq_len, int(causal), d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(),
+               workspace.nbytes, out.data_ptr(), workspace.status.data_ptr())
     check(rc, "b200attn_paged_prefill")
     return out
 
