@@ -23,6 +23,7 @@
 // ticket; the last one joins the pieces in order, so the result does not depend on who is last, and sets the counter
 // back to zero.  Nobody waits for anybody.
 #include "paged.cuh"
+#include "streamk.cuh"
 
 namespace b200attn {
 
@@ -31,6 +32,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16 * kWarps;        // tokens the block takes per round
+constexpr int kWhole = 256;               // sequences up to this many tokens are not cut into pieces
 constexpr int kStage = 256;               // pages whose number and scales are in shared memory at a time
 constexpr float kPBits = 15.f;            // p is held times 2^15
 
@@ -94,10 +96,12 @@ paged_decode_kernel(const DecodeParams p) {
   __shared__ int s_last;
   extern __shared__ float s_acc[];        // [kWarps][G][D]
 
+  pdl_wait();
+  pdl_launch_dependents();
   const int len = paged_len(g, p.seq_len[b] + p.seq_len_offset, p.status, tid == 0 && split == 0 && h == 0 && layer == 0);
   // pieces: as many as the grid has room for, each a whole number of rounds
   const int rounds = (len + kUnit - 1) / kUnit;
-  const int per = (rounds + p.num_splits - 1) / p.num_splits;
+  const int per = rounds * kUnit <= kWhole ? rounds : (rounds + p.num_splits - 1) / p.num_splits;
   const int pieces = per > 0 ? (rounds + per - 1) / per : 0;
   if (split >= pieces) {
     if (pieces == 0 && split == 0)        // no tokens: zeros
@@ -361,27 +365,478 @@ paged_decode_kernel(const DecodeParams p) {
   }
 }
 
-// Pieces per pair: enough thread blocks for two rounds of a full GPU, none under 256 tokens.
-int decode_splits(const PagedGeometry& g, int max_seq_len) {
+// ---------------------------------------------------------------------------------------------
+// Much work: a persistent grid, the tiles of all pairs in one line divided evenly over it (stream-K), so that ragged batches of
+// any shape fill the GPU and end together.  A producer warp streams K and V tiles of 64 tokens with TMA into a ring, one box
+// per page (or piece of a page); four warps take 16 tokens of a tile each, as in the kernel above; an epilogue warp merges
+// their states, and the CTA that holds a split pair's last piece collects the others' (tagged words, see streamk.cuh).
+// ---------------------------------------------------------------------------------------------
+constexpr int kTileT = 64;
+constexpr int kThreadsP = (kConsumerWarps + 2) * 32;
+constexpr int kDumps = 2, kStages = 3;
+constexpr int kAhead = 8;                 // tiles whose pages and scales the producer looks up at a time
+
+struct PagedMma {
+  MmaParams m;                            // geometry (capacity = the table's), queries, lengths, workspace, output
+  PagedGeometry g;
+  const int* page_table;
+  int page_shift;
+};
+
+template <int D, int MINB>
+__global__ void __launch_bounds__(kThreadsP, MINB)
+paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedMma pp) {
+  constexpr int DH = D / 128;
+  constexpr int KSTEPS = D / 16;
+  constexpr int TILE_BYTES = kTileT * D;
+  constexpr int DP = D + 4;
+  const MmaParams& p = pp.m;
+  const Geometry& g = p.g;
+  const int G = g.group;
+  constexpr int stages = kStages;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int gq = lane >> 2, tq = lane & 3;
+  const uint32_t q_bytes = (uint32_t)G * D * 2;
+  const int dump_warp_floats = G * DP;
+
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  const uint32_t raw_addr = smem_u32(s_dyn);
+  uint8_t* smem = s_dyn + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + (size_t)stages * TILE_BYTES;
+  uint8_t* sQ = sV + (size_t)stages * TILE_BYTES;                                     // [2][G*D] bf16
+  float* sDump = reinterpret_cast<float*>(sQ + 2 * q_bytes);                          // [2][4][G][DP]
+  float* sML = sDump + kDumps * kConsumerWarps * dump_warp_floats;                    // [2][4][16]: m[8], l[8]
+  float2* sScale = reinterpret_cast<float2*>(sML + kDumps * kConsumerWarps * 16);     // [stages][4]: K and V scale of 16 tokens; K < 0: no page
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + stages * 4);
+  DeferredCombine* sComb = reinterpret_cast<DeferredCombine*>(bars + 2 * stages + 8);
+  int* sFlags = reinterpret_cast<int*>(sComb + 1);                                    // [0] timed_out [1] queries [2] flags [3] tiles copied [4] fewest tiles of a CTA
+  int* sLen = sFlags + 8;                                                             // [batch]
+  int* sCum = sLen + g.batch;                                                         // [batch+1]
+  volatile int* timed_out = sFlags;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8u * stages;
+  const uint32_t qfull0 = empty0 + 8u * stages, qempty0 = qfull0 + 16u;
+  const uint32_t dfull0 = qempty0 + 16u, dempty0 = dfull0 + 16u;
+
+  if (tid == 32) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full0 + 8u * s, 1);
+      mbar_init(empty0 + 8u * s, kConsumerWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(qfull0 + 8u * i, 1);
+      mbar_init(qempty0 + 8u * i, kConsumerWarps);
+      mbar_init(dfull0 + 8u * i, kConsumerWarps);
+      mbar_init(dempty0 + 8u * i, 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    sFlags[0] = 0; sFlags[1] = 0; sFlags[3] = 0;
+    sComb->valid = 0;
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+  }
+  if (warp == 0) {   // lengths, and the tiles before each sequence
+    pdl_wait();      // the kernel before this one has completed: lengths, cache and workspace are as it left them
+    int before = 0, first_tiles = 0, longest = 0;
+    bool any_empty = false, uniform = true;
+    for (int b0 = 0; b0 < g.batch; b0 += 32) {
+      const int b = b0 + lane;
+      const int len = b < g.batch ? paged_len(pp.g, p.seq_len[b] + p.seq_len_offset, p.status, blockIdx.x == 0) : 0;
+      const int n = (len + kTileT - 1) / kTileT;
+      if (b0 == 0) first_tiles = __shfl_sync(0xffffffffu, n, 0);
+      longest = max(longest, __reduce_max_sync(0xffffffffu, n));
+      any_empty |= __any_sync(0xffffffffu, b < g.batch && n == 0);
+      uniform &= __all_sync(0xffffffffu, b >= g.batch || n == first_tiles);
+      int inc = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += t;
+      }
+      if (b < g.batch) { sLen[b] = len; sCum[b] = before + inc - n; }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) { sCum[g.batch] = before; sFlags[2] = (any_empty ? 1 : 0) | (uniform ? 2 : 0); sFlags[4] = max(1, (int)ceilf(sqrtf((float)longest))); }
+  } else {
+    pdl_wait();
+  }
+  __syncthreads();
+  if (tid == 0) pdl_launch_dependents();
+
+  if (sFlags[2] & 1) {   // sequences without tokens: zeros
+    const long long rows = (long long)g.n_layers * g.batch;
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+      if (sLen[r % g.batch] == 0)
+        for (int i = tid; i < g.h_q * D / 2; i += kThreadsP) reinterpret_cast<uint32_t*>(p.out + r * g.h_q * D)[i] = 0u;
+  }
+  const long long total = (long long)sCum[g.batch] * g.h_kv * g.n_layers;
+  // A piece takes time with its tiles, a join with its pieces: at least the root of the longest sequence's tiles per CTA
+  // (one pair of 8192 tokens cut into 128 pieces: 92 us).
+  const long long most_ctas = max(1LL, total / sFlags[4]);
+  int n_eff;
+  long long r0, r1;
+  cta_range(total, (int)min((long long)gridDim.x, most_ctas), (int)blockIdx.x, (sFlags[2] & 2) ? sCum[1] - sCum[0] : 0, n_eff, r0, r1);
+  const bool has_work = r0 < r1;
+
+  if (warp == kProducerWarp) {
+    if (has_work) {
+      // Lane 4 k + i looks up the page and the scales of tokens 16 i .. of the k-th tile of the next kAhead; the lane of a box's
+      // first 16 tokens (a box: a page, or the 64 tokens of the tile that a larger page holds) then issues its copies.
+      const uint64_t policy = l2_policy_evict_first();
+      const int box_rows = min(pp.g.page_size, kTileT), n_it = (int)(r1 - r0);
+      int id = -1, row = 0, layer = 0, seg_pair = -1, pair = 0, seg = 0;
+      float2 sc = make_float2(0.f, 0.f);
+      auto look_up = [&](int it0, int& id_, int& row_, int& layer_, int& pair_, float2& sc_) {
+        id_ = -1; row_ = 0; sc_ = make_float2(0.f, 0.f); layer_ = 0; pair_ = 0;
+        const int it = it0 + (lane >> 2);
+        if (it >= n_it) return;
+        const Cursor c = locate(r0 + it, sCum, sLen, g.batch, g.h_kv);
+        layer_ = c.layer;
+        pair_ = (c.layer * g.batch + c.b) * g.h_kv + c.h;
+        const int tok = c.tile * kTileT + (lane & 3) * 16;
+        if (tok >= c.len_b) return;
+        const int page = __ldg(pp.page_table + (long long)c.b * pp.g.max_pages + (tok >> pp.page_shift));
+        if (page < 0 || page >= pp.g.n_pages) {
+          atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
+          sc_.x = -1.f;
+          return;
+        }
+        id_ = page;
+        row_ = ((page * g.h_kv + c.h) << pp.page_shift) + (tok & (pp.g.page_size - 1));
+        const long long si = ((long long)c.layer * pp.g.n_pages + page) * g.h_kv + c.h;
+        sc_ = make_float2(__ldg(p.k_scale + si), __ldg(p.v_scale + si));
+      };
+      int id2, row2, layer2, pair2_;
+      float2 sc2;
+      look_up(0, id, row, layer, pair, sc);
+      bool ok = true;
+      for (int it0 = 0; it0 < n_it && ok; it0 += kAhead) {
+        look_up(it0 + kAhead, id2, row2, layer2, pair2_, sc2);
+        for (int k = 0; k < kAhead && it0 + k < n_it; ++k) {
+          const int it = it0 + k, s = it % stages;
+          const int cur_pair = __shfl_sync(0xffffffffu, pair, 4 * k);
+          if (cur_pair != seg_pair) {   // the G query rows of this pair
+            const int qb = seg & 1;
+            if (seg >= 2) ok = mbar_wait(qempty0 + 8u * qb, ((seg >> 1) - 1) & 1, timed_out, p.status);
+            __syncwarp();
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(qfull0 + 8u * qb, q_bytes);
+              const int lb = cur_pair / g.h_kv;
+              bulk_load(smem_u32(sQ + qb * q_bytes), p.q + ((long long)lb * g.h_q + (cur_pair - lb * g.h_kv) * G) * D, q_bytes, qfull0 + 8u * qb);
+            }
+            seg_pair = cur_pair;
+            ++seg;
+          }
+          if (it >= stages) ok = mbar_wait(empty0 + 8u * s, ((it / stages) - 1) & 1, timed_out, p.status);
+          __syncwarp();
+          if (!ok) break;
+          const uint32_t fb = full0 + 8u * s;
+          const bool mine = (lane >> 2) == k;
+          if (mine) sScale[s * 4 + (lane & 3)] = sc;
+          const bool box = mine && id >= 0 && ((lane & 3) * 16) % box_rows == 0;
+          const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, box));
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(fb, 2u * boxes * box_rows * D);
+          __syncwarp();
+          if (box) {
+#pragma unroll
+            for (int hf = 0; hf < DH; ++hf) {
+              const uint32_t off = (uint32_t)s * TILE_BYTES + hf * kTileT * 128 + (lane & 3) * 16 * 128;
+              tma_load_3d_hint(smem_u32(sK) + off, &kmap, hf * 128, row, layer, fb, policy);
+              tma_load_3d_hint(smem_u32(sV) + off, &vmap, hf * 128, row, layer, fb, policy);
+            }
+          }
+          if (lane == 0) { sFlags[3] = it + 1; sFlags[1] = seg; }   // for the drain after a wait that ran out
+        }
+        id = id2; row = row2; layer = layer2; pair = pair2_; sc = sc2;
+      }
+    }
+  } else if (warp == kEpilogueWarp) {
+    if (has_work)
+      epilogue_warp<D, kDumps, kConsumerWarps, false, true>(p, lane, r0, r1, total, n_eff, sCum, sLen, sDump, sML, dfull0, dempty0, timed_out,
+                                                           nullptr, sComb, 0);
+  } else if (has_work) {
+    Cursor c = locate(r0, sCum, sLen, g.batch, g.h_kv);
+    long long cur = r0;
+    int it = 0, seg = 0;
+    const uint32_t sK_addr = smem_u32(sK), sV_addr = smem_u32(sV);
+    const int row_lo = warp * 16 + gq;
+    while (cur < r1) {
+      const long long pair_end = cur - c.tile + c.tiles_b, seg_end = pair_end < r1 ? pair_end : r1;
+      const int ntiles = (int)(seg_end - cur), qb = seg & 1;
+      // ---- query fragments: head gq, dims hf * 128 + 32 tq + 4 ks ..; each head scaled by a power of two into f16's range ----
+      uint32_t qf[KSTEPS][2];
+      float sc0, sc1;
+      {
+        const bool qok = mbar_wait(qfull0 + 8u * qb, (seg >> 1) & 1, timed_out, p.status);
+        float qv[DH][32];
+        float amax = 0.f;
+#pragma unroll
+        for (int hf = 0; hf < DH; ++hf)
+#pragma unroll
+          for (int v4 = 0; v4 < 4; ++v4) {
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (gq < G && qok) raw = lds128(smem_u32(sQ + qb * q_bytes) + (gq * D + 32 * tq) * 2 + hf * 256 + v4 * 16);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              qv[hf][v4 * 8 + 2 * i] = bf16_bits_to_float(w[i] & 0xFFFFu);
+              qv[hf][v4 * 8 + 2 * i + 1] = bf16_bits_to_float(w[i] >> 16);
+              amax = fmaxf(amax, fmaxf(fabsf(qv[hf][v4 * 8 + 2 * i]), fabsf(qv[hf][v4 * 8 + 2 * i + 1])));
+            }
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qempty0 + 8u * qb);
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        int ex = (int)((__float_as_uint(amax) >> 23) & 0xFF);
+        ex = ex < 1 ? 1 : (ex > 253 ? 253 : ex);
+        const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+        for (int hf = 0; hf < DH; ++hf)
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            const __half2 b0 = __floats2half2_rn(qv[hf][4 * w] * down, qv[hf][4 * w + 1] * down);
+            const __half2 b1 = __floats2half2_rn(qv[hf][4 * w + 2] * down, qv[hf][4 * w + 3] * down);
+            qf[hf * 8 + w][0] = *reinterpret_cast<const uint32_t*>(&b0);
+            qf[hf * 8 + w][1] = *reinterpret_cast<const uint32_t*>(&b1);
+          }
+        const float mult = up * p.score_scale;
+        sc0 = __shfl_sync(0xffffffffu, mult, 8 * tq);
+        sc1 = __shfl_sync(0xffffffffu, mult, 8 * tq + 4);
+      }
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, r = 0.f, inv_r = 0.f;
+      float o[KSTEPS][4];
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
+
+      for (int ti = 0; ti < ntiles; ++ti, ++it) {
+        const int s = it % stages;
+        const bool ok = mbar_wait(full0 + 8u * s, (it / stages) & 1, timed_out, p.status);
+        const int tok0 = (c.tile + ti) * kTileT + warp * 16;
+        const float2 sc = sScale[s * 4 + warp];
+        if (ok && tok0 < c.len_b && sc.x >= 0.f) {
+          float sacc[4] = {0.f, 0.f, 0.f, 0.f}, sacc2[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint32_t kt = sK_addr + s * TILE_BYTES;
+#pragma unroll
+          for (int hf = 0; hf < DH; ++hf)
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+              const uint32_t off = hf * kTileT * 128 + (((2 * tq + ch) ^ gq) << 4);
+              const uint4 klo = lds128(kt + off + row_lo * 128), khi = lds128(kt + off + (row_lo + 8) * 128);
+              const uint32_t wl[4] = {klo.x, klo.y, klo.z, klo.w}, wh[4] = {khi.x, khi.y, khi.z, khi.w};
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+                mma_f16((w & 1) ? sacc2 : sacc, cvt_lo(wl[w]), cvt_lo(wh[w]), cvt_hi(wl[w]), cvt_hi(wh[w]), qf[hf * 8 + ch * 4 + w][0], qf[hf * 8 + ch * 4 + w][1]);
+            }
+          const float c0 = sc0 * sc.x, c1 = sc1 * sc.x;
+          float s0 = (sacc[0] + sacc2[0]) * c0, s1 = (sacc[1] + sacc2[1]) * c1, s2 = (sacc[2] + sacc2[2]) * c0, s3 = (sacc[3] + sacc2[3]) * c1;
+          if (tok0 + gq >= c.len_b) { s0 = -INFINITY; s1 = -INFINITY; }
+          if (tok0 + gq + 8 >= c.len_b) { s2 = -INFINITY; s3 = -INFINITY; }
+          float mx0 = fmaxf(s0, s2), mx1 = fmaxf(s1, s3);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+          }
+          const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+          const float b0 = n0 == -INFINITY ? 0.f : n0 - kPBits, b1 = n1 == -INFINITY ? 0.f : n1 - kPBits;
+          float a0 = ex2(m0 - kPBits - b0), a1 = ex2(m1 - kPBits - b1);
+          const float p0 = ex2(s0 - b0), p1 = ex2(s1 - b1), p2 = ex2(s2 - b0), p3 = ex2(s3 - b1);
+          m0 = n0; m1 = n1;
+          l0 = l0 * a0 + (p0 + p2);
+          l1 = l1 * a1 + (p1 + p3);
+          if (sc.y > r) {                 // a page with a larger V scale (the same for the whole warp)
+            a0 *= r / sc.y; a1 *= r / sc.y;
+            r = sc.y;
+            inv_r = 1.f / r;
+          }
+          if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j) { o[j][0] *= a0; o[j][1] *= a1; o[j][2] *= a0; o[j][3] *= a1; }
+          }
+          const float vs = sc.y * inv_r;
+          const __half2 pa = __floats2half2_rn(p0 * vs, p1 * vs), pb = __floats2half2_rn(p2 * vs, p3 * vs);
+          const uint32_t pb0 = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&pa)), pb1 = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&pb));
+          const uint32_t vt = sV_addr + s * TILE_BYTES;
+          const int vr = warp * 16 + 2 * tq;
+          const bool tail = tok0 + 16 > c.len_b;
+#pragma unroll
+          for (int hf = 0; hf < DH; ++hf) {
+            const uint32_t vb = vt + hf * kTileT * 128;
+            uint4 va = lds128(vb + vr * 128 + ((gq ^ (2 * tq)) << 4)), vbb = lds128(vb + (vr + 1) * 128 + ((gq ^ (2 * tq + 1)) << 4));
+            uint4 vc = lds128(vb + (vr + 8) * 128 + ((gq ^ (2 * tq)) << 4)), vd = lds128(vb + (vr + 9) * 128 + ((gq ^ (2 * tq + 1)) << 4));
+            if (tail) {                   // slots behind the last token may hold anything, NaN patterns included
+              const int tv = tok0 + 2 * tq;
+              const uint4 z = make_uint4(0, 0, 0, 0);
+              if (tv >= c.len_b) va = z;
+              if (tv + 1 >= c.len_b) vbb = z;
+              if (tv + 8 >= c.len_b) vc = z;
+              if (tv + 9 >= c.len_b) vd = z;
+            }
+            const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vbb.x, vbb.y, vbb.z, vbb.w};
+            const uint32_t wc[4] = {vc.x, vc.y, vc.z, vc.w}, wd[4] = {vd.x, vd.y, vd.z, vd.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t x01 = prmt(wa[w], wb[w], 0x5140), x23 = prmt(wa[w], wb[w], 0x7362), y01 = prmt(wc[w], wd[w], 0x5140), y23 = prmt(wc[w], wd[w], 0x7362);
+              mma_f16(o[hf * 8 + 2 * w], cvt_lo(x01), cvt_hi(x01), cvt_lo(y01), cvt_hi(y01), pb0, pb1);
+              mma_f16(o[hf * 8 + 2 * w + 1], cvt_lo(x23), cvt_hi(x23), cvt_lo(y23), cvt_hi(y23), pb0, pb1);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty0 + 8u * s);
+      }
+      // ---- end of the segment: the warp's state to the epilogue warp ----
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+      }
+      const int db = seg % kDumps;
+      if (seg < kDumps || mbar_wait(dempty0 + 8u * db, ((seg / kDumps) - 1) & 1, timed_out, p.status)) {
+        float* ml = sML + (db * kConsumerWarps + warp) * 16;
+        if (gq == 0) {
+          ml[2 * tq] = m0; ml[2 * tq + 1] = m1;
+          ml[8 + 2 * tq] = l0; ml[8 + 2 * tq + 1] = l1;
+        }
+        const uint32_t dbase = smem_u32(sDump + (db * kConsumerWarps + warp) * dump_warp_floats);
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j) {   // regs 0, 1: dim (j >> 3) * 128 + 16 gq + 2 (j & 7) of heads 2 tq, 2 tq + 1; regs 2, 3: that dim + 1
+          const int u = (j >> 3) * 64 + 8 * gq + (j & 7);
+          const uint32_t pos8 = 8u * (uint32_t)((u & ~7) | ((j & 7) ^ gq));
+          if (2 * tq < G) sts64(dbase + 2 * tq * DP * 4 + pos8, o[j][0] * r, o[j][2] * r);
+          if (2 * tq + 1 < G) sts64(dbase + (2 * tq + 1) * DP * 4 + pos8, o[j][1] * r, o[j][3] * r);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dfull0 + 8u * db);
+      ++seg;
+      cur = seg_end;
+      if (cur < r1) next_pair(c, sCum, sLen, g.batch, g.h_kv);
+    }
+  }
+  __syncthreads();
+  if (sFlags[0] && tid == kConsumerThreads) {
+    // A wait ran out.  Copies already issued still land in this CTA's shared memory: wait for them (bounded).
+    const int n_it = sFlags[3], segs = sFlags[1];
+    for (int s = 0; s < stages && s < n_it; ++s) {
+      const int last = ((n_it - 1 - s) / stages) * stages + s;
+      const unsigned long long t0 = global_timer_ns();
+      while (!mbar_try_wait(full0 + 8u * s, (last / stages) & 1) && global_timer_ns() - t0 < kWaitBudgetNs) {}
+    }
+    for (int qb = 0; qb < 2 && qb < segs; ++qb) {
+      const int last = ((segs - 1 - qb) / 2) * 2 + qb;
+      const unsigned long long t0 = global_timer_ns();
+      while (!mbar_try_wait(qfull0 + 8u * qb, (last >> 1) & 1) && global_timer_ns() - t0 < kWaitBudgetNs) {}
+    }
+  }
+  if (sComb->valid && !sFlags[0]) combine_deferred<D>(combine_args_of(p, nullptr, 0), *sComb, warp, kThreadsP / 32, lane);
+}
+
+size_t streamk_smem(const PagedGeometry& g) {
+  size_t b = 1024;
+  b += (size_t)2 * kStages * kTileT * g.head_dim;
+  b += (size_t)2 * g.group * g.head_dim * 2;
+  b += (size_t)kDumps * kConsumerWarps * g.group * (g.head_dim + 4) * 4;
+  b += (size_t)kDumps * kConsumerWarps * 16 * 4;
+  b += (size_t)kStages * 4 * 8;
+  b += (size_t)(2 * kStages + 8) * 8;
+  b += sizeof(DeferredCombine) + 32;
+  b += (size_t)(2 * g.batch + 1) * 4;
+  return (b + 15) & ~(size_t)15;
+}
+// CTAs of the persistent grid: every slot of the device (three per SM with heads of 128).
+int streamk_ctas(const PagedGeometry& g) {
+  int per_sm = (int)((227 * 1024) / (streamk_smem(g) + 1024));
+  const int most = g.head_dim == 128 ? 3 : 1;
+  per_sm = per_sm < 1 ? 1 : per_sm > most ? most : per_sm;
+  return per_sm * device_sms();
+}
+
+// Longest sequence a call can meet, as far as the host knows.
+long long most_tokens(const PagedGeometry& g, int max_seq_len) {
   const long long cap = (long long)g.max_pages * g.page_size;
-  const long long most = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
-  const long long pairs = (long long)g.n_layers * g.batch * g.h_kv;
+  return max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
+}
+
+// Which kernel: the register kernel starts and ends faster, the stream-K kernel streams faster and balances.  Heads of 128,
+// register / stream-K, us: 256 tokens, 8 pairs 7.0 / 9.6, 1024 pairs 21.0 / 27.6; 1024 tokens, 8 pairs 9.3 / 14.7, 1024 pairs
+// 55 / 64; 2048 tokens, 64 pairs 15.4 / 20.3, 256 pairs 41 / 37, 1024 pairs 100 / 102; 8192 tokens, 8 pairs 16 / 35, 64 pairs
+// 46 / 38, 1024 pairs 366 / 343.  Heads of 256 cross over at about half as many tokens.
+bool use_streamk(const PagedGeometry& g, int max_seq_len) {
+  if (g.batch > kMaxBatchMma || (long long)g.n_pages * g.h_kv * g.page_size > 0x7fffffffLL) return false;
+  const long long bytes = most_tokens(g, max_seq_len) * g.head_dim, pairs = (long long)g.n_layers * g.batch * g.h_kv;
+  return bytes > 1024 * 128 && bytes * pairs > 131072LL * 128;
+}
+
+// Register kernel: pieces per pair.  Joining costs about 4 us and grows with their number, so few pairs are cut into up to 16,
+// and many pairs not at all (8 pairs of 512 tokens: 8 pieces 8.1 us, whole 9.6; of 8192: 32 pieces 16 us, 128 pieces 39;
+// 256 pairs of 512: 3 pieces 21 us, whole 14).
+int decode_splits(const PagedGeometry& g, int max_seq_len) {
+  const long long most = most_tokens(g, max_seq_len), pairs = (long long)g.n_layers * g.batch * g.h_kv;
   const long long slots = (long long)device_sms() * (g.head_dim == 128 ? 4 : 2);
-  long long want = (2 * slots + pairs - 1) / pairs;
-  const long long by_len = (most + 255) / 256;
-  if (want > by_len) want = by_len;
-  return (int)(want < 1 ? 1 : want > 128 ? 128 : want);
+  long long n = slots / pairs;
+  const long long by_len = (most + kUnit - 1) / kUnit;
+  n = n < by_len ? n : by_len;
+  return most <= kWhole || n < 4 ? 1 : n > 16 ? 16 : (int)n;
 }
 
 }  // namespace
 
 size_t paged_decode_workspace_bytes(const PagedGeometry& g, int max_seq_len) {
+  Geometry q{};
+  q.group = g.group; q.head_dim = g.head_dim;
+  if (use_streamk(g, max_seq_len)) return mma_workspace_bytes(q, streamk_ctas(g));
   const size_t pairs = (size_t)g.n_layers * g.batch * g.h_kv, splits = decode_splits(g, max_seq_len);
   if (splits == 1) return 0;
   return pairs * splits * ((size_t)g.group * g.head_dim + 16) * 4 + pairs * 4;
 }
 
+namespace {
+
+cudaError_t launch_paged_streamk(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
+  Geometry cache{};
+  cache.n_layers = g.n_layers; cache.batch = g.n_pages; cache.h_kv = g.h_kv; cache.capacity = g.page_size; cache.head_dim = g.head_dim;
+  const int box = g.page_size < kTileT ? g.page_size : kTileT;
+  CUtensorMap kmap, vmap;
+  if (!encode_cache_map(&kmap, a.k_pages, cache, g.k_layer_stride, box) || !encode_cache_map(&vmap, a.v_pages, cache, g.v_layer_stride, box))
+    return cudaErrorInvalidValue;
+  PagedMma p{};
+  p.g = g;
+  p.page_table = a.page_table;
+  p.page_shift = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
+  MmaParams& m = p.m;
+  m.g.n_layers = g.n_layers; m.g.batch = g.batch; m.g.h_q = g.h_q; m.g.h_kv = g.h_kv; m.g.head_dim = g.head_dim; m.g.group = g.group;
+  m.g.capacity = g.max_pages * g.page_size;
+  m.q = (const uint16_t*)a.q;
+  m.k_scale = a.k_scale; m.v_scale = a.v_scale;
+  m.seq_len = a.seq_len;
+  m.seq_len_offset = a.seq_len_offset;
+  m.score_scale = a.softmax_scale * kLog2e;
+  m.ws_pkt = (unsigned long long*)a.workspace;
+  m.out = (uint16_t*)a.out;
+  m.out_hq_total = g.h_q;
+  m.status = a.status;
+  const int n = streamk_ctas(g);
+  const size_t smem = streamk_smem(g);
+  auto launch = [&](auto kernel) -> cudaError_t {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, n, kThreadsP, smem, stream, kmap, vmap, p);
+  };
+  if (g.head_dim != 128) return launch(paged_streamk_kernel<256, 1>);
+  return n <= 2 * device_sms() ? launch(paged_streamk_kernel<128, 2>) : launch(paged_streamk_kernel<128, 3>);
+}
+
+}  // namespace
+
 cudaError_t launch_paged_decode(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
+  if (use_streamk(g, a.max_seq_len)) return launch_paged_streamk(g, a, stream);
   DecodeParams p{};
   p.g = g;
   p.q = (const uint16_t*)a.q;
@@ -398,14 +853,9 @@ cudaError_t launch_paged_decode(const PagedGeometry& g, const PagedAttnArgs& a, 
   p.status = a.status;
   const long long grid = pairs * p.num_splits;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  const size_t smem = (size_t)kWarps * g.group * g.head_dim * 4;
-  auto launch = [&](auto kernel) -> cudaError_t {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)grid, kThreads, smem, stream>>>(p);
-    return cudaGetLastError();
-  };
-  return g.head_dim == 128 ? launch(paged_decode_kernel<128>) : launch(paged_decode_kernel<256>);
+  const size_t smem = (size_t)kWarps * g.group * g.head_dim * 4;   // at most 32 KB
+  return g.head_dim == 128 ? launch_pdl(paged_decode_kernel<128>, (int)grid, kThreads, smem, stream, p)
+                           : launch_pdl(paged_decode_kernel<256>, (int)grid, kThreads, smem, stream, p);
 }
 
 }  // namespace b200attn

@@ -9,11 +9,11 @@ pytestmark = pytest.mark.gpu
 HEADS = [(40, 8, 128), (24, 4, 256), (8, 1, 128), (3, 3, 128), (7, 1, 256)]
 
 
-def _run_attention(pkg, dev, case, *, causal=None, qlens=None, seed=0, offset=0, hint=None, softmax_scale=None, table_edit=None):
+def _run_attention(pkg, dev, case, *, causal=None, qlens=None, seed=0, offset=0, hint=None, softmax_scale=None, spare_pages=2):
     """Decode (qlens None) or prefill of ragged sequences; compares every sequence with the 64-bit form."""
     n_layers, (h_q, h_kv, d), page, lens = case
     g = torch.Generator().manual_seed(seed)
-    width = max(1, max(-(-n // page) for n in lens)) + 2
+    width = max(1, max(-(-n // page) for n in lens)) + spare_pages
     n_pages = sum(-(-n // page) for n in lens) + 3
     kb, vb, ks, vs = ref.random_cache(g, n_layers, n_pages, h_kv, page, d, pow2=seed % 2 == 0)
     table = ref.random_table(g, lens, page, width, n_pages)
@@ -397,3 +397,75 @@ def test_prefill_enough_rows_for_the_whole_gpu(pkg, cuda_device, causal):
     pair, or a pair whose second tile has one token."""
     _run_attention(pkg, cuda_device, (1, (40, 8, 128), 64, [700, 1000, 26, 80, 25]), qlens=[700, 333, 26, 51, 25], causal=causal, seed=31)
     _run_attention(pkg, cuda_device, (1, (16, 16, 128), 32, [600, 129]), qlens=[600, 129], causal=causal, seed=32)
+
+
+def _spare(pairs, d, page):
+    """Table columns that make the largest possible call a large one, whatever the lengths are."""
+    return max(1100 * 128 // d, 133000 * 128 // (d * pairs)) // page + 2
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_decode_lengths_in_a_wide_table(pkg, cuda_device, heads, page):
+    """Empty, one token, ends inside and at the end of pages and tiles, far below what the table could hold."""
+    lens = [0, 1, 15, 16, 17, 63, 64, 65, 0, 127, 128, 129, 300, 511, 1000]
+    _run_attention(pkg, cuda_device, (1, heads, page, lens), seed=page, spare_pages=_spare(len(lens) * heads[1], heads[2], page))
+
+
+@pytest.mark.parametrize("heads", [(8, 1, 128), (5, 1, 256), (20, 4, 128)])
+def test_decode_one_long_sequence_and_layers(pkg, cuda_device, heads):
+    """One pair on the whole GPU (many pieces to join); layers of a long and short sequences; equal short lengths."""
+    _run_attention(pkg, cuda_device, (1, heads, 32, [20011]), seed=40, spare_pages=_spare(heads[1], heads[2], 32))
+    _run_attention(pkg, cuda_device, (3, heads, 128, [7000, 1, 2049]), seed=41, spare_pages=_spare(9 * heads[1], heads[2], 128))
+    _run_attention(pkg, cuda_device, (2, heads, 64, [320, 320, 320]), seed=42, spare_pages=_spare(6 * heads[1], heads[2], 64), hint=500000)
+    _run_attention(pkg, cuda_device, (1, heads, 16, [0, 0]), seed=43, spare_pages=_spare(2 * heads[1], heads[2], 16))
+
+
+def test_decode_more_sequences_than_one_block_can_list(pkg, cuda_device):
+    lens = [i * 7 % 40 for i in range(2100)]
+    _run_attention(pkg, cuda_device, (1, (3, 3, 128), 16, lens), seed=44, spare_pages=80)
+
+
+def test_bad_page_numbers_in_a_wide_table(pkg, cuda_device):
+    g = torch.Generator().manual_seed(2)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 4, 1, 16, 128)
+    q = torch.randn(1, 2, 5, 128, generator=g).to(torch.bfloat16)
+    for bad in (-1, 4, 1 << 30):
+        table = torch.full((2, 5000), bad, dtype=torch.int32)
+        table[0, :6] = torch.tensor([2, bad, 1, bad, bad, 3])     # the second sequence has bad pages only
+        up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+        ws = pkg.PagedWorkspace(pkg.make_paged_shape(5, kb, vb, ks, table), cuda_device)
+        lens = torch.tensor([90, 300], dtype=torch.int32, device=cuda_device)
+        out = pkg.paged_decode_attention(q.to(cuda_device), *up, lens, workspace=ws).cpu()
+        want, big = ref.attention(q[0, :1], kb[0], vb[0], ks[0], vs[0], torch.tensor([2, 1, 3]), 42)
+        ref.assert_attention(out[0, :1], want, big, bad)
+        assert (out[0, 1] == 0).all()
+        assert ws.read_status() == pkg._lib.STATUS_BAD_PAGE
+
+
+def test_ragged_batch_launched_many_times(pkg, cuda_device):
+    """Launches back to back, eager and as one graph: no wait runs out, and the bits stay the same."""
+    g = torch.Generator().manual_seed(6)
+    lens = [(i * 613) % 3000 + 1 for i in range(32)]
+    kb, vb, ks, vs = ref.random_cache(g, 1, 900, 8, 64, 128)
+    table = torch.randint(0, 900, (32, 256), generator=g).to(torch.int32)
+    q = torch.randn(1, 32, 40, 128, generator=g).to(torch.bfloat16).to(cuda_device)
+    up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    shape = pkg.make_paged_shape(40, kb, vb, ks, table)
+    ws, outs = [pkg.PagedWorkspace(shape, cuda_device) for _ in range(2)], [torch.empty_like(q) for _ in range(2)]
+    for i in range(4000):
+        pkg.paged_decode_attention(q, *up, n, workspace=ws[i % 2], out=outs[i % 2])
+    first = outs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(8):
+            pkg.paged_decode_attention(q, *up, n, workspace=ws[i % 2], out=outs[i % 2])
+    for _ in range(500):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, outs[0]) and torch.equal(first, outs[1])
+    assert [w.read_status() for w in ws] == [0, 0]
+    for b in (0, 7, 31):
+        want, big = ref.attention(q[0, b:b + 1].cpu(), kb[0], vb[0], ks[0], vs[0], table[b], lens[b])
+        ref.assert_attention(first[0, b:b + 1].cpu(), want, big)
