@@ -32,6 +32,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16 * kWarps;        // tokens the block takes per round
+constexpr int kMostPieces = 16;           // of a sequence
 constexpr int kWhole = 256;               // sequences up to this many tokens are not cut into pieces
 constexpr int kStage = 256;               // pages whose number and scales are in shared memory at a time
 constexpr float kPBits = 15.f;            // p is held times 2^15
@@ -347,17 +348,30 @@ paged_decode_kernel(const DecodeParams p) {
   if (tid == 0) p.counters[pair] = 0;
   for (int i = tid; i < G * D / 4; i += kThreads) {
     const int j = i / (D / 4);
-    float M = -INFINITY, L = 0.f;
+    float M = -INFINITY, L = 0.f, f[kMostPieces];
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int s = 0; s < pieces; ++s) M = fmaxf(M, __ldcg(part + s * stride + G * D + j));
-#pragma unroll 8
-    for (int s = 0; s < pieces; ++s) {
-      const float ms = __ldcg(part + s * stride + G * D + j);
-      const float f = ms == -INFINITY ? 0.f : ex2f(ms - M);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(part + s * stride) + i);
-      L += __ldcg(part + s * stride + G * D + 8 + j) * f;
-      a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
+#pragma unroll
+    for (int s = 0; s < kMostPieces; ++s) {   // all loads of a group in flight together, whatever the number of pieces
+      f[s] = s < pieces ? __ldcg(part + s * stride + G * D + j) : -INFINITY;
+      M = fmaxf(M, f[s]);
+    }
+#pragma unroll
+    for (int s0 = 0; s0 < kMostPieces; s0 += 8) {
+      if (s0 >= pieces) break;
+      float4 v[8];
+      float l[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float* from = part + min(s0 + s, pieces - 1) * stride;
+        v[s] = __ldcg(reinterpret_cast<const float4*>(from) + i);
+        l[s] = __ldcg(from + G * D + 8 + j);
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float w = f[s0 + s] == -INFINITY ? 0.f : ex2f(f[s0 + s] - M);
+        L += l[s] * w;
+        a.x += v[s].x * w; a.y += v[s].y * w; a.z += v[s].z * w; a.w += v[s].w * w;
+      }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
     const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
@@ -783,7 +797,7 @@ int decode_splits(const PagedGeometry& g, int max_seq_len) {
   long long n = slots / pairs;
   const long long by_len = (most + kUnit - 1) / kUnit;
   n = n < by_len ? n : by_len;
-  return most <= kWhole || n < 4 ? 1 : n > 16 ? 16 : (int)n;
+  return most <= kWhole || n < 4 ? 1 : n > kMostPieces ? kMostPieces : (int)n;
 }
 
 }  // namespace
