@@ -266,6 +266,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   rest /= g.h_kv;
   const int layer = rest % g.n_layers, number = p.tiles - 1 - rest / g.n_layers;
   const int per_tile = kRows / G, per_block = per_tile << p.pair;   // query tokens of a tile, of a block
+  pdl_wait();
   if (warp == 0) {
     int before = 0;
     if (lane == 0) s_info[0] = -1;
@@ -620,57 +621,66 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     const bool real = row / G < per_tile && tok < ntok;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     regs_up<P::REGS_SOFTMAX>();
-    // The query rows as two e4m3 rows each.  A warp takes 32 rows (16 where two groups share a tile), D / 8 lanes per row, and has
-    // all its loads in flight before it looks at the first; every thread then picks up the multiplier of its own row.
+    // The query rows as two e4m3 rows each.  A warp takes 32 rows (16 where two groups share a tile), D / 8 lanes per row.  It copies
+    // all of them into the place of their result (16 bytes of bf16 become 8 of the first row and 8 of the second; the lanes of two
+    // neighbouring chunks write where they have read), then converts four loads at a time.  Every thread then picks up the multiplier
+    // of its own row.
     const bool halves = NS == 2 && !two;
     float rowmul;
     {
-      constexpr int LPR = D / 8, RPL = 32 / LPR, BATCH = 16;  // lanes per row, rows per load, loads in flight
+      constexpr int LPR = D / 8, RPL = 32 / LPR, BATCH = 4;   // lanes per row, rows per step, steps at a time
       const uint32_t sq = sQ + (two ? grp * P::QTILE : 0);
       float* s_mul = s_rowmul[two ? grp : 0];
-      const int first = halves ? warp * 16 : (warp & 3) * 32, loads = (halves ? 16 : 32) / RPL;
-      const int sub = lane / LPR, c8 = lane % LPR;            // row of the load, 8 dims of it
+      const int first = halves ? warp * 16 : (warp & 3) * 32, steps = (halves ? 16 : 32) / RPL;
+      const int sub = lane / LPR, c8 = lane % LPR, c = c8 >> 1;   // row of the step, 8 dims of it, their 16-byte chunk of the result
+      const uint32_t over_g = (65536u + G - 1) / G;           // r / G = r * over_g >> 16 for r < 128, G <= 8
+      const uint32_t base = sq + (uint32_t)(c >> 3) * (kRows * 128), odd = (c8 & 1) * (uint32_t)(DH * kRows * 128);
+      const int last_row = min(per_tile, ntok - tile_tok) * G;    // rows from here on are no token's
+      const uint16_t* q0_ptr = p.q + (out_row0 + (long long)tile_tok * g.h_q) * D + c8 * 8;
+#pragma unroll 4
+      for (int i = 0; i < steps; ++i) {
+        const int r = first + i * RPL + sub, rt = (int)(r * over_g >> 16);
+        const uint16_t* from = r < last_row ? q0_ptr + (rt * g.h_q + (r - rt * G)) * D : p.q;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + odd), "l"(from), "r"(r < last_row ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
 #pragma unroll 1
-      for (int i0 = 0; i0 < loads; i0 += BATCH) {
-        uint4 raw[BATCH];
+      for (int i0 = 0; i0 < steps; i0 += BATCH) {
+        uint32_t w[BATCH][4], top[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-          const int r = first + (i0 + i) * RPL + sub, t = tile_tok + r / G;
-          raw[i] = make_uint4(0, 0, 0, 0);
-          if (i0 + i < loads && r / G < per_tile && t < ntok)
-            raw[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (out_row0 + (long long)t * g.h_q + r % G) * D) + c8);
+          const int r = first + (i0 + i) * RPL + sub;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                       : "r"(base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + odd));
         }
 #pragma unroll
+        for (int i = 0; i < BATCH; ++i)   // the largest |q| of the row: bf16 magnitudes compare as integers
+          top[i] = __vmaxu2(__vmaxu2(w[i][0] & 0x7FFF7FFFu, w[i][1] & 0x7FFF7FFFu), __vmaxu2(w[i][2] & 0x7FFF7FFFu, w[i][3] & 0x7FFF7FFFu));
+#pragma unroll
+        for (int off = LPR / 2; off > 0; off >>= 1)
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+        __syncwarp();                                         // both lanes of a chunk have read
+#pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-          if (i0 + i < loads) {
-            const int r = first + (i0 + i) * RPL + sub;
-            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-            float x[8], amax = 0.f;
+          const int r = first + (i0 + i) * RPL + sub;
+          int ex = (int)(max(top[i] & 0xFFFFu, top[i] >> 16) >> 7);
+          ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
+          const float down = __uint_as_float((uint32_t)(261 - ex) << 23);   // brings the largest |q| into [128, 256)
+          if (c8 == 0) s_mul[r] = __uint_as_float((uint32_t)(ex - 7) << 23) * p.score_scale;
+          uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[2 * e] = __uint_as_float(w[e] << 16);
-              x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-              amax = max3(amax, fabsf(x[2 * e]), fabsf(x[2 * e + 1]));
-            }
-#pragma unroll
-            for (int off = LPR / 2; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-            int ex = (int)((__float_as_uint(amax) >> 23) & 0xFF);
-            ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
-            const float down = __uint_as_float((uint32_t)(261 - ex) << 23);   // brings the largest |q| into [128, 256)
-            if (c8 == 0) s_mul[r] = __uint_as_float((uint32_t)(ex - 7) << 23) * p.score_scale;
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float x0 = x[4 * e] * down, x1 = x[4 * e + 1] * down, x2 = x[4 * e + 2] * down, x3 = x[4 * e + 3] * down;
-              const float h0 = e4m3_head(x0), h1 = e4m3_head(x1), h2 = e4m3_head(x2), h3 = e4m3_head(x3);
-              hi[e] = pack_e4m3x2(h0, h1) | (pack_e4m3x2(h2, h3) << 16);
-              lo[e] = pack_e4m3x2(x0 - h0, x1 - h1) | (pack_e4m3x2(x2 - h2, x3 - h3) << 16);
-            }
-            const int c = c8 >> 1;                            // 16-byte chunk of the row
-            const uint32_t off = (uint32_t)(c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c8 & 1) * 8;
-            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(sq + off), "r"(hi[0]), "r"(hi[1]) : "memory");
-            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(sq + DH * kRows * 128 + off), "r"(lo[0]), "r"(lo[1]) : "memory");
+          for (int e = 0; e < 2; ++e) {
+            const float x0 = __uint_as_float(w[i][2 * e] << 16) * down, x1 = __uint_as_float(w[i][2 * e] & 0xFFFF0000u) * down;
+            const float x2 = __uint_as_float(w[i][2 * e + 1] << 16) * down, x3 = __uint_as_float(w[i][2 * e + 1] & 0xFFFF0000u) * down;
+            const float h0 = e4m3_head(x0), h1 = e4m3_head(x1), h2 = e4m3_head(x2), h3 = e4m3_head(x3);
+            hi[e] = pack_e4m3x2(h0, h1) | (pack_e4m3x2(h2, h3) << 16);
+            lo[e] = pack_e4m3x2(x0 - h0, x1 - h1) | (pack_e4m3x2(x2 - h2, x3 - h3) << 16);
           }
+          const uint32_t at = base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c8 & 1) * 8;
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + DH * kRows * 128), "r"(lo[0]), "r"(lo[1]) : "memory");
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -958,8 +968,7 @@ cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a,
   auto launch = [&](auto kernel, int threads, int smem) -> cudaError_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)grid, threads, smem, stream>>>(kmap, vmap, p);
-    return cudaGetLastError();
+    return launch_pdl(kernel, (int)grid, threads, (size_t)smem, stream, kmap, vmap, p);
   };
   return g.head_dim == 128 ? launch(paged_prefill_kernel<128>, PrefillPlan<128>::THREADS, PrefillPlan<128>::SMEM)
                            : launch(paged_prefill_kernel<256>, PrefillPlan<256>::THREADS, PrefillPlan<256>::SMEM);
