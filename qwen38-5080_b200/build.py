@@ -31,7 +31,7 @@ def lib_path(bounds: bool = False) -> Path:
 def stamp_path(bounds: bool = False) -> Path:
     return Path(str(lib_path(bounds)) + ".hash")
 SOURCES = ["api.cu", "append.cu", "decode_simt.cu", "decode_mma.cu", "decode_umma2.cu", "static_scratch.cu", "peer_barrier.cu", "producer.cu",
-           "paged_api.cu", "paged_append.cu", "paged_decode.cu", "paged_prefill.cu"]
+           "paged_api.cu", "paged_append.cu", "paged_decode.cu", "paged_prefill.cu", "paged_few.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

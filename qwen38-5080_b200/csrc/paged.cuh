@@ -42,10 +42,23 @@ struct PagedAttnArgs {
   const int* q_start;
   int causal;
 };
-size_t paged_decode_workspace_bytes(const PagedGeometry& g, int max_seq_len);
+size_t paged_decode_workspace_bytes();
 cudaError_t launch_paged_decode(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream);
-size_t paged_prefill_workspace_bytes(const PagedGeometry& g, int n_tokens, int max_seq_len);
+size_t paged_prefill_workspace_bytes(const PagedGeometry& g);
 cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream);
+bool few_rows(const PagedGeometry& g, int n_tokens);
+size_t paged_few_partial_bytes(const PagedGeometry& g);
+cudaError_t launch_paged_few(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream);
+
+// A workspace: counters (zero between launches; a call that joins pieces has at most three tiles per SM to join), the stream-K
+// kernel's tagged words (zero between launches), partial results (anything).  The parts begin at the same place for every kernel
+// and shape, so calls that do not overlap in time may share a workspace whatever they are.
+constexpr size_t kPagedWordBytes = 8 * 2 * (8 * 128 + 16);   // per CTA: two states of 8 heads of 128 (of 256: one CTA per SM, not three)
+inline size_t paged_words_offset() { return ((size_t)device_sms() * 12 + 255) & ~(size_t)255; }
+inline size_t paged_partials_offset() { return paged_words_offset() + 3 * (size_t)device_sms() * kPagedWordBytes; }
+inline int* paged_counters(void* ws) { return (int*)ws; }
+inline unsigned long long* paged_words(void* ws) { return (unsigned long long*)((uint8_t*)ws + paged_words_offset()); }
+inline float* paged_partials(void* ws) { return (float*)((uint8_t*)ws + paged_partials_offset()); }
 
 // Valid length of a sequence: negative lengths count as 0, lengths beyond the table's capacity are clamped to it.
 __device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* status, bool report) {

@@ -70,7 +70,7 @@ int b200attn_paged_workspace_bytes(const B200AttnPagedShape* shape, int q_tokens
   if (!bytes) return B200ATTN_ERR_NULL;
   if (q_tokens < 0) return B200ATTN_ERR_SHAPE;
   if (max_seq_len < 0) return B200ATTN_ERR_CAPACITY;
-  *bytes = q_tokens ? paged_prefill_workspace_bytes(g, q_tokens, max_seq_len) : paged_decode_workspace_bytes(g, max_seq_len);
+  *bytes = q_tokens ? paged_prefill_workspace_bytes(g) : paged_decode_workspace_bytes();
   return B200ATTN_OK;
 }
 
@@ -82,7 +82,7 @@ static int check_attention(const B200AttnPagedShape* shape, PagedGeometry* g, co
   if (a.n_tokens < 0) return B200ATTN_ERR_SHAPE;
   if (a.max_seq_len < 0) return B200ATTN_ERR_CAPACITY;
   if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || !aligned16(a.workspace)) return B200ATTN_ERR_ALIGN;
-  const size_t need = prefill ? paged_prefill_workspace_bytes(*g, a.n_tokens, a.max_seq_len) : paged_decode_workspace_bytes(*g, a.max_seq_len);
+  const size_t need = prefill ? paged_prefill_workspace_bytes(*g) : paged_decode_workspace_bytes();
   if (need && !a.workspace) return B200ATTN_ERR_NULL;
   if (a.workspace_bytes < need) return B200ATTN_ERR_WORKSPACE;
   return B200ATTN_OK;

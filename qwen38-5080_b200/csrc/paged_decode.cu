@@ -47,7 +47,7 @@ struct DecodeParams {
   float score_scale;                      // softmax_scale * log2(e)
   int num_splits;
   float* part;                            // [pairs][num_splits][G * D + 16]: O, m[8], l[8]
-  int* counters;                          // [pairs]
+  int* counters;                          // [pairs], used when pairs are cut into pieces (4 or more, so there are few pairs)
   uint16_t* out;
   int* status;
 };
@@ -802,13 +802,9 @@ int decode_splits(const PagedGeometry& g, int max_seq_len) {
 
 }  // namespace
 
-size_t paged_decode_workspace_bytes(const PagedGeometry& g, int max_seq_len) {
-  Geometry q{};
-  q.group = g.group; q.head_dim = g.head_dim;
-  if (use_streamk(g, max_seq_len)) return mma_workspace_bytes(q, streamk_ctas(g));
-  const size_t pairs = (size_t)g.n_layers * g.batch * g.h_kv, splits = decode_splits(g, max_seq_len);
-  if (splits == 1) return 0;
-  return pairs * splits * ((size_t)g.group * g.head_dim + 16) * 4 + pairs * 4;
+size_t paged_decode_workspace_bytes() {
+  // register kernel: partial states of at most every block slot of the device
+  return paged_partials_offset() + (size_t)device_sms() * 4 * (8 * 128 + 16) * 4;
 }
 
 namespace {
@@ -832,7 +828,7 @@ cudaError_t launch_paged_streamk(const PagedGeometry& g, const PagedAttnArgs& a,
   m.seq_len = a.seq_len;
   m.seq_len_offset = a.seq_len_offset;
   m.score_scale = a.softmax_scale * kLog2e;
-  m.ws_pkt = (unsigned long long*)a.workspace;
+  m.ws_pkt = paged_words(a.workspace);
   m.out = (uint16_t*)a.out;
   m.out_hq_total = g.h_q;
   m.status = a.status;
@@ -861,8 +857,8 @@ cudaError_t launch_paged_decode(const PagedGeometry& g, const PagedAttnArgs& a, 
   p.score_scale = a.softmax_scale * kLog2e;
   p.num_splits = decode_splits(g, a.max_seq_len);
   const long long pairs = (long long)g.n_layers * g.batch * g.h_kv;
-  p.part = (float*)a.workspace;
-  p.counters = (int*)(p.part + (size_t)pairs * p.num_splits * ((size_t)g.group * g.head_dim + 16));
+  p.part = paged_partials(a.workspace);
+  p.counters = paged_counters(a.workspace);
   p.out = (uint16_t*)a.out;
   p.status = a.status;
   const long long grid = pairs * p.num_splits;

@@ -931,15 +931,14 @@ int prefill_splits(const PagedGeometry& g, int n_tokens, int max_seq_len) {
 
 }  // namespace
 
-size_t paged_prefill_workspace_bytes(const PagedGeometry& g, int n_tokens, int max_seq_len) {
-  // A workspace serves every call with up to n_tokens query rows; fewer tokens can mean more pieces: tiles * pieces is at
-  // most the SM count whenever there are pieces, so that many slots do for all of them.
-  (void)n_tokens;
-  (void)max_seq_len;
-  return (size_t)device_sms() * ((size_t)kRows * (g.head_dim + 2) * 4 + 4) + 16;
+size_t paged_prefill_workspace_bytes(const PagedGeometry& g) {
+  // tiles x pieces is at most the SM count whenever there are pieces
+  const size_t many = (size_t)device_sms() * kRows * (g.head_dim + 2) * 4, few = paged_few_partial_bytes(g);
+  return paged_partials_offset() + (many > few ? many : few);
 }
 
 cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
+  if (few_rows(g, a.n_tokens)) return launch_paged_few(g, a, stream);
   Geometry cache{};
   cache.n_layers = g.n_layers; cache.batch = g.n_pages; cache.h_kv = g.h_kv; cache.capacity = g.page_size; cache.head_dim = g.head_dim;
   CUtensorMap kmap, vmap;
@@ -959,8 +958,8 @@ cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a,
   p.tiles = (int)prefill_tiles(g, a.n_tokens, p.pair);
   p.splits = prefill_splits(g, a.n_tokens, a.max_seq_len);
   p.score_scale = a.softmax_scale * kLog2e;
-  p.counters = (int*)a.workspace;
-  p.part = (float*)((uint8_t*)a.workspace + (((size_t)device_sms() * 4 + 15) & ~(size_t)15));
+  p.counters = paged_counters(a.workspace);
+  p.part = paged_partials(a.workspace);
   p.out = (uint16_t*)a.out;
   p.status = a.status;
   const long long grid = (long long)p.tiles * p.splits * g.h_kv * g.n_layers;

@@ -469,3 +469,48 @@ def test_ragged_batch_launched_many_times(pkg, cuda_device):
     for b in (0, 7, 31):
         want, big = ref.attention(q[0, b:b + 1].cpu(), kb[0], vb[0], ks[0], vs[0], table[b], lens[b])
         ref.assert_attention(first[0, b:b + 1].cpu(), want, big)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("page", [16, 128])
+def test_prefill_a_few_tokens_each(pkg, cuda_device, heads, causal, page):
+    """A handful of new tokens per sequence, none for some, many for one; fewer cached tokens than new ones."""
+    lens, qlens = [130, 300, 64, 5, 1, 20, 0, 257, 1100, 17], [1, 2, 1, 0, 1, 3, 2, 4, 1, 2]
+    _run_attention(pkg, cuda_device, (2, heads, page, lens), qlens=qlens, causal=causal, seed=51)
+    lens, qlens = [700, 31, 0, 9, 16, 2, 64, 128, 500, 12, 33, 1], [15, 1, 0, 0, 0, 0, 1, 1, 1, 1, 1, 1]
+    _run_attention(pkg, cuda_device, (1, heads, page, lens), qlens=qlens, causal=causal, seed=52)
+
+
+@pytest.mark.parametrize("heads", [(5, 1, 128), (40, 8, 128), (4, 2, 256), (8, 1, 256)])
+def test_prefill_a_few_tokens_on_long_caches(pkg, cuda_device, heads):
+    """Few sequences: the keys are cut into pieces, which do not all have tokens."""
+    _run_attention(pkg, cuda_device, (1, heads, 64, [6000, 4097, 40]), qlens=[2, 1, 2], causal=True, seed=53)
+    _run_attention(pkg, cuda_device, (1, heads, 32, [33, 9001]), qlens=[1, 1], causal=True, seed=54, hint=20000)
+    _run_attention(pkg, cuda_device, (1, heads, 16, [257]), qlens=[2], causal=False, seed=55, hint=100)
+
+
+def test_workspaces_serve_calls_of_any_shape(pkg, cuda_device):
+    """One workspace for calls that are laid out differently in it, in turn: short and long tables, few and many sequences."""
+    g = torch.Generator().manual_seed(8)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 300, 2, 64, 128)
+    up = [t.to(cuda_device) for t in (kb, vb, ks, vs)]
+    cases = []
+    for batch, lens, width in ((1, [700], 11), (2, [3000, 5000], 2000), (4, [900, 1000, 64, 1], 16), (3, [9000, 1, 130], 1500), (70, [200] * 70, 4)):
+        table = torch.zeros(batch, width, dtype=torch.int32)
+        table[:, :min(width, 150)] = torch.randint(0, 300, (batch, min(width, 150)), generator=g).to(torch.int32)
+        for h_q in (2, 10):
+            q = torch.randn(1, batch, h_q, 128, generator=g).to(torch.bfloat16)
+            cases.append((q, table, lens, pkg.make_paged_shape(h_q, kb, vb, ks, table)))
+    wd, wp = (pkg.PagedWorkspace(cases[0][3], cuda_device, q_tokens=n) for n in (None, 70))
+    for turn in range(3):
+        for q, table, lens, _ in cases:
+            n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+            starts = torch.arange(len(lens) + 1, dtype=torch.int32, device=cuda_device)
+            a = pkg.paged_decode_attention(q.to(cuda_device), *up, table.to(cuda_device), n, workspace=wd).cpu()
+            b = pkg.paged_prefill_attention(q.to(cuda_device), starts, *up, table.to(cuda_device), n, workspace=wp).cpu()
+            for i in sorted({0, len(lens) - 1, len(lens) // 2}):
+                want, big = ref.attention(q[0, i:i + 1], kb[0], vb[0], ks[0], vs[0], table[i], lens[i])
+                ref.assert_attention(a[0, i:i + 1], want, big, ("decode", turn, lens))
+                ref.assert_attention(b[0, i:i + 1], want, big, ("prefill", turn, lens))
+    assert wd.read_status() == 0 and wp.read_status() == 0
