@@ -33,6 +33,7 @@ struct AppendParams {
   const float *cos, *sin;
   const int *positions, *pair_axis;
   int n_positions, n_axes, rot;
+  int q_run;                              // groups of query heads that a warp takes in turn
   uint32_t q_units;       // warps' shares of the queries
   int kv_blocks, heads;   // pages that the call touches, at most; kv heads that a block takes in turn
 };
@@ -44,9 +45,12 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(e < 1 ? 1 : e) << 23);
 }
 
+constexpr float kFltMax = 3.402823466e38f;
+// Largest of the warp's values; none is negative, so their bits compare as integers.
+__device__ __forceinline__ float warp_max(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); }
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
-  return a <= 3.402823466e38f ? a : 0.f;   // NaN and infinities do not take part in the maximum
+  return a <= kFltMax ? a : 0.f;   // NaN and infinities do not take part in the maximum
 }
 
 // A lane's share of a head row: four dims at `a` and four at `b`.  In the rotated part b = a + R / 2: a lane holds both halves of
@@ -175,26 +179,34 @@ __device__ __forceinline__ int page_of(const AppendParams& p, int b, int page_in
   return id >= 0 && id < p.g.n_pages ? id : -1;
 }
 
-// Query rows: a warp takes kQLoads loads' worth of a token's heads, all in flight together, and rotates them with one set of
-// cosines and sines.  (One warp per token, head after head, waited for every load: 445 us for a 32768-token prompt of 40 / 8
-// heads against 160 us for its keys and values alone.)
+// Query rows: a warp takes kQLoads loads' worth of a token's heads at a time, all in flight together, and rotates them with one set
+// of cosines and sines.  (One warp per token, head after head, waited for every load: 445 us for a 32768-token prompt of 40 / 8
+// heads against 160 us for its keys and values alone.)  Where there are many tokens it goes on with the token's next heads, whose
+// rows are on their way meanwhile: finding the token's sequence, position and angles is half of the instructions otherwise.
 constexpr int kQLoads = 4;
 template <int D>
-__host__ __device__ constexpr int q_heads() { return kQLoads * 32 / (D / 8); }   // heads of a warp: 8 or 4
-template <int D>
+__host__ __device__ constexpr int q_heads() { return kQLoads * 32 / (D / 8); }   // heads of a group: 8 or 4
+template <int D, bool RUN>   // RUN: several groups in turn
 __device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t unit) {
   constexpr int TPR = D / 8, RPW = 32 / TPR;   // lanes per head row, rows per load
   const int lane = threadIdx.x & 31;
-  const uint32_t groups = (uint32_t)(p.g.h_q + q_heads<D>() - 1) / q_heads<D>();
-  const uint32_t r = unit / groups;            // (layer, token)
-  const int h0 = (int)(unit - r * groups) * q_heads<D>() + lane / TPR;
+  const int groups = (p.g.h_q + q_heads<D>() - 1) / q_heads<D>();
+  const int run = RUN ? p.q_run : 1;
+  const uint32_t chunks = (uint32_t)(groups + run - 1) / run;
+  const uint32_t r = unit / chunks;            // (layer, token)
+  const int g_first = (int)(unit - r * chunks) * run, g_end = min(groups, g_first + run);
   const int layer = (int)(r / (uint32_t)p.n_tokens), token = (int)(r - (uint32_t)layer * p.n_tokens);
   const Share<D> sh(lane, p.rot);
-  const long long row0 = (long long)r * p.g.h_q + h0;
+  const long long row0 = (long long)r * p.g.h_q + lane / TPR;
   Raw raw[kQLoads];
+  auto load = [&](int group) {
 #pragma unroll
-  for (int i = 0; i < kQLoads; ++i)
-    if (h0 + i * RPW < p.g.h_q) raw[i] = load_row<D>(p.q + (row0 + i * RPW) * D, sh);
+    for (int i = 0; i < kQLoads; ++i) {
+      const int h = group * q_heads<D>() + i * RPW;
+      if (h + lane / TPR < p.g.h_q) raw[i] = load_row<D>(p.q + (row0 + h) * D, sh);
+    }
+  };
+  load(g_first);
   int b = token, slot;
   if (p.q_start) {
     if (token >= __ldg(p.q_start + p.g.batch) || token < __ldg(p.q_start)) return;   // a row that belongs to nobody
@@ -207,16 +219,24 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t u
   rot.load<D>(p, sh, token, slot);
   float w1[8];
   if (p.wq) load_norm<D>(p.wq, layer, sh, w1);
+#pragma unroll 1
+  for (int group = g_first; group < (RUN ? g_end : g_first + 1); ++group) {
+    Raw now[kQLoads];
 #pragma unroll
-  for (int i = 0; i < kQLoads; ++i) {
-    float x[8];
-    unpack(raw[i], x);
-    if (p.wq) rms_norm<D>(x, w1, p.eps);
-    if (sh.on) rot.turn(x);
-    if (h0 + i * RPW < p.g.h_q) {
-      uint16_t* dst = p.q_out + (row0 + i * RPW) * D;
-      *reinterpret_cast<uint2*>(dst + sh.a) = pack4(x);
-      *reinterpret_cast<uint2*>(dst + sh.b) = pack4(x + 4);
+    for (int i = 0; i < kQLoads; ++i) now[i] = raw[i];
+    if (RUN && group + 1 < g_end) load(group + 1);
+#pragma unroll
+    for (int i = 0; i < kQLoads; ++i) {
+      float x[8];
+      unpack(now[i], x);
+      if (p.wq) rms_norm<D>(x, w1, p.eps);
+      if (sh.on) rot.turn(x);
+      const int h = group * q_heads<D>() + i * RPW;
+      if (h + lane / TPR < p.g.h_q) {
+        uint16_t* dst = p.q_out + (row0 + h) * D;
+        *reinterpret_cast<uint2*>(dst + sh.a) = pack4(x);
+        *reinterpret_cast<uint2*>(dst + sh.b) = pack4(x + 4);
+      }
     }
   }
 }
@@ -233,7 +253,7 @@ paged_append_token_kernel(const AppendParams p) {
   const uint32_t warp = blockIdx.x * 4 + (threadIdx.x >> 5);
   const uint32_t rows = (uint32_t)g.n_layers * g.batch * g.h_kv * 2, kv_warps = (rows + RPW - 1) / RPW;   // rows is even
   if (warp >= kv_warps) {
-    if (warp - kv_warps < p.q_units) rotate_queries<D>(p, warp - kv_warps);
+    if (warp - kv_warps < p.q_units) rotate_queries<D, false>(p, warp - kv_warps);
     return;
   }
   const uint32_t r2 = warp * RPW + lane / TPR;       // (layer, sequence, head, key or value)
@@ -392,16 +412,20 @@ paged_append_prompt_kernel(const AppendParams p) {
     for (int i = 0; i < NP; ++i) {
       if (!which && sh.on) rot[i].turn(x[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[i][e]));   // rows that are not new are zero
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][e]));   // rows that are not new are zero; NaN is passed over
     }
+    amax = warp_max(amax);
+    if (amax > kFltMax) {                                 // infinities among them: once more without
+      amax = 0.f;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(x[i][e]));
+      amax = warp_max(amax);
+    }
     if (lane == 0) s_max[h & 1][tid >> 5] = amax;
     __syncthreads();                                      // maxima are in; every thread has read the old scale
-    amax = lane < THREADS / 32 ? s_max[h & 1][lane] : 0.f;
-#pragma unroll
-    for (int off = THREADS / 64; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    amax = __shfl_sync(0xffffffffu, amax, 0);
+    amax = warp_max(lane < THREADS / 32 ? s_max[h & 1][lane] : 0.f);
     float s = pow2_scale(amax);
     uint8_t* base = pages + (long long)h * g.page_size * D;
     if (lo > 0) {
@@ -429,9 +453,9 @@ paged_append_prompt_kernel(const AppendParams p) {
 
 // The queries of prompts: a kernel of their own, with more warps on an SM than the one above has.
 template <int D>
-__global__ void __launch_bounds__(256) paged_rotate_queries_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, 3) paged_rotate_queries_kernel(const AppendParams p) {
   const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit < p.q_units) rotate_queries<D>(p, unit);
+  if (unit < p.q_units) rotate_queries<D, true>(p, unit);
 }
 
 __global__ void paged_advance_kernel(PagedGeometry g, const int* q_start, int* seq_pos) {
@@ -463,7 +487,12 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
     p.n_positions = a.rope->n_positions; p.n_axes = a.rope->n_axes; p.rot = a.rope->rotary_dim;
   }
   const int q_heads_ = g.head_dim == 128 ? q_heads<128>() : q_heads<256>();
-  const long long q_warps = a.q ? (long long)g.n_layers * a.n_tokens * ((g.h_q + q_heads_ - 1) / q_heads_) : 0;
+  // groups of heads that a warp takes in turn: as many as leave an SM 64 warps of queries
+  const int groups = (g.h_q + q_heads_ - 1) / q_heads_;
+  const long long run = (long long)g.n_layers * a.n_tokens * groups / (64LL * device_sms());
+  const int chunks = run <= 1 ? groups : run >= groups ? 1 : (groups + (int)run - 1) / (int)run;
+  p.q_run = a.q_start ? (groups + chunks - 1) / chunks : 1;
+  const long long q_warps = a.q ? (long long)g.n_layers * a.n_tokens * ((groups + p.q_run - 1) / p.q_run) : 0;
   const long long kv_rows = (long long)g.n_layers * g.batch * g.h_kv * 2;
   if (q_warps > 0x7fffffffLL || kv_rows > 0x7fffffffLL) return cudaErrorInvalidConfiguration;   // indices are 32-bit
   p.q_units = (uint32_t)q_warps;
