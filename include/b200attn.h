@@ -422,7 +422,8 @@ int b200attn_calibrate_scales(const B200AttnShape* shape, int n_tokens,
  *     k_scale / v_scale : f32 [n_layers][n_pages][h_kv]       one scale per (layer, page, kv head)
  *     page_table        : i32 [batch][max_pages]              page of tokens [i * page_size, (i+1) * page_size) of a sequence
  *
- * A value is float(byte) * scale.  The attention calls take any scale; the append makes powers of two (below).
+ * A value is float(byte) * scale.  The attention calls take any scale that is not negative and not NaN; the append makes powers
+ * of two (below).
  * Table entries at or beyond a sequence's last token are never read.  A page that the append writes must
  * belong to one sequence only; pages that are only read may be shared.  Queries and new keys / values of ragged
  * batches are packed: sequence b owns rows [q_start[b], q_start[b + 1]) of the token dimension; rows from
@@ -485,9 +486,10 @@ int b200attn_paged_rope_append(const B200AttnPagedShape* shape, const B200AttnRo
 
 /*
  * Scratch of the two attention calls below: partial results of sequences that are split over several thread blocks,
- * and one counter per split result.  q_tokens = 0: for b200attn_paged_decode; otherwise for b200attn_paged_prefill with up
- * to q_tokens query rows.  Zero it once with b200attn_workspace_init; every launch leaves its counters at zero.  Launches
- * that may overlap on the device need workspaces of their own.
+ * and counters.  q_tokens = 0: for b200attn_paged_decode; otherwise for b200attn_paged_prefill with up to q_tokens query
+ * tokens.  Zero it once with b200attn_workspace_init; every launch leaves its counters at zero, and calls of different shapes
+ * may use it in turn.  Launches that may overlap on the device need workspaces of their own.  After a status of
+ * B200ATTN_STATUS_WAIT_TIMEOUT it has to be zeroed again.
  */
 int b200attn_paged_workspace_bytes(const B200AttnPagedShape* shape, int q_tokens, int max_seq_len, size_t* bytes);
 
@@ -497,6 +499,7 @@ int b200attn_paged_workspace_bytes(const B200AttnPagedShape* shape, int q_tokens
  *   q, out      : bf16 [n_layers][batch][h_q][head_dim]
  *   max_seq_len : an upper bound of the lengths that the host knows (0: the table's capacity); it decides how the work is
  *                 split, not what is attended: longer sequences are attended in full all the same
+ *   softmax_scale : finite, not negative
  */
 int b200attn_paged_decode(const B200AttnPagedShape* shape, const void* q_bf16,
                           const void* k_pages_u8, const void* v_pages_u8, const float* k_scale, const float* v_scale,
@@ -509,6 +512,8 @@ int b200attn_paged_decode(const B200AttnPagedShape* shape, const void* q_bf16,
  * The queries of sequence b are its last tokens: with causal = 1, query i of n attends slots t <= seq_len[b] - n + i (none:
  * its row is zero); with causal = 0 all seq_len[b] slots (cross attention to states of another length).
  *   q, out  : bf16 [n_layers][n_tokens][h_q][head_dim], q_start i32 [batch + 1]
+ * Keys that a row does not see have no influence on it, NaN keys included; a NaN among the values of one of a sequence's last
+ * n tokens can reach the rows before it as well (0 * NaN).
  */
 int b200attn_paged_prefill(const B200AttnPagedShape* shape, int n_tokens, const void* q_bf16, const int* q_start,
                            const void* k_pages_u8, const void* v_pages_u8, const float* k_scale, const float* v_scale,

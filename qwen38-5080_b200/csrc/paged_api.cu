@@ -80,6 +80,7 @@ static int check_attention(const B200AttnPagedShape* shape, PagedGeometry* g, co
   if (!a.q || !a.k_pages || !a.v_pages || !a.k_scale || !a.v_scale || !a.page_table || !a.seq_len || !a.out || !a.status) return B200ATTN_ERR_NULL;
   if (prefill && !a.q_start) return B200ATTN_ERR_NULL;
   if (a.n_tokens < 0) return B200ATTN_ERR_SHAPE;
+  if (!(a.softmax_scale >= 0.f && a.softmax_scale <= 3.402823466e38f)) return B200ATTN_ERR_SHAPE;   // the kernels count on multipliers >= 0
   if (a.max_seq_len < 0) return B200ATTN_ERR_CAPACITY;
   if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || !aligned16(a.workspace)) return B200ATTN_ERR_ALIGN;
   const size_t need = prefill ? paged_prefill_workspace_bytes(*g) : paged_decode_workspace_bytes();

@@ -435,7 +435,7 @@ int few_blocks(const PagedGeometry& g) { return g.head_dim == 128 ? FewPlan<128,
 // The host knows the tokens and sequences of a call, not how they are spread; a sequence with more rows than a tile takes several,
 // each of which reads the keys again.
 bool few_rows(const PagedGeometry& g, int n_tokens) {
-  return (long long)((n_tokens + g.batch - 1) / g.batch) * g.group <= kFewRows && (long long)g.n_pages * g.h_kv * g.page_size <= 0x7fffffffLL;
+  return ((long long)n_tokens + g.batch - 1) / g.batch * g.group <= kFewRows && (long long)g.n_pages * g.h_kv * g.page_size <= 0x7fffffffLL;
 }
 
 cudaError_t launch_paged_few(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {

@@ -67,8 +67,8 @@ def make_paged_shape(h_q: int, k_pages, v_pages, k_scale, page_table) -> B200Att
 
 class PagedWorkspace:
     """Scratch of the attention calls, allocated once (before any graph capture): for decode, or with `q_tokens` for prefill
-    calls of up to that many query tokens.  `max_seq_len`: an upper bound of the lengths (default: the table's capacity); it
-    decides how the work is split.  Launches that may overlap on the device need workspaces of their own."""
+    calls of up to that many query tokens; calls of different shapes may use it in turn.  `max_seq_len`: an upper bound of the
+    lengths (default: the table's capacity); it decides how the work is split.  Launches that may overlap on the device need workspaces of their own."""
 
     def __init__(self, shape: B200AttnPagedShape, device, *, max_seq_len: int | None = None, q_tokens: int | None = None):
         self.max_seq_len = int(max_seq_len or 0)

@@ -144,3 +144,23 @@ def test_rope_tables_are_those_of_64_bits(pkg):
     for pos, j in ((0, 0), (1, 5), (131071, 0), (131071, 31), (99999, 3)):
         a = pos * 1e6 ** (-2 * j / 64)
         assert abs(float(cos[pos, j]) - math.cos(a)) < 1e-7 and abs(float(sin[pos, j]) - math.sin(a)) < 1e-7
+
+
+def test_softmax_scales_that_are_negative_or_not_finite_are_refused(pkg):
+    L, lib = pkg._lib, pkg._lib.lib()
+    s = ctypes.byref(_shape(pkg))
+    for scale in (-0.1, float("nan"), float("inf"), float("-inf")):
+        assert lib.b200attn_paged_decode(s, A, A, A, A, A, A, A, 0, 0, scale, A, 1 << 40, A, A, None) == L.ERR_SHAPE
+        assert lib.b200attn_paged_prefill(s, 4, A, A, A, A, A, A, A, A, 0, 1, scale, A, 1 << 40, A, A, None) == L.ERR_SHAPE
+
+
+def test_workspace_bytes_do_not_depend_on_the_batch_or_the_length(pkg):
+    """Calls of different shapes may use a workspace in turn."""
+    lib = pkg._lib.lib()
+
+    def size(q_tokens, most, **kw):
+        n = ctypes.c_size_t(0)
+        assert lib.b200attn_paged_workspace_bytes(ctypes.byref(_shape(pkg, **kw)), q_tokens, most, ctypes.byref(n)) == 0
+        return n.value
+    for q_tokens in (0, 5):
+        assert len({size(q_tokens, most, batch=b) for b in (1, 7, 900) for most in (0, 1, 100000)}) == 1

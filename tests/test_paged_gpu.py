@@ -514,3 +514,53 @@ def test_workspaces_serve_calls_of_any_shape(pkg, cuda_device):
                 ref.assert_attention(a[0, i:i + 1], want, big, ("decode", turn, lens))
                 ref.assert_attention(b[0, i:i + 1], want, big, ("prefill", turn, lens))
     assert wd.read_status() == 0 and wp.read_status() == 0
+
+
+def test_as_many_sequences_as_one_block_can_list(pkg, cuda_device):
+    lens = [i * 11 % 50 for i in range(2048)]
+    _run_attention(pkg, cuda_device, (1, (8, 1, 256), 16, lens), seed=46, spare_pages=80)
+
+
+def test_pages_beyond_two_gigabytes(pkg, cuda_device):
+    """The last pages of a large pool: appended to, then read by every attention kernel."""
+    g = torch.Generator().manual_seed(12)
+    h_q, h_kv, d, page, n_pages = 40, 8, 128, 64, 34000
+    kb, vb = (torch.zeros(1, n_pages, h_kv, page, d, dtype=torch.uint8, device=cuda_device) for _ in range(2))
+    ks, vs = (torch.ones(1, n_pages, h_kv, device=cuda_device) for _ in range(2))
+    lens, width = [300, 129, 1], 600
+    table = torch.full((3, width), -1, dtype=torch.int32)
+    at = n_pages - 1
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            table[b, i], at = at, at - 1
+    low = at + 1                                            # the pages used are [low, n_pages)
+    k, v = (torch.randn(1, sum(lens), h_kv, d, generator=g).to(torch.bfloat16).to(cuda_device) for _ in range(2))
+    starts = torch.tensor([0, 300, 429, 430], dtype=torch.int32, device=cuda_device)
+    pos, status = torch.zeros(3, dtype=torch.int32, device=cuda_device), torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    up = (kb, vb, ks, vs, table.to(cuda_device))
+    pkg.paged_rope_append(None, k, v, None, None, *up, pos, q_start=starts, status=status)
+    assert pos.tolist() == lens and status.item() == 0
+    small = [t[:, low:].cpu() for t in (kb, vb, ks, vs)]
+    for b, n in enumerate(lens):                            # the bytes are the new tokens', to half a step of e4m3
+        rows = torch.cat([small[0][0, table[b, i] - low].permute(1, 0, 2) for i in range(-(-n // page))])[:n]
+        scale = torch.stack([small[2][0, table[b, i // page] - low] for i in range(n)])[:, :, None].double()
+        want = k[0, starts[b]:starts[b] + n].cpu().double()
+        assert ((ref.values(rows) * scale - want).abs() <= want.abs() * 2.0 ** -4 + scale * 2.0 ** -10).all()
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    q = torch.randn(1, 3, h_q, d, generator=g).to(torch.bfloat16)
+    many = torch.randn(1, 200, h_q, d, generator=g).to(torch.bfloat16)
+    shape = pkg.make_paged_shape(h_q, kb, vb, ks, table)
+    wp = pkg.PagedWorkspace(shape, cuda_device, q_tokens=200)
+    first = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=cuda_device)
+    got = [pkg.paged_decode_attention(q.to(cuda_device), *up, n, workspace=pkg.PagedWorkspace(shape, cuda_device, max_seq_len=most)) for most in (300, 38400)]
+    got.append(pkg.paged_prefill_attention(q.to(cuda_device), first, *up, n, workspace=wp))
+    rows = torch.tensor([0, 100, 199, 200], dtype=torch.int32, device=cuda_device)
+    out = pkg.paged_prefill_attention(many.to(cuda_device), rows, *up, n, workspace=wp, causal=False).cpu()
+    for b, length in enumerate(lens):
+        ids = torch.where(table[b] >= 0, table[b] - low, table[b])
+        want, big = ref.attention(q[0, b:b + 1], small[0][0], small[1][0], small[2][0], small[3][0], ids, length)
+        for i, x in enumerate(got):
+            ref.assert_attention(x[0, b:b + 1].cpu(), want, big, (i, b))
+        a, z = rows[b].item(), rows[b + 1].item()
+        want, big = ref.attention(many[0, a:z], small[0][0], small[1][0], small[2][0], small[3][0], ids, length)
+        ref.assert_attention(out[0, a:z], want, big, ("many", b))
