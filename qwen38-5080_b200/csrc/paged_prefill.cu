@@ -293,7 +293,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     }
   }
   if (tid == 32) {
-    mbar_init(qready, kSoftmaxWarps);
+    mbar_init(qready, kSoftmaxWarps + (NS == 1 ? 4 : 0));
     for (int i = 0; i < KST; ++i) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, 1); }
     for (int i = 0; i < kInfo; ++i) mbar_init(kinfo + 8 * i, 1);
     for (int i = 0; i < kVRing; ++i) { mbar_init(vfull + 8 * i, 4); mbar_init(vempty + 8 * i, 1); }
@@ -330,6 +330,67 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   constexpr uint32_t tmem = 0;                              // all 512 columns are this block's: they begin at 0
 
   float r_v = 0.f;                                          // largest V scale of the block's keys (V and softmax warps)
+  // Query rows first .. of the tile at tile_tok as two e4m3 rows each, by one warp; D / 8 lanes per row, 32 / (D / 8) rows a step.  It
+  // copies all of them into the place of their result (16 bytes of bf16 become 8 of the first row and 8 of the second; the lanes of
+  // two neighbouring chunks write where they have read), then converts four loads at a time.
+  auto stage_queries = [&](uint32_t sq, float* s_mul, int tile_tok, int first, int steps) {
+    constexpr int LPR = D / 8, RPL = 32 / LPR, BATCH = 4;     // lanes per row, rows per step, steps at a time
+    const int sub = lane / LPR, c8 = lane % LPR, c = c8 >> 1;   // row of the step, 8 dims of it, their 16-byte chunk of the result
+    const uint32_t over_g = (65536u + G - 1) / G;             // r / G = r * over_g >> 16 for r < 128, G <= 8
+    const uint32_t base = sq + (uint32_t)(c >> 3) * (kRows * 128), odd = (c8 & 1) * (uint32_t)(DH * kRows * 128);
+    const int last_row = min(per_tile, ntok - tile_tok) * G;  // rows from here on are no token's
+    const uint16_t* q0_ptr = p.q + (out_row0 + (long long)tile_tok * g.h_q) * D + c8 * 8;
+#pragma unroll 4
+    for (int i = 0; i < steps; ++i) {
+      const int r = first + i * RPL + sub, rt = (int)(r * over_g >> 16);
+      const uint16_t* from = r < last_row ? q0_ptr + (rt * g.h_q + (r - rt * G)) * D : p.q;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + odd), "l"(from), "r"(r < last_row ? 16 : 0) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+#pragma unroll 1
+    for (int i0 = 0; i0 < steps; i0 += BATCH) {
+      uint32_t w[BATCH][4], top[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = first + (i0 + i) * RPL + sub;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                     : "r"(base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + odd));
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i)   // the largest |q| of the row: bf16 magnitudes compare as integers
+        top[i] = __vmaxu2(__vmaxu2(w[i][0] & 0x7FFF7FFFu, w[i][1] & 0x7FFF7FFFu), __vmaxu2(w[i][2] & 0x7FFF7FFFu, w[i][3] & 0x7FFF7FFFu));
+#pragma unroll
+      for (int off = LPR / 2; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+      __syncwarp();                                         // both lanes of a chunk have read
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = first + (i0 + i) * RPL + sub;
+        int ex = (int)(max(top[i] & 0xFFFFu, top[i] >> 16) >> 7);
+        ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
+        const float down = __uint_as_float((uint32_t)(261 - ex) << 23);   // brings the largest |q| into [128, 256)
+        if (c8 == 0) s_mul[r] = __uint_as_float((uint32_t)(ex - 7) << 23) * p.score_scale;
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x0 = __uint_as_float(w[i][2 * e] << 16) * down, x1 = __uint_as_float(w[i][2 * e] & 0xFFFF0000u) * down;
+          const float x2 = __uint_as_float(w[i][2 * e + 1] << 16) * down, x3 = __uint_as_float(w[i][2 * e + 1] & 0xFFFF0000u) * down;
+          const float h0 = e4m3_head(x0), h1 = e4m3_head(x1), h2 = e4m3_head(x2), h3 = e4m3_head(x3);
+          hi[e] = pack_e4m3x2(h0, h1) | (pack_e4m3x2(h2, h3) << 16);
+          lo[e] = pack_e4m3x2(x0 - h0, x1 - h1) | (pack_e4m3x2(x2 - h2, x3 - h3) << 16);
+        }
+        const uint32_t at = base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c8 & 1) * 8;
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + DH * kRows * 128), "r"(lo[0]), "r"(lo[1]) : "memory");
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(qready);
+  };
+
   if (warp >= kTma) regs_down<P::REGS_OTHER>();
   if (warp == kTma) {
     // ================= K tiles; pages and scales of their keys =================
@@ -526,6 +587,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // ================= V: bytes to f16, shared memory to shared memory =================
     regs_down<P::REGS_OTHER>();
     const int vw = warp - kFirstV, vt = tid - kFirstV * 32;
+    if (NS == 1) stage_queries(sQ, s_rowmul[0], 0, vw * 32 + 16, 16 / (256 / D));   // heads of 256: half of the query rows (all of them by four warps: 3 us more)
     // the largest V scale of the block's keys
     {
       float r = 0.f;
@@ -621,72 +683,15 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     const bool real = row / G < per_tile && tok < ntok;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     regs_up<P::REGS_SOFTMAX>();
-    // The query rows as two e4m3 rows each.  A warp takes 32 rows (16 where two groups share a tile), D / 8 lanes per row.  It copies
-    // all of them into the place of their result (16 bytes of bf16 become 8 of the first row and 8 of the second; the lanes of two
-    // neighbouring chunks write where they have read), then converts four loads at a time.  Every thread then picks up the multiplier
-    // of its own row.
+    // The query rows: 32 for a warp; 16 where two groups share a tile, or the V warps take the other half.  Every thread then picks up
+    // the multiplier of its own row.
     const bool halves = NS == 2 && !two;
     float rowmul;
     {
-      constexpr int LPR = D / 8, RPL = 32 / LPR, BATCH = 4;   // lanes per row, rows per step, steps at a time
-      const uint32_t sq = sQ + (two ? grp * P::QTILE : 0);
       float* s_mul = s_rowmul[two ? grp : 0];
-      const int first = halves ? warp * 16 : (warp & 3) * 32, steps = (halves ? 16 : 32) / RPL;
-      const int sub = lane / LPR, c8 = lane % LPR, c = c8 >> 1;   // row of the step, 8 dims of it, their 16-byte chunk of the result
-      const uint32_t over_g = (65536u + G - 1) / G;           // r / G = r * over_g >> 16 for r < 128, G <= 8
-      const uint32_t base = sq + (uint32_t)(c >> 3) * (kRows * 128), odd = (c8 & 1) * (uint32_t)(DH * kRows * 128);
-      const int last_row = min(per_tile, ntok - tile_tok) * G;    // rows from here on are no token's
-      const uint16_t* q0_ptr = p.q + (out_row0 + (long long)tile_tok * g.h_q) * D + c8 * 8;
-#pragma unroll 4
-      for (int i = 0; i < steps; ++i) {
-        const int r = first + i * RPL + sub, rt = (int)(r * over_g >> 16);
-        const uint16_t* from = r < last_row ? q0_ptr + (rt * g.h_q + (r - rt * G)) * D : p.q;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + odd), "l"(from), "r"(r < last_row ? 16 : 0) : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      __syncwarp();
-#pragma unroll 1
-      for (int i0 = 0; i0 < steps; i0 += BATCH) {
-        uint32_t w[BATCH][4], top[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int r = first + (i0 + i) * RPL + sub;
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
-                       : "r"(base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + odd));
-        }
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)   // the largest |q| of the row: bf16 magnitudes compare as integers
-          top[i] = __vmaxu2(__vmaxu2(w[i][0] & 0x7FFF7FFFu, w[i][1] & 0x7FFF7FFFu), __vmaxu2(w[i][2] & 0x7FFF7FFFu, w[i][3] & 0x7FFF7FFFu));
-#pragma unroll
-        for (int off = LPR / 2; off > 0; off >>= 1)
-#pragma unroll
-          for (int i = 0; i < BATCH; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
-        __syncwarp();                                         // both lanes of a chunk have read
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int r = first + (i0 + i) * RPL + sub;
-          int ex = (int)(max(top[i] & 0xFFFFu, top[i] >> 16) >> 7);
-          ex = ex < 8 ? 8 : (ex > 253 ? 253 : ex);
-          const float down = __uint_as_float((uint32_t)(261 - ex) << 23);   // brings the largest |q| into [128, 256)
-          if (c8 == 0) s_mul[r] = __uint_as_float((uint32_t)(ex - 7) << 23) * p.score_scale;
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x0 = __uint_as_float(w[i][2 * e] << 16) * down, x1 = __uint_as_float(w[i][2 * e] & 0xFFFF0000u) * down;
-            const float x2 = __uint_as_float(w[i][2 * e + 1] << 16) * down, x3 = __uint_as_float(w[i][2 * e + 1] & 0xFFFF0000u) * down;
-            const float h0 = e4m3_head(x0), h1 = e4m3_head(x1), h2 = e4m3_head(x2), h3 = e4m3_head(x3);
-            hi[e] = pack_e4m3x2(h0, h1) | (pack_e4m3x2(h2, h3) << 16);
-            lo[e] = pack_e4m3x2(x0 - h0, x1 - h1) | (pack_e4m3x2(x2 - h2, x3 - h3) << 16);
-          }
-          const uint32_t at = base + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c8 & 1) * 8;
-          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
-          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + DH * kRows * 128), "r"(lo[0]), "r"(lo[1]) : "memory");
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qready);
+      stage_queries(sQ + (two ? grp * P::QTILE : 0), s_mul, tile_tok, halves ? warp * 16 : (warp & 3) * 32, (halves || NS == 1 ? 16 : 32) / (256 / D));
       if (halves) asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (NS == 1) wait_for(qready, 0, gave_up, p.status);    // the V warps' rows
       rowmul = s_mul[row];
     }
     // keys this row sees; rows of no token see all of them (their results go nowhere, and they need no mask)
