@@ -26,7 +26,7 @@
 // 16 a cycle per SM make 1024 cycles a tile, the products of a 128-wide head 1048.
 //
 // Few rows on a long cache: the keys are cut into pieces over several thread blocks, which leave (m, l, O) in the
-// workspace; the last one to finish joins them in order.  Nobody waits for another thread block; waits inside one are bounded.
+// workspace, and a second kernel joins them in order.  Nobody waits for another thread block; waits inside one are bounded.
 #include "paged.cuh"
 #include "tcgen05.cuh"
 
@@ -43,6 +43,10 @@ constexpr float kBitsP = 4.f, kMostP = 61440.f;   // p is held times 2^4 in f16;
 constexpr int kPolyEvery = 4;              // of every 4 * kPolyEvery exponentials, two by polynomial
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
 
+struct PrefillTile {
+  long long row0;                          // output row of (token 0, head 0)
+  int rows, pieces;
+};
 struct PrefillParams {
   PagedGeometry g;
   const uint16_t* q;
@@ -51,7 +55,7 @@ struct PrefillParams {
   int n_tokens, causal, page_shift, pair, tiles, splits;   // pair: a block takes two query tiles; tiles: upper bound of the query tiles of one layer
   float score_scale;
   float* part;                             // [query tiles * heads * layers][splits][128 * (D + 2)]
-  int* counters;
+  PrefillTile* done;                       // [query tiles * heads * layers], where there are pieces: what to join
   uint16_t* out;
   int* status;
 };
@@ -306,7 +310,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   }
   __syncthreads();
   const int b = uniform(s_info[0]);
-  if (b < 0) return;                                        // the grid is an upper bound
+  pdl_launch_dependents();
+  const bool reports = p.splits > 1 && piece == 0 && tid == 0;
+  if (b < 0) {                                              // the grid is an upper bound
+    if (reports) p.done[blockIdx.x / p.splits] = PrefillTile{0, 0, 0};
+    return;
+  }
   const int q0 = uniform(s_info[5]), nq = uniform(s_info[6]);
   const int first_tok = uniform(s_info[1]) * per_block, ntok = min(per_block, nq - first_tok);
   const bool two = NS == 2 && ntok > per_tile;              // two query tiles, one for each softmax group; else they share one
@@ -316,6 +325,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int per_piece = (all_tiles + p.splits - 1) / p.splits;
   const int pieces = per_piece > 0 ? (all_tiles + per_piece - 1) / per_piece : 0;
   const long long out_row0 = ((long long)layer * p.n_tokens + q0 + first_tok) * g.h_q + h * G;   // of (token 0, head 0)
+  if (reports) p.done[blockIdx.x / p.splits] = PrefillTile{out_row0, ntok * G, pieces};
   if (piece >= pieces) {
     if (pieces == 0 && piece == 0)                          // nothing to see: zeros
       for (int i = tid; i < ntok * G * (D / 8); i += P::THREADS) {
@@ -877,38 +887,54 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     }
     tc_fence_before();
     asm volatile("bar.arrive 3, %0;" ::"n"((kSoftmaxWarps + 2) * 32) : "memory");
-    if (pieces == 1) return;
+  }
+}
 
-    // ---- the last piece to be finished joins all of them ----
-    const long long tile_id = blockIdx.x / p.splits;
-    __threadfence();
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-    if (tid == 0) s_info[4] = atomicAdd(p.counters + tile_id, 1) == pieces - 1;
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-    if (!s_info[4]) return;
-    __threadfence();
-    if (tid == 0) p.counters[tile_id] = 0;
-    constexpr long long stride = kRows * (D + 2);
-    const float* all = p.part + tile_id * p.splits * stride;
-    for (int i = tid; i < ntok * G * (D / 4); i += kSoftmaxWarps * 32) {
-      const int r = i / (D / 4);
-      float Mx = -INFINITY, Ls = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int s = 0; s < pieces; ++s) Mx = fmaxf(Mx, __ldcg(all + s * stride + kRows * D + r));
-#pragma unroll 4
-      for (int s = 0; s < pieces; ++s) {
-        const float ms = __ldcg(all + s * stride + kRows * D + r);
-        const float w = ms == -INFINITY ? 0.f : ex2(ms - Mx);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(all + s * stride) + i);
-        Ls += __ldcg(all + s * stride + kRows * D + kRows + r) * w;
-        acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
+// Joins the pieces of a query tile's keys: a block takes kJoinRows rows, a thread four dims of a row at a time, all loads of eight
+// pieces in flight together.  (The last block to finish joining all rows of its tile by itself: 408 us for 20 tokens on 32768 keys,
+// 24 / 4 heads of 256 in 36 pieces, against 81; 50 us with at most 24 pieces.)
+constexpr int kJoinRows = 8, kJoinThreads = 128;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PrefillParams p) {
+  pdl_wait();
+  const int tile = (int)(blockIdx.x / (kRows / kJoinRows)), first = (int)(blockIdx.x % (kRows / kJoinRows)) * kJoinRows;
+  const PrefillTile t = p.done[tile];
+  if (t.pieces < 2 || first >= t.rows) return;
+  constexpr long long stride = kRows * (D + 2);
+  const float* all = p.part + (long long)tile * p.splits * stride;
+  const int G = p.g.group, end = min(t.rows, first + kJoinRows) * (D / 4);
+  for (int i = first * (D / 4) + threadIdx.x; i < end; i += kJoinThreads) {
+    const int r = i / (D / 4);
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < t.pieces; s0 += 8) {
+      float m[8], l[8];
+      float4 v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float* from = all + min(s0 + s, t.pieces - 1) * stride;
+        m[s] = __ldcg(from + kRows * D + r);
+        l[s] = __ldcg(from + kRows * D + kRows + r);
+        v[s] = __ldcg(reinterpret_cast<const float4*>(from) + i);
+        if (s0 + s >= t.pieces) m[s] = -INFINITY;
       }
-      const float inv = Ls > 0.f ? 1.f / Ls : 0.f;
-      const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-      reinterpret_cast<uint2*>(p.out + (out_row0 + (long long)(r / G) * g.h_q + r % G) * D)[i % (D / 4)] =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      float Mn = M;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) Mn = fmaxf(Mn, m[s]);
+      const float keep = M == -INFINITY ? 0.f : ex2(M - Mn);
+      M = Mn;
+      L *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float w = m[s] == -INFINITY ? 0.f : ex2(m[s] - M);
+        L += l[s] * w;
+        acc.x += v[s].x * w; acc.y += v[s].y * w; acc.z += v[s].z * w; acc.w += v[s].w * w;
+      }
     }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    reinterpret_cast<uint2*>(p.out + (t.row0 + (long long)(r / G) * p.g.h_q + r % G) * D)[i % (D / 4)] =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
 }
 
@@ -922,7 +948,8 @@ long long prefill_tiles(const PagedGeometry& g, int n_tokens, int pair) {
 int prefill_pair(const PagedGeometry& g, int n_tokens) {
   return g.head_dim == 128 && prefill_tiles(g, n_tokens, 1) * g.h_kv * g.n_layers >= device_sms() ? 1 : 0;
 }
-// Pieces of the keys: where the query tiles do not fill the GPU, as many as do, none under 4 tiles of keys.
+// Pieces of the keys: where the query tiles do not fill the GPU, as many as do, none under 4 tiles of keys and at most 24
+// (20 tokens on 32768 keys, 24 / 4 heads of 256: 12 / 24 / 36 pieces 64 / 50 / 81 us).
 int prefill_splits(const PagedGeometry& g, int n_tokens, int max_seq_len) {
   const long long cap = (long long)g.max_pages * g.page_size;
   const long long most = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
@@ -931,7 +958,7 @@ int prefill_splits(const PagedGeometry& g, int n_tokens, int max_seq_len) {
   long long want = device_sms() / blocks;
   const long long by_len = (most + 4 * kKeys - 1) / (4 * kKeys);
   if (want > by_len) want = by_len;
-  return (int)(want < 1 ? 1 : want);
+  return (int)(want < 1 ? 1 : want > 24 ? 24 : want);
 }
 
 }  // namespace
@@ -939,7 +966,7 @@ int prefill_splits(const PagedGeometry& g, int n_tokens, int max_seq_len) {
 size_t paged_prefill_workspace_bytes(const PagedGeometry& g) {
   // tiles x pieces is at most the SM count whenever there are pieces
   const size_t many = (size_t)device_sms() * kRows * (g.head_dim + 2) * 4, few = paged_few_partial_bytes(g);
-  return paged_partials_offset() + (many > few ? many : few);
+  return paged_partials_offset() + (many > few ? many : few) + (size_t)device_sms() * sizeof(PrefillTile);
 }
 
 cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a, cudaStream_t stream) {
@@ -963,19 +990,20 @@ cudaError_t launch_paged_prefill(const PagedGeometry& g, const PagedAttnArgs& a,
   p.tiles = (int)prefill_tiles(g, a.n_tokens, p.pair);
   p.splits = prefill_splits(g, a.n_tokens, a.max_seq_len);
   p.score_scale = a.softmax_scale * kLog2e;
-  p.counters = paged_counters(a.workspace);
   p.part = paged_partials(a.workspace);
+  p.done = (PrefillTile*)(p.part + (size_t)device_sms() * kRows * (g.head_dim + 2));   // tiles x pieces is at most the SM count
   p.out = (uint16_t*)a.out;
   p.status = a.status;
   const long long grid = (long long)p.tiles * p.splits * g.h_kv * g.n_layers;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  auto launch = [&](auto kernel, int threads, int smem) -> cudaError_t {
+  auto launch = [&](auto kernel, auto join, int threads, int smem) -> cudaError_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, (int)grid, threads, (size_t)smem, stream, kmap, vmap, p);
+    if (e == cudaSuccess) e = launch_pdl(kernel, (int)grid, threads, (size_t)smem, stream, kmap, vmap, p);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    return launch_pdl(join, (int)(grid / p.splits * (kRows / kJoinRows)), kJoinThreads, 0, stream, p);
   };
-  return g.head_dim == 128 ? launch(paged_prefill_kernel<128>, PrefillPlan<128>::THREADS, PrefillPlan<128>::SMEM)
-                           : launch(paged_prefill_kernel<256>, PrefillPlan<256>::THREADS, PrefillPlan<256>::SMEM);
+  return g.head_dim == 128 ? launch(paged_prefill_kernel<128>, paged_join_kernel<128>, PrefillPlan<128>::THREADS, PrefillPlan<128>::SMEM)
+                           : launch(paged_prefill_kernel<256>, paged_join_kernel<256>, PrefillPlan<256>::THREADS, PrefillPlan<256>::SMEM);
 }
 
 }  // namespace b200attn
