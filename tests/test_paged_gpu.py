@@ -564,3 +564,46 @@ def test_pages_beyond_two_gigabytes(pkg, cuda_device):
         a, z = rows[b].item(), rows[b + 1].item()
         want, big = ref.attention(many[0, a:z], small[0][0], small[1][0], small[2][0], small[3][0], ids, length)
         ref.assert_attention(out[0, a:z], want, big, ("many", b))
+
+
+def test_captured_calls_follow_lengths_and_share_workspaces(pkg, cuda_device):
+    """Two graphs over the same workspaces, replayed in turn with other lengths and queries: many rows, few rows, one row."""
+    g = torch.Generator().manual_seed(15)
+    h_q, h_kv, d, page = 10, 2, 128, 32
+    kb, vb, ks, vs = ref.random_cache(g, 1, 400, h_kv, page, d)
+    table = torch.randperm(400, generator=g)[:360].to(torch.int32).view(2, 180)
+    up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+    shape = pkg.make_paged_shape(h_q, kb, vb, ks, table)
+    wd, wp = pkg.PagedWorkspace(shape, cuda_device), pkg.PagedWorkspace(shape, cuda_device, q_tokens=90)
+    n = torch.zeros(2, dtype=torch.int32, device=cuda_device)
+    q1, few, many = (torch.zeros(1, m, h_q, d, dtype=torch.bfloat16, device=cuda_device) for m in (2, 5, 90))
+    s_few, s_many = torch.zeros(3, dtype=torch.int32, device=cuda_device), torch.zeros(3, dtype=torch.int32, device=cuda_device)
+    outs = [torch.empty_like(t) for t in (q1, few, many)]
+
+    def calls():
+        pkg.paged_decode_attention(q1, *up, n, workspace=wd, out=outs[0])
+        pkg.paged_prefill_attention(few, s_few, *up, n, workspace=wp, out=outs[1])
+        pkg.paged_prefill_attention(many, s_many, *up, n, workspace=wp, out=outs[2])
+    calls()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            calls()
+            calls()
+    for turn, (lens, a, b) in enumerate([([5000, 33], [0, 4, 5], [0, 80, 90]), ([70, 5760], [0, 0, 5], [0, 1, 90]), ([0, 1], [0, 2, 3], [0, 45, 46])]):
+        qs = [torch.randn(t.shape, generator=g).to(torch.bfloat16) for t in (q1, few, many)]
+        for dst, src in zip((q1, few, many, n, s_few, s_many), (*qs, torch.tensor(lens), torch.tensor(a), torch.tensor(b))):
+            dst.copy_(src)
+        for o in outs:
+            o.fill_(7.0)
+        graphs[turn % 2].replay()
+        graphs[1 - turn % 2].replay()
+        torch.cuda.synchronize()
+        for q, starts, out in zip(qs, ([0, 1, 2], a, b), outs):
+            out = out.cpu()
+            assert (out[0, starts[2]:] == 7.0).all()
+            for i in range(2):
+                rows = slice(starts[i], starts[i + 1])
+                want, big = ref.attention(q[0, rows], kb[0], vb[0], ks[0], vs[0], table[i], lens[i], causal=q is not qs[0])
+                ref.assert_attention(out[0, rows], want, big, (turn, i, starts))
+    assert wd.read_status() == 0 and wp.read_status() == 0
