@@ -6,7 +6,7 @@
 //
 // Two kernels (use_streamk says which, with the figures): one that starts and ends quickly for short caches and few of them,
 // described here, and one that streams at the copy rate for everything else, described at its place.  One layer of one user on 512
-// tokens takes 8 us; 64 layers of one on 8192 tokens 175 us, 6.1 TB/s; 8 users on 65536 tokens with heads of 256 175 us, 5.9 TB/s.
+// tokens takes 8 us; 64 layers of one on 8192 tokens 166 us, 6.5 TB/s; 8 users on 65536 tokens with heads of 256 168 us, 6.1 TB/s.
 //
 // A thread block of four warps takes a piece of one (layer, sequence, kv head) pair; a warp takes 16 tokens at a time,
 // straight from global memory into registers in the layout that the tensor core wants, so there is nothing to fill, no
@@ -391,7 +391,8 @@ paged_decode_kernel(const DecodeParams p) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kTileT = 64;
 constexpr int kThreadsP = (kConsumerWarps + 2) * 32;
-constexpr int kDumps = 2, kStages = 3;
+constexpr int kDumps = 2;
+constexpr int kMostStages = 5;            // tiles of the ring, if they fit
 constexpr int kAhead = 8;                 // tiles whose pages and scales the producer looks up at a time
 
 struct PagedMma {
@@ -411,7 +412,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const MmaParams& p = pp.m;
   const Geometry& g = p.g;
   const int G = g.group;
-  constexpr int stages = kStages;
+  const int stages = p.stages;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int gq = lane >> 2, tq = lane & 3;
   const uint32_t q_bytes = (uint32_t)G * D * 2;
@@ -531,10 +532,11 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       float2 sc2;
       look_up(0, id, row, layer, pair, sc);
       bool ok = true;
+      int s = 0, lap = 0;                   // slot of the ring, times around it
       for (int it0 = 0; it0 < n_it && ok; it0 += kAhead) {
         look_up(it0 + kAhead, id2, row2, layer2, pair2_, sc2);
         for (int k = 0; k < kAhead && it0 + k < n_it; ++k) {
-          const int it = it0 + k, s = it % stages;
+          const int it = it0 + k;
           const int cur_pair = __shfl_sync(0xffffffffu, pair, 4 * k);
           if (cur_pair != seg_pair) {   // the G query rows of this pair
             const int qb = seg & 1;
@@ -549,7 +551,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             seg_pair = cur_pair;
             ++seg;
           }
-          if (it >= stages) ok = mbar_wait(empty0 + 8u * s, ((it / stages) - 1) & 1, timed_out, p.status);
+          if (lap) ok = mbar_wait(empty0 + 8u * s, (lap - 1) & 1, timed_out, p.status);
           __syncwarp();
           if (!ok) break;
           const uint32_t fb = full0 + 8u * s;
@@ -569,6 +571,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
           }
           if (lane == 0) { sFlags[3] = it + 1; sFlags[1] = seg; }   // for the drain after a wait that ran out
+          if (++s == stages) { s = 0; ++lap; }
         }
         id = id2; row = row2; layer = layer2; pair = pair2_; sc = sc2;
       }
@@ -580,7 +583,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   } else if (has_work) {
     Cursor c = locate(r0, sCum, sLen, g.batch, g.h_kv);
     long long cur = r0;
-    int it = 0, seg = 0;
+    int s = 0, lap = 0, seg = 0;
     const uint32_t sK_addr = smem_u32(sK), sV_addr = smem_u32(sV);
     const int row_lo = warp * 16 + gq;
     while (cur < r1) {
@@ -632,9 +635,8 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
       for (int j = 0; j < KSTEPS; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
 
-      for (int ti = 0; ti < ntiles; ++ti, ++it) {
-        const int s = it % stages;
-        const bool ok = mbar_wait(full0 + 8u * s, (it / stages) & 1, timed_out, p.status);
+      for (int ti = 0; ti < ntiles; ++ti) {
+        const bool ok = mbar_wait(full0 + 8u * s, lap & 1, timed_out, p.status);
         const int tok0 = (c.tile + ti) * kTileT + warp * 16;
         const float2 sc = sScale[s * 4 + warp];
         if (ok && tok0 < c.len_b && sc.x >= 0.f) {
@@ -708,6 +710,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty0 + 8u * s);
+        if (++s == stages) { s = 0; ++lap; }
       }
       // ---- end of the segment: the warp's state to the epilogue warp ----
 #pragma unroll
@@ -756,24 +759,26 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   if (sComb->valid && !sFlags[0]) combine_deferred<D>(combine_args_of(p, nullptr, 0), *sComb, warp, kThreadsP / 32, lane);
 }
 
-size_t streamk_smem(const PagedGeometry& g) {
+size_t streamk_smem(const PagedGeometry& g, int stages) {
   size_t b = 1024;
-  b += (size_t)2 * kStages * kTileT * g.head_dim;
+  b += (size_t)2 * stages * kTileT * g.head_dim;
   b += (size_t)2 * g.group * g.head_dim * 2;
   b += (size_t)kDumps * kConsumerWarps * g.group * (g.head_dim + 4) * 4;
   b += (size_t)kDumps * kConsumerWarps * 16 * 4;
-  b += (size_t)kStages * 4 * 8;
-  b += (size_t)(2 * kStages + 8) * 8;
+  b += (size_t)stages * 4 * 8;
+  b += (size_t)(2 * stages + 8) * 8;
   b += sizeof(DeferredCombine) + 32;
   b += (size_t)(2 * g.batch + 1) * 4;
   return (b + 15) & ~(size_t)15;
 }
-// CTAs of the persistent grid: every slot of the device (three per SM with heads of 128).
-int streamk_ctas(const PagedGeometry& g) {
-  int per_sm = (int)((227 * 1024) / (streamk_smem(g) + 1024));
-  const int most = g.head_dim == 128 ? 3 : 1;
-  per_sm = per_sm < 1 ? 1 : per_sm > most ? most : per_sm;
-  return per_sm * device_sms();
+// CTAs per SM of the persistent grid, and the ring with which they fit.  Heads of 128, 32 sequences to 16384 tokens / 64 layers x 8192: three
+// CTAs with 3 tiles 101 / 177 us, two with 3, 4, 5, 6 tiles 93 / 172, 89 / 167, 89 / 166, 89 / 166; heads of 256, 8 x 65536: one CTA
+// with 3, 4, 5 tiles 174, 168, 168, two with 2 tiles 206.
+int streamk_ctas_per_sm(const PagedGeometry& g) { return g.head_dim == 128 ? 2 : 1; }
+int streamk_stages(const PagedGeometry& g) {
+  int n = kMostStages;
+  while (n > 2 && (streamk_smem(g, n) + 1024) * streamk_ctas_per_sm(g) > 227 * 1024) --n;
+  return n;
 }
 
 // Longest sequence a call can meet, as far as the host knows.
@@ -783,13 +788,14 @@ long long most_tokens(const PagedGeometry& g, int max_seq_len) {
 }
 
 // Which kernel: the register kernel starts and ends faster, the stream-K kernel streams faster and balances.  Heads of 128,
-// register / stream-K, us: 256 tokens, 8 pairs 7.0 / 9.6, 1024 pairs 21.0 / 27.6; 1024 tokens, 8 pairs 9.3 / 14.7, 1024 pairs
-// 55 / 64; 2048 tokens, 64 pairs 15.4 / 20.3, 256 pairs 41 / 37, 1024 pairs 100 / 102; 8192 tokens, 8 pairs 16 / 35, 64 pairs
-// 46 / 38, 1024 pairs 366 / 343.  Heads of 256 cross over at about half as many tokens.
+// register / stream-K, us: 256 tokens, 8 pairs 6.4 / 8.5, 1024 pairs 20 / 23; 512 tokens, 256 pairs 13.9 / 12.5, 1024 pairs 32 / 34;
+// 1024 tokens, 8 pairs 9.7 / 10.2, 256 pairs 23 / 18, 1024 pairs 55 / 55; 2048 tokens, 64 pairs 15.3 / 15.7, 1024 pairs 100 / 93; 8192
+// tokens, 8 pairs 17 / 20, 64 pairs 33 / 31, 1024 pairs 392 / 358.  Heads of 256: 512 tokens, 512 pairs 34 / 37; 1024 tokens, 128 pairs
+// 25 / 20; 2048 tokens, 32 pairs 16 / 18; 8192 tokens, 32 pairs 34 / 34, 128 pairs 173 / 98.
 bool use_streamk(const PagedGeometry& g, int max_seq_len) {
   if (g.batch > kMaxBatchMma || (long long)g.n_pages * g.h_kv * g.page_size > 0x7fffffffLL) return false;
-  const long long bytes = most_tokens(g, max_seq_len) * g.head_dim, pairs = (long long)g.n_layers * g.batch * g.h_kv;
-  return bytes > 1024 * 128 && bytes * pairs > 131072LL * 128;
+  const long long most = most_tokens(g, max_seq_len), pairs = (long long)g.n_layers * g.batch * g.h_kv;
+  return most > 768 && most * g.head_dim * pairs > (1LL << 24);
 }
 
 // Register kernel: pieces per pair.  Joining costs about 4 us and grows with their number, so few pairs are cut into up to 16,
@@ -836,15 +842,15 @@ cudaError_t launch_paged_streamk(const PagedGeometry& g, const PagedAttnArgs& a,
   m.out = (uint16_t*)a.out;
   m.out_hq_total = g.h_q;
   m.status = a.status;
-  const int n = streamk_ctas(g);
-  const size_t smem = streamk_smem(g);
+  m.stages = streamk_stages(g);
+  const int n = streamk_ctas_per_sm(g) * device_sms();
+  const size_t smem = streamk_smem(g, m.stages);
   auto launch = [&](auto kernel) -> cudaError_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, n, kThreadsP, smem, stream, kmap, vmap, p);
   };
-  if (g.head_dim != 128) return launch(paged_streamk_kernel<256, 1>);
-  return n <= 2 * device_sms() ? launch(paged_streamk_kernel<128, 2>) : launch(paged_streamk_kernel<128, 3>);
+  return g.head_dim == 128 ? launch(paged_streamk_kernel<128, 2>) : launch(paged_streamk_kernel<256, 1>);
 }
 
 }  // namespace
