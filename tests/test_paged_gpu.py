@@ -607,3 +607,32 @@ def test_captured_calls_follow_lengths_and_share_workspaces(pkg, cuda_device):
                 want, big = ref.attention(q[0, rows], kb[0], vb[0], ks[0], vs[0], table[i], lens[i], causal=q is not qs[0])
                 ref.assert_attention(out[0, rows], want, big, (turn, i, starts))
     assert wd.read_status() == 0 and wp.read_status() == 0
+
+
+def test_pools_strided_over_layers(pkg, cuda_device):
+    """Every other layer of a larger pool, keys and values at different strides: appended to and attended; the layers between stay."""
+    g = torch.Generator().manual_seed(17)
+    h_q, h_kv, d, page, lens = 10, 2, 128, 32, [100, 45]
+    kb = torch.full((4, 9, h_kv, page, d), 0x11, dtype=torch.uint8, device=cuda_device)
+    vb = torch.full((6, 9, h_kv, page, d), 0x22, dtype=torch.uint8, device=cuda_device)
+    ks, vs = (torch.ones(2, 9, h_kv, device=cuda_device) for _ in range(2))
+    table = torch.full((2, 700), -1, dtype=torch.int32)
+    table[0, :4], table[1, :2] = torch.tensor([8, 1, 5, 0]), torch.tensor([3, 7])
+    pools = (kb[::2], vb[::3], ks, vs, table.to(cuda_device))
+    q, k, v = (torch.randn(2, sum(lens), h, d, generator=g).to(torch.bfloat16).to(cuda_device) for h in (h_q, h_kv, h_kv))
+    starts = torch.tensor([0, 100, 145], dtype=torch.int32, device=cuda_device)
+    pos, status = torch.zeros(2, dtype=torch.int32, device=cuda_device), torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    pkg.paged_rope_append(None, k, v, None, None, *pools, pos, q_start=starts, status=status)
+    assert (kb[1::2] == 0x11).all() and (vb[[1, 2, 4, 5]] == 0x22).all() and status.item() == 0
+    shape = pkg.make_paged_shape(h_q, *pools[:3], pools[4])
+    n, first = torch.tensor(lens, dtype=torch.int32, device=cuda_device), torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda_device)
+    wp, last = pkg.PagedWorkspace(shape, cuda_device, q_tokens=145), q[:, [99, 144]].contiguous()
+    outs = [pkg.paged_decode_attention(last, *pools, n, workspace=pkg.PagedWorkspace(shape, cuda_device, max_seq_len=most)) for most in (100, 22400)]
+    outs.append(pkg.paged_prefill_attention(last, first, *pools, n, workspace=wp))
+    outs.append(pkg.paged_prefill_attention(q, starts, *pools, n, workspace=wp)[:, [99, 144]])
+    for layer in range(2):
+        kl, vl, sk, sv = kb[2 * layer].cpu(), vb[3 * layer].cpu(), ks[layer].cpu(), vs[layer].cpu()
+        for b, length in enumerate(lens):
+            want, big = ref.attention(last[layer, b:b + 1].cpu(), kl, vl, sk, sv, table[b], length)
+            for i, out in enumerate(outs):
+                ref.assert_attention(out[layer, b:b + 1].cpu(), want, big, (layer, b, i))
