@@ -6,6 +6,7 @@ missing and cannot be built, importing the ops fails loudly.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from pathlib import Path
 
@@ -141,6 +142,27 @@ def lib() -> ctypes.CDLL:
                            f"`python {PKG_DIR / 'build.py'}`")
     _lib = handle
     return _lib
+
+
+_binding = None
+
+
+def paged_binding():
+    """The paged calls as a Python extension module over the loaded library (csrc/paged_binding.cpp), built first when it is
+    absent or older than its sources."""
+    global _binding
+    if _binding is None:
+        from . import build as _build
+        handle, path = lib(), _build.build_binding()
+        spec = importlib.util.spec_from_file_location("_paged_binding", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if module.source_hash != _build.binding_hash():
+            raise RuntimeError(f"{path} was built from other sources: rebuild it with `python {PKG_DIR / 'build.py'}`")
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value
+                      for f in (handle.b200attn_paged_rope_append, handle.b200attn_paged_decode, handle.b200attn_paged_prefill)))
+        _binding = module
+    return _binding
 
 
 def check(code: int, where: str) -> int:

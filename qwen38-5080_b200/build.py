@@ -14,6 +14,7 @@ import hashlib
 import os
 import shutil
 import subprocess
+import sysconfig
 import sys
 from pathlib import Path
 
@@ -119,5 +120,45 @@ def _build_locked(verbose: bool, bounds: bool) -> Path:
     return LIB_PATH
 
 
+BINDING_PATH = PKG_DIR / "_paged_binding.so"
+
+
+def binding_hash() -> str:
+    """Hash of what the Python binding of the paged calls is compiled from and against (baked into it, see `build_binding`)."""
+    import torch
+    h = hashlib.sha256(f"{torch.__version__} {sys.version}".encode())
+    for d in (CSRC / "paged_binding.cpp", PKG_DIR.parent / "include" / "b200attn.h"):
+        h.update(d.read_bytes())
+    return h.hexdigest()[:16]
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile csrc/paged_binding.cpp (host code against torch's headers) into _paged_binding.so, unless it is up to date."""
+    stamp, digest = Path(str(BINDING_PATH) + ".hash"), binding_hash()
+
+    def current() -> bool:
+        return not force and BINDING_PATH.exists() and stamp.exists() and stamp.read_text().strip() == digest
+    if current():
+        return BINDING_PATH
+    with open(PKG_DIR / ".build.lock", "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if current():
+            return BINDING_PATH
+        import torch
+        at, tmp = Path(torch.__file__).parent, BINDING_PATH.with_suffix(".so.tmp")
+        res = subprocess.run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+                              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DB200ATTN_BINDING_HASH="{digest}"',
+                              f"-I{at / 'include'}", f"-I{at / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
+                              str(CSRC / "paged_binding.cpp"), f"-L{at / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)],
+                             stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if res.returncode:
+            sys.stderr.write(res.stdout)
+            raise RuntimeError("g++ failed on paged_binding.cpp")
+        os.replace(tmp, BINDING_PATH)
+        stamp.write_text(digest + "\n")
+    return BINDING_PATH
+
+
 if __name__ == "__main__":
+    print(build_binding(force=True))
     print(build(verbose="-v" in sys.argv, force=True, bounds="--bounds" in sys.argv))

@@ -21,24 +21,16 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import B200AttnPagedShape, B200AttnRope, check
+from ._lib import B200AttnPagedShape, check
 
 _BYTE_TYPES = (torch.uint8, torch.float8_e4m3fn)
-_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _need(idx: int, dtype, names: str, *tensors) -> None:
-    """Every given tensor (None = not given): on CUDA device `idx`, contiguous, of type `dtype`.  `names` in the same order."""
-    for t in tensors:
-        if t is not None and (t.get_device() != idx or t.dtype is not dtype or not t.is_contiguous() or idx < 0):
-            name = names.split()[[x is t for x in tensors].index(True)]
-            if idx < 0 or t.get_device() != idx:
-                raise ValueError(f"{name} must be on the cache's CUDA device: there is no CPU path")
-            raise ValueError(f"{name} must be contiguous {dtype}, not {'' if t.is_contiguous() else 'strided '}{t.dtype}")
-
-
-def _call(idx: int, fn, *args) -> int:
-    """fn(*args, stream) on device `idx`, which is made current for the call if it is not, and its current stream."""
+def _call(k_pages, fn, *args) -> int:
+    """fn(*args, stream) on the cache's device, which is made current for the call if it is not, and its current stream."""
+    idx = k_pages.get_device()
+    if idx < 0:
+        raise ValueError("the cache must be on a CUDA device: there is no CPU path")
     if torch._C._cuda_getDevice() == idx:
         return fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     with torch.cuda.device(idx):
@@ -88,13 +80,8 @@ class PagedWorkspace:
         return int(self.status.item())
 
 
-def _cache_device(k_pages, v_pages, k_scale, v_scale, page_table) -> int:
-    idx = k_pages.get_device()
-    _need(idx, _F32, "k_scale v_scale", k_scale, v_scale)
-    _need(idx, _I32, "page_table", page_table)
-    if v_pages.get_device() != idx or v_scale.numel() != k_scale.numel():
-        raise ValueError("k_pages / v_pages and k_scale / v_scale must match")
-    return idx
+def _scratch(w: PagedWorkspace | None):
+    return (w.buf, w.nbytes, w.status, w.max_seq_len) if w is not None else (None, 0, None, 0)
 
 
 def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, seq_pos, *, q_start=None,
@@ -108,54 +95,10 @@ def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, pag
     [rotary_dim / 2] saying which axis turns which pair.  Norm weights bf16 [n_layers, head_dim]: RMS norm with weight 1 + w
     before the rotation.  `seq_pos`: tokens cached before the call, advanced afterwards if `advance`.  Capacity, bad pages
     and bad positions are reported in `status`."""
-    h_q = q.shape[-2] if q is not None else k_pages.shape[-3]
-    shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
-    h_kv, d = shape.h_kv, shape.head_dim
-    idx = _cache_device(k_pages, v_pages, k_scale, v_scale, page_table)
-    _need(idx, _BF16, "q k v q_norm_weight k_norm_weight q_out", q, k, v, q_norm_weight, k_norm_weight, q_out)
-    _need(idx, _I32, "seq_pos q_start positions pair_axis status", seq_pos, q_start, positions, pair_axis, status)
-    _need(idx, _F32, "cos sin", cos, sin)
-    n_layers = shape.n_layers
-    n_tokens = k.numel() // (n_layers * h_kv * d)
-    if k.numel() != n_layers * n_tokens * h_kv * d or v.shape != k.shape or k.shape[-2:] != (h_kv, d):
-        raise ValueError("k and v must be [n_layers, n_tokens, h_kv, head_dim]")
-    if q is not None and (q.numel() != n_layers * n_tokens * h_q * d or q.shape[-1] != d):
-        raise ValueError("q must be [n_layers, n_tokens, h_q, head_dim]")
-    if seq_pos.numel() != shape.batch:
-        raise ValueError("seq_pos must be int32 [batch]")
-    if q_start is None and n_tokens != shape.batch:
-        raise ValueError("without q_start there is one token per sequence")
-    if q_start is not None and q_start.numel() != shape.batch + 1:
-        raise ValueError("q_start must be int32 [batch + 1]")
-    for w in (q_norm_weight, k_norm_weight):
-        if w is not None and w.numel() != n_layers * d:
-            raise ValueError("norm weights must be [n_layers, head_dim]")
-    rope = None
-    if cos is not None and cos.shape[-1] > 0:
-        if sin is None or cos.dim() != 2 or sin.shape != cos.shape:
-            raise ValueError("cos and sin must be [n_positions, rotary_dim / 2]")
-        n_axes = 1
-        if positions is not None:
-            n_axes = 1 if positions.dim() == 1 else positions.shape[0]
-            if positions.numel() != n_axes * n_tokens:
-                raise ValueError("positions must be [n_tokens] or [n_axes, n_tokens]")
-        if pair_axis is not None and pair_axis.numel() != cos.shape[-1]:
-            raise ValueError("pair_axis must be int32 [rotary_dim / 2]")
-        rope = B200AttnRope(cos.data_ptr(), sin.data_ptr(), positions.data_ptr() if positions is not None else None,
-                            pair_axis.data_ptr() if pair_axis is not None else None, cos.shape[0], n_axes, 2 * cos.shape[-1], 0)
-    if q is not None:
-        if q_out is None:
-            q_out = torch.empty_like(q)
-        elif q_out.numel() != q.numel():
-            raise ValueError("q_out must have q's shape")
-    if n_tokens == 0:
-        return q_out if q is not None else None
-    rc = _call(idx, _lib.lib().b200attn_paged_rope_append, ctypes.byref(shape), ctypes.byref(rope) if rope is not None else None, n_tokens,
-               q_start.data_ptr() if q_start is not None else None, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
-               q_norm_weight.data_ptr() if q_norm_weight is not None else None,
-               k_norm_weight.data_ptr() if k_norm_weight is not None else None, eps, q_out.data_ptr() if q is not None else None,
-               k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
-               seq_pos.data_ptr(), int(advance), status.data_ptr())
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q)
+    rc = _call(k_pages, _lib.paged_binding().append, q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, seq_pos, q_start,
+               positions, pair_axis, q_norm_weight, k_norm_weight, eps, advance, status, q_out)
     check(rc, "b200attn_paged_rope_append")
     return q_out if q is not None else None
 
@@ -164,25 +107,12 @@ def paged_decode_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, se
                            softmax_scale: float | None = None, seq_len_offset: int = 0, out: torch.Tensor | None = None):
     """Attention of one query token per sequence (q bf16 [n_layers, batch, h_q, head_dim]) over the first
     seq_len[b] + seq_len_offset tokens of its pages; bf16 with q's shape.  A sequence without tokens gives zeros."""
-    h_q, d = q.shape[-2:]
-    shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
-    idx = _cache_device(k_pages, v_pages, k_scale, v_scale, page_table)
-    _need(idx, _BF16, "q out", q, out)
-    _need(idx, _I32, "seq_len", seq_len)
-    if d != shape.head_dim or q.numel() != shape.n_layers * shape.batch * h_q * d:
-        raise ValueError("q must be [n_layers, batch, h_q, head_dim]")
-    if seq_len.numel() != shape.batch:
-        raise ValueError("seq_len must be int32 [batch]")
-    if workspace.q_tokens or workspace.buf.get_device() != idx:
-        raise ValueError("the workspace must be one for decode, on the cache's device")
     if out is None:
         out = torch.empty_like(q)
-    elif out.numel() != q.numel():
-        raise ValueError("out must have q's shape")
-    rc = _call(idx, _lib.lib().b200attn_paged_decode, ctypes.byref(shape), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-               k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(), seq_len_offset, workspace.max_seq_len,
-               d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(), workspace.nbytes, out.data_ptr(),
-               workspace.status.data_ptr())
+    if workspace is not None and workspace.q_tokens:
+        raise ValueError("the workspace must be one for decode, on the cache's device")
+    rc = _call(k_pages, _lib.paged_binding().decode, q, k_pages, v_pages, k_scale, v_scale, page_table, seq_len, seq_len_offset,
+               *_scratch(workspace), softmax_scale, out)
     check(rc, "b200attn_paged_decode")
     return out
 
@@ -192,28 +122,10 @@ def paged_prefill_attention(q, q_start, k_pages, v_pages, k_scale, v_scale, page
     """Attention of many query tokens per sequence (q bf16 [n_layers, n_tokens, h_q, head_dim], packed by `q_start`) over the
     first seq_len[b] tokens of its pages.  causal: a sequence's queries are its last tokens, each sees those up to itself;
     not causal: all (cross attention).  Rows that see nothing are zero; rows behind q_start[batch] are left as they were."""
-    h_q, d = q.shape[-2:]
-    shape = make_paged_shape(h_q, k_pages, v_pages, k_scale, page_table)
-    idx = _cache_device(k_pages, v_pages, k_scale, v_scale, page_table)
-    _need(idx, _BF16, "q out", q, out)
-    _need(idx, _I32, "seq_len q_start", seq_len, q_start)
-    n_tokens = q.numel() // (shape.n_layers * h_q * d)
-    if d != shape.head_dim or q.numel() != shape.n_layers * n_tokens * h_q * d:
-        raise ValueError("q must be [n_layers, n_tokens, h_q, head_dim]")
-    if seq_len.numel() != shape.batch or q_start.numel() != shape.batch + 1:
-        raise ValueError("seq_len must be int32 [batch], q_start int32 [batch + 1]")
-    if workspace.q_tokens < n_tokens or workspace.buf.get_device() != idx:
-        raise ValueError(f"the workspace must be one for {n_tokens} query tokens, on the cache's device")
     if out is None:
         out = torch.empty_like(q)
-    elif out.numel() != q.numel():
-        raise ValueError("out must have q's shape")
-    if n_tokens == 0:
-        return out
-    rc = _call(idx, _lib.lib().b200attn_paged_prefill, ctypes.byref(shape), n_tokens, q.data_ptr(), q_start.data_ptr(), k_pages.data_ptr(),
-               v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(),
-               workspace.max_seq_len, int(causal), d ** -0.5 if softmax_scale is None else softmax_scale, workspace.buf.data_ptr(),
-               workspace.nbytes, out.data_ptr(), workspace.status.data_ptr())
+    rc = _call(k_pages, _lib.paged_binding().prefill, q, k_pages, v_pages, k_scale, v_scale, page_table, seq_len, q_start,
+               workspace.q_tokens if workspace is not None else 0, causal, *_scratch(workspace), softmax_scale, out)
     check(rc, "b200attn_paged_prefill")
     return out
 

@@ -164,3 +164,17 @@ def test_workspace_bytes_do_not_depend_on_the_batch_or_the_length(pkg):
         return n.value
     for q_tokens in (0, 5):
         assert len({size(q_tokens, most, batch=b) for b in (1, 7, 900) for most in (0, 1, 100000)}) == 1
+
+
+def test_things_that_are_not_tensors_are_refused(pkg):
+    kp = torch.zeros(10, 8, 64, 128, dtype=torch.uint8)
+    sc, table, lens = torch.ones(10, 8), torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    q = torch.zeros(1, 40, 128, dtype=torch.bfloat16)
+    binding = pkg._lib.paged_binding()
+    for bad in ((3, kp), (q, "pages"), (q, None)):
+        with pytest.raises(TypeError):
+            binding.decode(bad[0], bad[1], kp, sc, sc, table, lens, 0, None, 0, None, 0, None, q, 0)
+    with pytest.raises(ValueError, match="arguments"):
+        binding.decode(q, kp)
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.paged_prefill_attention(q, lens, kp, kp, sc, sc, table, lens, workspace=None)

@@ -636,3 +636,54 @@ def test_pools_strided_over_layers(pkg, cuda_device):
             want, big = ref.attention(last[layer, b:b + 1].cpu(), kl, vl, sk, sv, table[b], length)
             for i, out in enumerate(outs):
                 ref.assert_attention(out[layer, b:b + 1].cpu(), want, big, (layer, b, i))
+
+
+def test_python_calls_refuse_wrong_tensors(pkg, cuda_device):
+    """Types, shapes, strides and devices that do not fit raise ValueError before anything is launched."""
+    z = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device=cuda_device)
+    bf, i32 = torch.bfloat16, torch.int32
+    good = dict(q=z(2, 10, 128, t=bf), k=z(2, 2, 128, t=bf), v=z(2, 2, 128, t=bf), cos=z(64, 64), sin=z(64, 64), k_pages=z(6, 2, 16, 128, t=torch.uint8),
+                v_pages=z(6, 2, 16, 128, t=torch.uint8), k_scale=z(6, 2), v_scale=z(6, 2), page_table=z(2, 3, t=i32), seq_pos=z(2, t=i32),
+                q_start=torch.tensor([0, 1, 2], dtype=i32, device=cuda_device), status=z(1, t=i32))
+    shape = pkg.make_paged_shape(10, good["k_pages"], good["v_pages"], good["k_scale"], good["page_table"])
+    wd, wp = pkg.PagedWorkspace(shape, cuda_device), pkg.PagedWorkspace(shape, cuda_device, q_tokens=2)
+    cache = ("k_pages", "v_pages", "k_scale", "v_scale", "page_table")
+
+    def append(**kw):
+        a = {**good, **kw}
+        return pkg.paged_rope_append(a["q"], a["k"], a["v"], a["cos"], a["sin"], *(a[n] for n in cache), a["seq_pos"], q_start=a.get("q_start"),
+                                     positions=a.get("positions"), pair_axis=a.get("pair_axis"), q_norm_weight=a.get("wq"), status=a["status"],
+                                     q_out=a.get("q_out"), advance=False)
+
+    def decode(**kw):
+        a = {**good, **kw}
+        return pkg.paged_decode_attention(a["q"], *(a[n] for n in cache), a["seq_pos"], workspace=a.get("ws", wd), out=a.get("out"))
+
+    def prefill(**kw):
+        a = {**good, **kw}
+        return pkg.paged_prefill_attention(a["q"], a["q_start"], *(a[n] for n in cache), a["seq_pos"], workspace=a.get("ws", wp), out=a.get("out"))
+    for call in (append, decode, prefill):
+        call()
+        for bad in (dict(q=z(2, 10, 128)), dict(q=z(2, 10, 256, t=bf)[..., ::2]), dict(q=z(2, 10, 64, t=bf)), dict(q=good["q"].cpu()), dict(seq_pos=z(3, t=i32)),
+                    dict(seq_pos=z(2)), dict(k_scale=z(6, 3)), dict(v_scale=z(5, 2)), dict(k_scale=z(6, 2, t=bf)), dict(page_table=z(6, t=i32)),
+                    dict(page_table=z(2, 3)), dict(v_pages=z(7, 2, 16, 128, t=torch.uint8)), dict(v_pages=z(6, 2, 16, 128)),
+                    dict(k_pages=z(6, 16, 2, 128, t=torch.uint8).transpose(1, 2)), dict(page_table=good["page_table"].cpu()), dict(q=z(2, 128, t=bf))):
+            with pytest.raises(ValueError):
+                call(**bad)
+        with pytest.raises((TypeError, AttributeError)):
+            call(v_pages=None)
+    for bad in (dict(k=z(2, 3, 128, t=bf)), dict(v=z(3, 2, 128, t=bf)), dict(k=None), dict(status=None), dict(sin=None), dict(sin=z(63, 64)), dict(cos=z(64)),
+                dict(positions=z(3, t=i32)), dict(positions=z(2, 3, t=i32)), dict(pair_axis=z(63, t=i32)), dict(wq=z(127, t=bf)), dict(wq=z(128)),
+                dict(q_out=z(2, 9, 128, t=bf)), dict(q_start=z(2, t=i32)), dict(q_start=None, k=z(1, 2, 128, t=bf), v=z(1, 2, 128, t=bf), q=z(1, 10, 128, t=bf))):
+        with pytest.raises(ValueError):
+            append(**bad)
+    for call, other in ((decode, wp), (prefill, wd)):
+        for bad in (dict(out=z(2, 9, 128, t=bf)), dict(out=z(2, 10, 128)), dict(ws=other), dict(ws=None)):
+            with pytest.raises(ValueError):
+                call(**bad)
+    with pytest.raises(ValueError):
+        prefill(q=z(3, 10, 128, t=bf))                       # more tokens than the workspace is for
+    with pytest.raises(ValueError):
+        decode(q=z(3, 10, 128, t=bf))
+    torch.cuda.synchronize()
+    assert good["status"].item() == 0 and wd.read_status() == 0 and wp.read_status() == 0
