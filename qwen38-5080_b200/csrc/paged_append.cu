@@ -13,6 +13,7 @@
 //
 // Bound: HBM bytes (query in and out, key and value in, bytes out), and for single tokens the launch.
 #include "paged.cuh"
+#include "streamk.cuh"
 
 namespace b200attn {
 
@@ -247,6 +248,8 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t u
 template <int D>
 __global__ void __launch_bounds__(128)
 paged_append_token_kernel(const AppendParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   constexpr int TPR = D / 8, RPW = 32 / TPR;
   const PagedGeometry& g = p.g;
   const int lane = threadIdx.x & 31, lr = lane % TPR;
@@ -319,6 +322,8 @@ paged_append_token_kernel(const AppendParams p) {
 template <int D, int NP, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 paged_append_prompt_kernel(const AppendParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   constexpr int TPR = D / 8, RPP = THREADS / TPR;
   const PagedGeometry& g = p.g;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -454,11 +459,14 @@ paged_append_prompt_kernel(const AppendParams p) {
 // The queries of prompts: a kernel of their own, with more warps on an SM than the one above has.
 template <int D>
 __global__ void __launch_bounds__(256, 3) paged_rotate_queries_kernel(const AppendParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit < p.q_units) rotate_queries<D, true>(p, unit);
 }
 
 __global__ void paged_advance_kernel(PagedGeometry g, const int* q_start, int* seq_pos) {
+  pdl_wait();
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= g.batch) return;
   const int n = q_start ? q_start[b + 1] - q_start[b] : 1, p = seq_pos[b];
@@ -496,10 +504,12 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
   const long long kv_rows = (long long)g.n_layers * g.batch * g.h_kv * 2;
   if (q_warps > 0x7fffffffLL || kv_rows > 0x7fffffffLL) return cudaErrorInvalidConfiguration;   // indices are 32-bit
   p.q_units = (uint32_t)q_warps;
+  cudaError_t e = cudaSuccess;
   if (!a.q_start) {
     const long long rpw = g.head_dim == 128 ? 2 : 1, grid = ((kv_rows + rpw - 1) / rpw + q_warps + 3) / 4;
-    if (g.head_dim == 128) paged_append_token_kernel<128><<<(unsigned)grid, 128, 0, stream>>>(p);
-    else paged_append_token_kernel<256><<<(unsigned)grid, 128, 0, stream>>>(p);
+    if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    e = g.head_dim == 128 ? launch_pdl(paged_append_token_kernel<128>, (int)grid, 128, 0, stream, p)
+                          : launch_pdl(paged_append_token_kernel<256>, (int)grid, 128, 0, stream, p);
   } else if (a.n_tokens > 0) {
     // pages that the call touches: n tokens touch at most n pages, and at most n / page_size + 2 (an open first and last page)
     const long long most = (long long)a.n_tokens / g.page_size + 2LL * g.batch;
@@ -512,10 +522,11 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
     const long long grid = pages * ((g.h_kv + p.heads - 1) / p.heads), q_grid = (q_warps + 7) / 8;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     if (q_grid) {
-      if (g.head_dim == 128) paged_rotate_queries_kernel<128><<<(unsigned)q_grid, 256, 0, stream>>>(p);
-      else paged_rotate_queries_kernel<256><<<(unsigned)q_grid, 256, 0, stream>>>(p);
+      e = g.head_dim == 128 ? launch_pdl(paged_rotate_queries_kernel<128>, (int)q_grid, 256, 0, stream, p)
+                            : launch_pdl(paged_rotate_queries_kernel<256>, (int)q_grid, 256, 0, stream, p);
+      if (e != cudaSuccess) return e;
     }
-    auto launch = [&](auto kernel) { kernel<<<(unsigned)grid, threads, 0, stream>>>(p); };
+    auto launch = [&](auto kernel) { e = launch_pdl(kernel, (int)grid, threads, 0, stream, p); };
     if (g.head_dim == 128) {
       switch (g.page_size) {
         case 16: launch(paged_append_prompt_kernel<128, 2, 128>); break;
@@ -532,12 +543,7 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
       }
     }
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  if (a.advance_pos) {
-    paged_advance_kernel<<<(g.batch + 127) / 128, 128, 0, stream>>>(g, a.q_start, a.seq_pos);
-    e = cudaGetLastError();
-  }
+  if (e == cudaSuccess && a.advance_pos) e = launch_pdl(paged_advance_kernel, (g.batch + 127) / 128, 128, 0, stream, g, a.q_start, a.seq_pos);
   return e;
 }
 
