@@ -462,7 +462,7 @@ typedef struct B200AttnRope {
 } B200AttnRope;
 
 /*
- * Rotate queries and keys and quantise-and-append keys and values to the pages, all layers in one launch.
+ * Rotate queries and keys and quantise-and-append keys and values to the pages, all layers in one call.
  *   q, q_out : bf16 [n_layers][n_tokens][h_q][head_dim]   (q_out may be q; both NULL: keys and values only)
  *   k, v     : bf16 [n_layers][n_tokens][h_kv][head_dim]
  *   q_start  : i32 [batch + 1] on the device; NULL: one token per sequence, n_tokens == batch

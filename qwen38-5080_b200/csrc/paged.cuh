@@ -60,6 +60,29 @@ inline int* paged_counters(void* ws) { return (int*)ws; }
 inline unsigned long long* paged_words(void* ws) { return (unsigned long long*)((uint8_t*)ws + paged_words_offset()); }
 inline float* paged_partials(void* ws) { return (float*)((uint8_t*)ws + paged_partials_offset()); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pair2(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split2(unsigned long long p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Valid length of a sequence: negative lengths count as 0, lengths beyond the table's capacity are clamped to it.
 __device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* status, bool report) {
   const long long cap = (long long)g.max_pages * g.page_size;

@@ -134,12 +134,13 @@ struct Rotation {
     }
   }
   __device__ __forceinline__ void turn(float (&x)[8]) const {
-    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    const unsigned long long cc[2] = {pair2(c.x, c.y), pair2(c.z, c.w)}, ss[2] = {pair2(s.x, s.y), pair2(s.z, s.w)};
+    const unsigned long long nn[2] = {pair2(-s.x, -s.y), pair2(-s.z, -s.w)};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float u = x[e], v = x[4 + e];
-      x[e] = u * cc[e] - v * ss[e];
-      x[4 + e] = v * cc[e] + u * ss[e];
+    for (int e = 0; e < 2; ++e) {
+      const unsigned long long u = pair2(x[2 * e], x[2 * e + 1]), v = pair2(x[4 + 2 * e], x[5 + 2 * e]);
+      split2(fma2(u, cc[e], mul2(v, nn[e])), x[2 * e], x[2 * e + 1]);
+      split2(fma2(v, cc[e], mul2(u, ss[e])), x[4 + 2 * e], x[5 + 2 * e]);
     }
   }
 };
@@ -147,14 +148,21 @@ struct Rotation {
 // RMS norm over the head's lanes; every lane of the warp calls it.
 template <int D>
 __device__ __forceinline__ void rms_norm(float (&x)[8], const float (&w1)[8], float eps) {
-  float ss = 0.f;
+  unsigned long long y[4], sum = 0ull;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+  for (int e = 0; e < 4; ++e) {
+    y[e] = pair2(x[2 * e], x[2 * e + 1]);
+    sum = fma2(y[e], y[e], sum);
+  }
+  float ss, odd;
+  split2(sum, ss, odd);
+  ss += odd;
 #pragma unroll
   for (int off = D / 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
   const float inv = __frsqrt_rn(ss * (1.f / D) + eps);
+  const unsigned long long inv2 = pair2(inv, inv);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w1[e];
+  for (int e = 0; e < 4; ++e) split2(mul2(mul2(y[e], inv2), pair2(w1[2 * e], w1[2 * e + 1])), x[2 * e], x[2 * e + 1]);
 }
 template <int D>
 __device__ __forceinline__ void load_norm(const uint16_t* w, int layer, const Share<D>& sh, float (&w1)[8]) {

@@ -87,7 +87,7 @@ def _scratch(w: PagedWorkspace | None):
 def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, seq_pos, *, q_start=None,
                       positions=None, pair_axis=None, q_norm_weight=None, k_norm_weight=None, eps: float = 1e-6,
                       advance: bool = True, status: torch.Tensor, q_out: torch.Tensor | None = None):
-    """Rotate queries and keys and quantise-and-append keys and values to the pages, in one launch; returns the rotated
+    """Rotate queries and keys and quantise-and-append keys and values to the pages, all layers in one call; returns the rotated
     queries (None if `q` is None).
 
     Without `q_start`: one token per sequence.  `cos`, `sin`: fp32 tables [n_positions, rotary_dim / 2] (None: no rotation);
