@@ -60,6 +60,12 @@ inline int* paged_counters(void* ws) { return (int*)ws; }
 inline unsigned long long* paged_words(void* ws) { return (unsigned long long*)((uint8_t*)ws + paged_words_offset()); }
 inline float* paged_partials(void* ws) { return (float*)((uint8_t*)ws + paged_partials_offset()); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ unsigned long long pair2(float x, float y) {
   unsigned long long r;

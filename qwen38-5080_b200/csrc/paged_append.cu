@@ -90,12 +90,22 @@ __device__ __forceinline__ uint2 pack4(const float* x) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(x[0], x[1]), q = __floats2bfloat162_rn(x[2], x[3]);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
 }
+// 1 / s, of a power of two by its exponent (scales that the append made are)
+__device__ __forceinline__ float reciprocal(float s) {
+  const uint32_t bits = __float_as_uint(s), e = bits >> 23;
+  return (bits & 0x7FFFFFu) == 0 && e >= 1 && e < 254 ? __uint_as_float((254u - e) << 23) : __fdiv_rn(1.f, s);
+}
 // 4 floats -> 4 e4m3 bytes: nearest even, saturating at 448; NaN -> 0x7F
 __device__ __forceinline__ uint32_t quant4(const float* x, float inv) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1] * inv), "f"(x[0] * inv));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3] * inv), "f"(x[2] * inv));
-  return (uint32_t)lo | ((uint32_t)hi << 16);
+  uint32_t bytes;
+  float x0, x1, x2, x3;
+  split2(mul2(pair2(x[0], x[1]), pair2(inv, inv)), x0, x1);
+  split2(mul2(pair2(x[2], x[3]), pair2(inv, inv)), x2, x3);
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}" : "=r"(bytes) : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+  return bytes;
 }
 // 16 e4m3 bytes re-expressed in a larger power-of-two scale: value * ratio, ratio = old / new < 1
 __device__ __forceinline__ uint4 rescale16(const uint4& raw, float ratio) {
@@ -381,17 +391,25 @@ paged_append_prompt_kernel(const AppendParams p) {
   const int lo = max(pos - slot0, 0);                                                   // rows [lo, hi) are new
   const int hi = (int)min((long long)g.page_size, (long long)pos + nt - slot0);
   const Share<D> sh(lane, p.rot);
-  const uint16_t* src = (which ? p.v : p.k) + ((long long)layer * p.n_tokens + q0 + slot0 - pos) * g.h_kv * D;
+  // the thread's first row of the next head, and whether its rows are new (addresses by addition: computed anew for every row and head
+  // they were a third of the kernel's instructions)
+  const uint16_t* src = (which ? p.v : p.k) + (((long long)layer * p.n_tokens + q0 + slot0 - pos + tid / TPR) * g.h_kv + h_first) * D;
+  const int row_step = RPP * g.h_kv * D;
+  bool is_new[NP];
   Raw raw[NP];
-  auto load = [&](int h) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int row = i * RPP + tid / TPR;
-      raw[i] = Raw{make_uint2(0, 0), make_uint2(0, 0)};
-      if (row >= lo && row < hi) raw[i] = load_row<D>(src + ((long long)row * g.h_kv + h) * D, sh);
-    }
+  for (int i = 0; i < NP; ++i) {
+    const int row = i * RPP + tid / TPR;
+    is_new[i] = row >= lo && row < hi;
+    raw[i] = Raw{make_uint2(0, 0), make_uint2(0, 0)};     // rows that are not new stay zero
+  }
+  auto load = [&]() {
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (is_new[i]) raw[i] = load_row<D>(src + i * row_step, sh);
+    src += D;
   };
-  load(h_first);
+  load();
   const int page = page_index < g.max_pages ? page_of(p, b, page_index) : -1;
   if (page < 0) {
     if (tid == 0) atomicOr(p.status, page_index < g.max_pages ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);
@@ -405,15 +423,15 @@ paged_append_prompt_kernel(const AppendParams p) {
       rot[i].load<D>(p, sh, q0 + slot0 + row - pos, slot0 + row);
     }
   float* scales = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv;
-  uint8_t* pages = (which ? p.v_pages : p.k_pages) + (long long)layer * (which ? g.v_layer_stride : g.k_layer_stride) +
-                   (long long)page * g.h_kv * g.page_size * D;
+  uint8_t* base = (which ? p.v_pages : p.k_pages) + (long long)layer * (which ? g.v_layer_stride : g.k_layer_stride) +
+                   ((long long)page * g.h_kv + h_first) * g.page_size * D;   // the page of the head
 #pragma unroll 1
-  for (int h = h_first; h < h_end; ++h) {
+  for (int h = h_first; h < h_end; ++h, base += g.page_size * D) {
     float x[NP][8];
 #pragma unroll
     for (int i = 0; i < NP; ++i) unpack(raw[i], x[i]);
     const float old = lo > 0 ? scales[h] : 0.f;
-    if (h + 1 < h_end) load(h + 1);
+    if (h + 1 < h_end) load();
     if (!which && p.wk) {
       float w1[8];
       load_norm<D>(p.wk, layer, sh, w1);
@@ -425,7 +443,7 @@ paged_append_prompt_kernel(const AppendParams p) {
     for (int i = 0; i < NP; ++i) {
       if (!which && sh.on) rot[i].turn(x[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][e]));   // rows that are not new are zero; NaN is passed over
+      for (int e = 0; e < 8; e += 2) amax = max3(amax, fabsf(x[i][e]), fabsf(x[i][e + 1]));   // NaN is passed over
     }
     amax = warp_max(amax);
     if (amax > kFltMax) {                                 // infinities among them: once more without
@@ -440,7 +458,6 @@ paged_append_prompt_kernel(const AppendParams p) {
     __syncthreads();                                      // maxima are in; every thread has read the old scale
     amax = warp_max(lane < THREADS / 32 ? s_max[h & 1][lane] : 0.f);
     float s = pow2_scale(amax);
-    uint8_t* base = pages + (long long)h * g.page_size * D;
     if (lo > 0) {
       if (s > old) {
         const float ratio = old / s;
@@ -451,12 +468,12 @@ paged_append_prompt_kernel(const AppendParams p) {
       }
     }
     if (tid == 0) scales[h] = s;
-    const float inv = __fdiv_rn(1.f, s);
+    const float inv = reciprocal(s);
+    uint8_t* rows = base + tid / TPR * D;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int row = i * RPP + tid / TPR;
-      if (row >= lo && row < hi) {
-        uint8_t* dst = base + (long long)row * D;
+      if (is_new[i]) {
+        uint8_t* dst = rows + i * RPP * D;
         *reinterpret_cast<uint32_t*>(dst + sh.a) = quant4(x[i], inv);
         *reinterpret_cast<uint32_t*>(dst + sh.b) = quant4(x[i] + 4, inv);
       }
