@@ -89,6 +89,11 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
   return r;
 }
 
+// Plain loads, not the non-coherent ones: a dependent launch can begin while the kernel that writes the data still runs (it reads them
+// after its wait), and non-coherent loads are for data that nobody writes during the kernel.
+template <class T>
+__device__ __forceinline__ T ld(const T* p) { return *p; }
+
 // Valid length of a sequence: negative lengths count as 0, lengths beyond the table's capacity are clamped to it.
 __device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* status, bool report) {
   const long long cap = (long long)g.max_pages * g.page_size;

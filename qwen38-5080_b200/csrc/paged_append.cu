@@ -73,7 +73,7 @@ struct Raw { uint2 a, b; };
 // Read once: not worth a line of L1.
 __device__ __forceinline__ uint2 ldg_once(const uint16_t* p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 template <int D>
@@ -129,18 +129,18 @@ struct Rotation {
     if (p.rot == 0) return;
     const int half = p.rot >> 1, j0 = sh.on ? sh.a : 0;
     if (p.pair_axis == nullptr) {
-      const int pos = clamped(p, p.positions ? __ldg(p.positions + token) : slot, false, sh.on);
-      c = __ldg(reinterpret_cast<const float4*>(p.cos + (long long)pos * half + j0));
-      s = __ldg(reinterpret_cast<const float4*>(p.sin + (long long)pos * half + j0));
+      const int pos = clamped(p, p.positions ? ld(p.positions + token) : slot, false, sh.on);
+      c = ld(reinterpret_cast<const float4*>(p.cos + (long long)pos * half + j0));
+      s = ld(reinterpret_cast<const float4*>(p.sin + (long long)pos * half + j0));
     } else {
-      const int4 ax = __ldg(reinterpret_cast<const int4*>(p.pair_axis + j0));
+      const int4 ax = ld(reinterpret_cast<const int4*>(p.pair_axis + j0));
       int at[4];
 #pragma unroll
-      for (int a = 0; a < 4; ++a) at[a] = !p.positions ? slot : a < p.n_axes ? __ldg(p.positions + (long long)a * p.n_tokens + token) : 0;
+      for (int a = 0; a < 4; ++a) at[a] = !p.positions ? slot : a < p.n_axes ? ld(p.positions + (long long)a * p.n_tokens + token) : 0;
       auto pick = [&](int a) { return (long long)clamped(p, a == 1 ? at[1] : a == 2 ? at[2] : a == 3 ? at[3] : at[0], a < 0 || a >= p.n_axes, sh.on) * half + j0; };
       const long long i0 = pick(ax.x), i1 = pick(ax.y) + 1, i2 = pick(ax.z) + 2, i3 = pick(ax.w) + 3;
-      c = make_float4(__ldg(p.cos + i0), __ldg(p.cos + i1), __ldg(p.cos + i2), __ldg(p.cos + i3));
-      s = make_float4(__ldg(p.sin + i0), __ldg(p.sin + i1), __ldg(p.sin + i2), __ldg(p.sin + i3));
+      c = make_float4(ld(p.cos + i0), ld(p.cos + i1), ld(p.cos + i2), ld(p.cos + i3));
+      s = make_float4(ld(p.sin + i0), ld(p.sin + i1), ld(p.sin + i2), ld(p.sin + i3));
     }
   }
   __device__ __forceinline__ void turn(float (&x)[8]) const {
@@ -177,7 +177,7 @@ __device__ __forceinline__ void rms_norm(float (&x)[8], const float (&w1)[8], fl
 template <int D>
 __device__ __forceinline__ void load_norm(const uint16_t* w, int layer, const Share<D>& sh, float (&w1)[8]) {
   const uint16_t* row = w + (long long)layer * D;
-  const Raw r{__ldg(reinterpret_cast<const uint2*>(row + sh.a)), __ldg(reinterpret_cast<const uint2*>(row + sh.b))};
+  const Raw r{ld(reinterpret_cast<const uint2*>(row + sh.a)), ld(reinterpret_cast<const uint2*>(row + sh.b))};
   unpack(r, w1);
 #pragma unroll
   for (int e = 0; e < 8; ++e) w1[e] += 1.f;
@@ -188,7 +188,7 @@ __device__ __forceinline__ int sequence_of(const int* q_start, int batch, int t)
   int lo = 0, hi = batch - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(q_start + mid) <= t) lo = mid; else hi = mid - 1;
+    if (ld(q_start + mid) <= t) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -228,11 +228,11 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t u
   load(g_first);
   int b = token, slot;
   if (p.q_start) {
-    if (token >= __ldg(p.q_start + p.g.batch) || token < __ldg(p.q_start)) return;   // a row that belongs to nobody
+    if (token >= ld(p.q_start + p.g.batch) || token < ld(p.q_start)) return;   // a row that belongs to nobody
     b = sequence_of(p.q_start, p.g.batch, token);
-    slot = __ldg(p.seq_pos + b) + token - __ldg(p.q_start + b);
+    slot = ld(p.seq_pos + b) + token - ld(p.q_start + b);
   } else {
-    slot = __ldg(p.seq_pos + b);
+    slot = ld(p.seq_pos + b);
   }
   Rotation rot;
   rot.load<D>(p, sh, token, slot);
@@ -285,7 +285,7 @@ paged_append_token_kernel(const AppendParams p) {
   const int b = (int)(lb % g.batch), layer = (int)(lb / g.batch);
   const Share<D> sh(lane, p.rot);
   const Raw raw = load_row<D>((which ? p.v : p.k) + (long long)row * D, sh);
-  const int pos = __ldg(p.seq_pos + b);
+  const int pos = ld(p.seq_pos + b);
   const bool fits = pos >= 0 && pos < (long long)g.max_pages * g.page_size;
   const int page = fits ? page_of(p, b, pos / g.page_size) : -1, fill = fits ? pos % g.page_size : 0;
   if (page < 0 && lr == 0) atomicOr(p.status, fits ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);

@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t widen_lo(uint32_t w) { return e4m3x2_to_f16x
 __device__ __forceinline__ uint32_t widen_hi(uint32_t w) { return e4m3x2_to_f16x2((uint16_t)(w >> 16)); }
 __device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -517,7 +517,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         pair_ = (c.layer * g.batch + c.b) * g.h_kv + c.h;
         const int tok = c.tile * kTileT + (lane & 3) * 16;
         if (tok >= c.len_b) return;
-        const int page = __ldg(pp.page_table + (long long)c.b * pp.g.max_pages + (tok >> pp.page_shift));
+        const int page = ld(pp.page_table + (long long)c.b * pp.g.max_pages + (tok >> pp.page_shift));
         if (page < 0 || page >= pp.g.n_pages) {
           atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
           sc_.x = -1.f;
@@ -526,7 +526,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         id_ = page;
         row_ = ((page * g.h_kv + c.h) << pp.page_shift) + (tok & (pp.g.page_size - 1));
         const long long si = ((long long)c.layer * pp.g.n_pages + page) * g.h_kv + c.h;
-        sc_ = make_float2(__ldg(p.k_scale + si), __ldg(p.v_scale + si));
+        sc_ = make_float2(ld(p.k_scale + si), ld(p.v_scale + si));
       };
       int id2, row2, layer2, pair2_;
       float2 sc2;

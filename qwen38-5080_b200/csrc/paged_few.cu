@@ -136,11 +136,11 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     sc = make_float2(-1.f, 0.f);
     if (i0 + lane >= n) return;
     const int tok = (u0 + (i0 + lane) * kWarps) * kRowsU;
-    const int page = __ldg(p.page_table + (long long)b * g.max_pages + (tok >> p.page_shift));
+    const int page = ld(p.page_table + (long long)b * g.max_pages + (tok >> p.page_shift));
     if (page < 0 || page >= g.n_pages) { atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE); return; }
     row = ((page * g.h_kv + h) << p.page_shift) + (tok & (g.page_size - 1));
     const long long si = ((long long)layer * g.n_pages + page) * g.h_kv + h;
-    sc = make_float2(__ldg(p.k_scale + si), __ldg(p.v_scale + si));
+    sc = make_float2(ld(p.k_scale + si), ld(p.v_scale + si));
   };
   int row, next_row;
   float2 sc, next_sc;
@@ -181,7 +181,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 raw = make_uint4(0, 0, 0, 0);
-        if (real) raw = __ldg(reinterpret_cast<const uint4*>(p.q + (row0 + (long long)tok * g.h_q + col % G) * D + hf * 128 + 32 * tq + 8 * i));
+        if (real) raw = ld(reinterpret_cast<const uint4*>(p.q + (row0 + (long long)tok * g.h_q + col % G) * D + hf * 128 + 32 * tq + 8 * i));
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

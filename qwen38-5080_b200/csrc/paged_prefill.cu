@@ -392,13 +392,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     auto page_at = [&](int j) -> int {
       const int key = (j0 + j) * kKeys + lane * 16;
       if (lane >= 8 || j >= nt || key >= key_end) return -2;   // no key
-      return max(-1, __ldg(p.page_table + (long long)b * g.max_pages + (key >> p.page_shift)));
+      return max(-1, ld(p.page_table + (long long)b * g.max_pages + (key >> p.page_shift)));
     };
     auto scales_at = [&](int id) -> float2 {
       if (id == -2) return make_float2(0.f, 0.f);
       if (id < 0 || id >= g.n_pages) return make_float2(-1.f, 0.f);
       const long long si = ((long long)layer * g.n_pages + id) * g.h_kv + h;
-      return make_float2(__ldg(p.k_scale + si), __ldg(p.v_scale + si));
+      return make_float2(ld(p.k_scale + si), ld(p.v_scale + si));
     };
     auto publish = [&](int j, int id, float2 sc) {
       if (j >= nt) return;
