@@ -483,12 +483,14 @@ paged_append_prompt_kernel(const AppendParams p) {
   }
 }
 
-// The queries of prompts: a kernel of their own, with more warps on an SM than the one above has.
+// The queries of prompts: a kernel of their own, with more warps on an SM than the one above has.  (Blocks of 256 threads, three to an SM:
+// 46.5 us for 7,500 tokens of 24 heads of 256 with norms, against 44.4.)
+constexpr int kQThreads = 128;
 template <int D>
-__global__ void __launch_bounds__(256, 3) paged_rotate_queries_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kQThreads, 6) paged_rotate_queries_kernel(const AppendParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t unit = blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5);
   if (unit < p.q_units) rotate_queries<D, true>(p, unit);
 }
 
@@ -546,11 +548,11 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
     const long long pages = (long long)p.kv_blocks * 2 * g.n_layers, blocks = 2LL * device_sms() * (1024 / threads);
     long long heads = pages * g.h_kv / blocks;
     p.heads = (int)(heads < 1 ? 1 : heads > g.h_kv ? g.h_kv : heads);
-    const long long grid = pages * ((g.h_kv + p.heads - 1) / p.heads), q_grid = (q_warps + 7) / 8;
+    const long long grid = pages * ((g.h_kv + p.heads - 1) / p.heads), q_grid = (q_warps + kQThreads / 32 - 1) / (kQThreads / 32);
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     if (q_grid) {
-      e = g.head_dim == 128 ? launch_pdl(paged_rotate_queries_kernel<128>, (int)q_grid, 256, 0, stream, p)
-                            : launch_pdl(paged_rotate_queries_kernel<256>, (int)q_grid, 256, 0, stream, p);
+      e = g.head_dim == 128 ? launch_pdl(paged_rotate_queries_kernel<128>, (int)q_grid, kQThreads, 0, stream, p)
+                            : launch_pdl(paged_rotate_queries_kernel<256>, (int)q_grid, kQThreads, 0, stream, p);
       if (e != cudaSuccess) return e;
     }
     auto launch = [&](auto kernel) { e = launch_pdl(kernel, (int)grid, threads, 0, stream, p); };
