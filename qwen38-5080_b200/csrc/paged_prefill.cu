@@ -43,6 +43,9 @@ constexpr int kUnitBytes = 32768;
 constexpr float kBitsP = 4.f, kMostP = 61440.f;   // p is held times 2^4 in f16; what 64 keys may add up to before the reference moves
 constexpr int kPolyEvery = 4;              // of every 4 * kPolyEvery exponentials, two by polynomial
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
+// V is held relative to the largest scale of the block's keys, but to no less than this: kVUp / 2^-126, which zero values have, is not finite.
+// 2^-126 then stands as 2^-8, times 2^7 still exact in f16 for every byte; smaller scales keep what subnormal bf16 outputs can hold.
+constexpr float kLeastV = 0x1p-118f;
 
 struct PrefillTile {
   long long row0;                          // output row of (token 0, head 0)
@@ -578,7 +581,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     if (NS == 1) stage_queries(sQ, s_rowmul[0], 0, vw * 32 + 16, 16 / (256 / D));   // heads of 256: half of the query rows (all of them by four warps: 3 us more)
     // the largest V scale of the block's keys
     {
-      float r = 0.f;
+      float r = kLeastV;
       const int pg0 = j0 * kKeys / g.page_size, pg1 = (key_end - 1) / g.page_size;
       for (int i = pg0 + vt; i <= pg1; i += 128) {
         const int id = p.page_table[(long long)b * g.max_pages + i];
@@ -590,7 +593,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       asm volatile("bar.sync 2, 128;" ::: "memory");
       r_v = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     }
-    const float inv_r = r_v > 0.f ? kVUp / r_v : 0.f;
+    const float inv_r = kVUp / r_v;
     // A lane's 16 bytes: chunk k4 of 64-dim block blk of a row.  Eight lanes that go together take 4 chunks of rows q and q ^ 5 of
     // an 8-row group: with both layouts swizzled (16-byte chunk index xor row) neither their loads nor their stores share a bank.
     const int k4 = lane & 3, rb = (lane >> 2) & 1, blk = D == 128 ? (lane >> 3) & 1 : lane >> 3;
@@ -822,8 +825,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
       L = s_ml[0][1][row] * f0 + s_ml[1][1][row] * f1;
     }
-    const float unit = r_v * (1.f / kVUp);
-    const float scale = pieces > 1 ? unit : (L > 0.f ? unit / L : 0.f);
+    const float unit = r_v * (1.f / kVUp), inv = pieces > 1 ? 1.f : L > 0.f ? 1.f / L : 0.f;   // two factors: unit / L can be 0 where O * unit / L is not
     float* part = p.part + ((long long)(blockIdx.x / p.splits) * p.splits + piece) * (kRows * (D + 2));
     if (alive && !*gave_up) {
 #pragma unroll 1
@@ -847,7 +849,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             uint32_t w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const __nv_bfloat162 v2 = __floats2bfloat162_rn(o[16 * i + 2 * e] * scale, o[16 * i + 2 * e + 1] * scale);
+              const __nv_bfloat162 v2 = __floats2bfloat162_rn(o[16 * i + 2 * e] * inv * unit, o[16 * i + 2 * e + 1] * inv * unit);
               w[e] = *reinterpret_cast<const uint32_t*>(&v2);
             }
             stg256(dst + 16 * i, w);
@@ -855,7 +857,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         } else if (real) {
           float4* dst = reinterpret_cast<float4*>(part + (long long)row * D + 32 * c);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i] * scale, o[4 * i + 1] * scale, o[4 * i + 2] * scale, o[4 * i + 3] * scale);
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i] * unit, o[4 * i + 1] * unit, o[4 * i + 2] * unit, o[4 * i + 3] * unit);
         }
       }
       if (pieces > 1 && real && (!halves || grp == 0)) {

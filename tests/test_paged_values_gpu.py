@@ -1,0 +1,93 @@
+"""GPU tests of the paged operators on values at the edges of their types: all of them zero, far apart, loud, quiet, NaN.  Every
+attention kernel is reached (FORMS), and compared with the 64-bit form of paged_ref.py."""
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+# name: heads, query tokens of each sequence (None: decode), longest sequence that the host names
+FORMS = {
+    "one token, short": ((5, 1, 128), None, 1), "one token, short, heads of 256": ((7, 1, 256), None, 1),
+    "one token, long": ((5, 1, 128), None, None), "one token, long, heads of 256": ((7, 1, 256), None, None),
+    "few rows": ((5, 1, 128), 2, None), "few rows, heads of 256": ((7, 1, 256), 2, None),
+    "a tile": ((5, 1, 128), 20, None), "two tiles": ((64, 8, 128), 32, None), "tiles, heads of 256": ((7, 1, 256), 30, None),
+}
+PAGE = 16
+TWO_TILES = 640   # rows of a call, those of nobody among them, that make the tile kernel's thread blocks take two tiles each
+
+
+def _cache(g, form, lens):
+    """Random pools, scales and table for sequences of these lengths, in a table wide enough for the kernel that streams long caches."""
+    (_, h_kv, d), m, _ = FORMS[form]
+    need = sum(-(-n // PAGE) for n in lens)
+    spare = max(1100 * 128 // d, 133000 * 128 // (d * len(lens) * h_kv)) // PAGE + 2 if m is None else 1
+    kb, vb, ks, vs = ref.random_cache(g, 1, need + 1, h_kv, PAGE, d)
+    table = ref.random_table(g, lens, PAGE, max(-(-n // PAGE) for n in lens) + spare, need + 1)
+    return kb, vb, ks, vs, table
+
+
+def _queries(g, form, lens):
+    (h_q, _, d), m, _ = FORMS[form]
+    return torch.randn(1, len(lens) * (m or 1), h_q, d, generator=g).to(torch.bfloat16)
+
+
+def _attend(pkg, dev, form, cache, lens, q, causal=False):
+    """The call of a form; a list with every sequence's rows."""
+    (h_q, _, _), m, longest = FORMS[form]
+    up = [t.to(dev) for t in cache]
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    rows = q.shape[1]
+    if form == "two tiles":
+        q = torch.cat([q, torch.zeros(1, max(0, TWO_TILES - rows), *q.shape[2:], dtype=q.dtype)], 1)
+    shape = pkg.make_paged_shape(h_q, *cache[:3], cache[4])
+    ws = pkg.PagedWorkspace(shape, dev, max_seq_len=longest, q_tokens=m and q.shape[1])
+    if m is None:
+        out = pkg.paged_decode_attention(q.to(dev), *up, n, workspace=ws)
+    else:
+        starts = torch.arange(len(lens) + 1, dtype=torch.int32, device=dev) * m
+        out = pkg.paged_prefill_attention(q.to(dev), starts, *up, n, workspace=ws, causal=causal)
+    torch.cuda.synchronize()
+    assert ws.read_status() == 0
+    return list(out[0, :rows].cpu().split(m or 1))
+
+
+def _want(form, cache, b, length, q, causal=False):
+    kb, vb, ks, vs, table = cache
+    m = FORMS[form][1] or 1
+    return ref.attention(q[0, b * m:(b + 1) * m], kb[0], vb[0], ks[0], vs[0], table[b], length, causal=causal and FORMS[form][1] is not None)
+
+
+def _compare(form, cache, lens, q, got, causal=False, slack=0.0):
+    for b, n in enumerate(lens):
+        want, big = _want(form, cache, b, n, q, causal)
+        ref.assert_attention(got[b], want, big + slack * 2.0 ** 10, (form, b))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_values_that_are_all_zero(pkg, cuda_device, form):
+    """Zero values as the append stores them, with the smallest scale there is: zeros, not NaN."""
+    g = torch.Generator().manual_seed(1)
+    lens = [300, 40, 129]
+    cache = _cache(g, form, lens)
+    (_, h_kv, d), _, _ = FORMS[form]
+    up = [t.to(cuda_device) for t in cache]
+    k = torch.randn(1, sum(lens), h_kv, d, generator=g).to(torch.bfloat16).to(cuda_device)
+    starts = torch.tensor([0, 300, 340, 469], dtype=torch.int32, device=cuda_device)
+    pos, status = torch.zeros(3, dtype=torch.int32, device=cuda_device), torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    pkg.paged_rope_append(None, k, torch.zeros_like(k), None, None, *up, pos, q_start=starts, status=status)
+    assert status.item() == 0 and pos.tolist() == lens
+    for rows in _attend(pkg, cuda_device, form, [t.cpu() for t in up], lens, _queries(g, form, lens), causal=True):
+        assert (rows == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_values_that_are_zero_in_one_piece_of_the_keys(pkg, cuda_device, form):
+    """A long sequence, cut into pieces of 512 keys by the tile kernels: the values of the second 512 are zero."""
+    g = torch.Generator().manual_seed(2)
+    cache = _cache(g, form, [2000])
+    ids = cache[4][0, 512 // PAGE:1024 // PAGE].long()
+    cache[1][:, ids], cache[3][:, ids] = 0, 2.0 ** -126
+    q = _queries(g, form, [2000])
+    _compare(form, cache, [2000], q, _attend(pkg, cuda_device, form, cache, [2000], q))
