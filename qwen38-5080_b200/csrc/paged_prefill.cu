@@ -28,6 +28,8 @@
 //
 // Few rows on a long cache: the keys are cut into pieces over several thread blocks, which leave (m, l, O) in the
 // workspace, and a second kernel joins them in order.  Nobody waits for another thread block; waits inside one are bounded.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "tcgen05.cuh"
 
@@ -194,11 +196,19 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// x within [-126, 127]; NaN stays NaN.
+__device__ __forceinline__ float within_exponents(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-126.f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(127.f));
+  return r;
+}
 // 2^x of two values without the special-function unit: x = n + f, n the nearest integer (from the low bits of x + 1.5 2^23), 2^f by
 // the degree-3 polynomial of least relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 = 2^-13.7, against the f16 rounding of
-// up to 2^-11 that follows), n added to its exponent.
+// up to 2^-11 that follows), n added to its exponent.  Above 127 it gives about 2^127, and so does NaN (0x7FFFFFFF << 23 plus 0x7FFFFFFF
+// wraps to the largest float): both are far above what the caller accepts of a sum.
 __device__ __forceinline__ void ex2_pair(float& x, float& y) {
-  const unsigned long long v = pair2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const unsigned long long v = pair2(within_exponents(x), within_exponents(y));
   const unsigned long long t = add2(v, pair2(12582912.f, 12582912.f));
   const unsigned long long f = add2(v, fma2(t, pair2(-1.f, -1.f), pair2(12582912.f, 12582912.f)));
   unsigned long long q = fma2(f, pair2(0.0551716691f, 0.0551716691f), pair2(0.242611122f, 0.242611122f));
@@ -715,8 +725,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         uint32_t x[64], pk[32];
         float u;
-        // Exponentials against the reference as it stands; their sum tells whether f16 can hold them.
-        auto exponentials = [&]() {
+        // Exponentials against the reference as it stands; their sum tells whether f16 can hold them.  all_exact: none by polynomial, which
+        // would make a hidden score 2^-126 and a NaN a large number.
+        auto exponentials = [&](auto all_exact) {
           const float mb = kBitsP - (m == -INFINITY ? 0.f : m);
           const unsigned long long mb2 = pair2(mb, mb);
           unsigned long long sum0 = 0ull, sum1 = 0ull;
@@ -727,7 +738,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             split2(fma2(pair2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, mb2), x0, x1);
             split2(fma2(pair2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), f2, mb2), x2, x3);
             x0 = ex2(x0); x1 = ex2(x1);
-            if ((e / 4) % kPolyEvery == kPolyEvery - 1) {     // a share of them on the FMA pipe
+            if (!decltype(all_exact)::value && (e / 4) % kPolyEvery == kPolyEvery - 1) {   // a share of them on the FMA pipe
               ex2_pair(x2, x3);
             } else {
               x2 = ex2(x2); x3 = ex2(x3);
@@ -745,11 +756,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         bool fits = open && !bad && !__any_sync(0xffffffffu, m == -INFINITY);
         if (fits) {
           tmem_ld64(ss, x);
-          exponentials();
-          fits = !__any_sync(0xffffffffu, u > kMostP);
+          exponentials(std::false_type());
+          fits = __all_sync(0xffffffffu, u <= kMostP);       // (false for NaN)
         }
         if (!fits) {
-          // Hidden keys, no reference yet, or exponentials too large: the scores again, hidden ones out, the reference to their
+          // Hidden keys, no reference yet, or exponentials too large or NaN: the scores again, hidden ones out, the reference to their
           // maximum if that is larger, and what O and the sum hold so far rescaled to it.
           tmem_ld64(ss, x);
           float tmax = -INFINITY;
@@ -787,7 +798,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
               tmem_st16_nowait(to + 16 * c, o);
             }
           }
-          exponentials();
+          exponentials(std::true_type());
         }
         l += u;
         // into the columns that the scores leave

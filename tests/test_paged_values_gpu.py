@@ -91,3 +91,75 @@ def test_values_that_are_zero_in_one_piece_of_the_keys(pkg, cuda_device, form):
     cache[1][:, ids], cache[3][:, ids] = 0, 2.0 ** -126
     q = _queries(g, form, [2000])
     _compare(form, cache, [2000], q, _attend(pkg, cuda_device, form, cache, [2000], q))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_that_see_nothing_beside_loud_values(pkg, cuda_device, form):
+    """Fewer cached tokens than queries: the first rows of a tile see nothing, the others values of 10^8."""
+    g = torch.Generator().manual_seed(3)
+    m = FORMS[form][1] or 1
+    lens = [max(1, m - 7 + b) for b in range(8)]
+    cache = _cache(g, form, lens)
+    cache[3].mul_(2.0 ** 33)
+    q = _queries(g, form, lens)
+    got = _attend(pkg, cuda_device, form, cache, lens, q, causal=True)
+    _compare(form, cache, lens, q, got, causal=True)
+    for rows, n in zip(got, lens):
+        assert (rows[:max(0, m - n)] == 0).all()
+
+
+def _far_key(cache, b, index, jump, d):
+    """Key `index` of sequence b gets a score of about `jump` with queries near 1; the rest of its page scores 0."""
+    kb, _, ks, _, table = cache
+    page, row = int(table[b, index // PAGE]), index % PAGE
+    kb[0, page], ks[0, page] = 0, 0.125
+    byte = torch.tensor(jump / d ** 0.5 / 0.125).to(torch.float8_e4m3fn).view(torch.uint8)
+    kb[0, page, :, row] = byte
+
+
+@pytest.mark.parametrize("jump", [60.0, 100.0, 200.0, 400.0])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_key_far_above_the_rest(pkg, cuda_device, form, jump):
+    """One key of the second 128 scores far above all others: at each of 16 neighbouring places, a sequence each."""
+    g = torch.Generator().manual_seed(4)
+    lens = [300 + b for b in range(16)]
+    cache = _cache(g, form, lens)
+    for b in range(16):
+        _far_key(cache, b, 192 + b, jump, FORMS[form][0][2])
+    q = (1 + 0.1 * _queries(g, form, lens).float()).to(torch.bfloat16)
+    _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_that_grow_along_the_sequence(pkg, cuda_device, form):
+    """Keys that get louder with every page: the running reference of every row moves many times."""
+    g = torch.Generator().manual_seed(5)
+    lens = [900, 333]
+    cache = _cache(g, form, lens)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // PAGE)):
+            cache[2][:, cache[4][b, i]] = 2.0 ** (-9 + 8 * i * PAGE // 900)
+    q = _queries(g, form, lens)
+    for causal in (False, True):
+        _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q, causal), causal)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_a_key_that_is_nan(pkg, cuda_device, form):
+    """A NaN in a key that is seen makes the row NaN, wherever it stands; one that is hidden does nothing."""
+    g = torch.Generator().manual_seed(6)
+    lens = [300] * 16
+    cache = _cache(g, form, lens)
+    for b in range(16):
+        cache[0][0, cache[4][b, 12], :, b, 5] = 0x7F
+    for rows in _attend(pkg, cuda_device, form, cache, lens, _queries(g, form, lens)):
+        assert torch.isnan(rows).all()
+    if FORMS[form][1] is None:
+        return
+    cache, m = _cache(g, form, lens), FORMS[form][1]
+    q = _queries(g, form, lens)
+    clean = _attend(pkg, cuda_device, form, cache, lens, q, causal=True)
+    for b in range(16):
+        cache[0][0, cache[4][b, 299 // PAGE], :, 299 % PAGE, b] = 0xFF
+    for rows, before in zip(_attend(pkg, cuda_device, form, cache, lens, q, causal=True), clean):
+        assert torch.equal(rows[:m - 1], before[:m - 1]) and torch.isnan(rows[m - 1]).all()
