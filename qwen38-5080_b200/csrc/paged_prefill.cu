@@ -830,11 +830,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     for (int i = 1; i < 4; ++i) r_v = fmaxf(r_v, s_red[i]); // written before the first V unit was
     float f0 = 1.f, f1 = 0.f, M = m, L = l;
     if (halves) {
-      const float m0 = s_ml[0][0][row], m1 = s_ml[1][0][row];
+      const float m0 = s_ml[0][0][row], m1 = s_ml[1][0][row], l0 = s_ml[0][1][row], l1 = s_ml[1][1][row];
       M = fmaxf(m0, m1);
-      f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M);
-      f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-      L = s_ml[0][1][row] * f0 + s_ml[1][1][row] * f1;
+      f0 = m0 == -INFINITY ? l0 : ex2(m0 - M);              // no reference: the sum is 0 (no key seen) or NaN (a NaN query), and so is the weight
+      f1 = m1 == -INFINITY ? l1 : ex2(m1 - M);
+      L = l0 * f0 + l1 * f1;
     }
     const float unit = r_v * (1.f / kVUp), inv = pieces > 1 ? 1.f : L > 0.f ? 1.f / L : 0.f;   // two factors: unit / L can be 0 where O * unit / L is not
     float* part = p.part + ((long long)(blockIdx.x / p.splits) * p.splits + piece) * (kRows * (D + 2));

@@ -163,3 +163,22 @@ def test_a_key_that_is_nan(pkg, cuda_device, form):
         cache[0][0, cache[4][b, 299 // PAGE], :, 299 % PAGE, b] = 0xFF
     for rows, before in zip(_attend(pkg, cuda_device, form, cache, lens, q, causal=True), clean):
         assert torch.equal(rows[:m - 1], before[:m - 1]) and torch.isnan(rows[m - 1]).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("lens", [[300, 40], [2000, 1]])
+def test_a_query_that_is_nan(pkg, cuda_device, form, lens):
+    """A row whose query has a NaN is NaN; its neighbours are what they are without it."""
+    g = torch.Generator().manual_seed(7)
+    cache = _cache(g, form, lens)
+    q = _queries(g, form, lens)
+    row = min(3, (FORMS[form][1] or 1) - 1)
+    q[0, row, 2, 17] = float("nan")
+    got = _attend(pkg, cuda_device, form, cache, lens, q)
+    assert torch.isnan(got[0][row, 2]).all()
+    got[0][row, 2], q[0, row, 2] = 0, 0
+    want, big = _want(form, cache, 0, lens[0], q)
+    want[row, 2] = 0
+    ref.assert_attention(got[0], want, big, form)
+    want, big = _want(form, cache, 1, lens[1], q)
+    ref.assert_attention(got[1], want, big, form)
