@@ -60,6 +60,10 @@ inline int* paged_counters(void* ws) { return (int*)ws; }
 inline unsigned long long* paged_words(void* ws) { return (unsigned long long*)((uint8_t*)ws + paged_words_offset()); }
 inline float* paged_partials(void* ws) { return (float*)((uint8_t*)ws + paged_partials_offset()); }
 
+// The least scale that V is held relative to where that is the largest of the keys so far: its reciprocal is finite, that of a
+// subnormal scale may not be.
+constexpr float kLeastScale = 0x1p-126f;
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

@@ -249,8 +249,9 @@ paged_decode_kernel(const DecodeParams p) {
         l0 = l0 * a0 + (p0 + p2);
         l1 = l1 * a1 + (p1 + p3);
         if (sc.y > r) {                   // a page with a larger V scale (the same for the whole warp)
-          a0 *= r / sc.y; a1 *= r / sc.y;
-          r = sc.y;
+          const float louder = fmaxf(sc.y, kLeastScale);
+          a0 *= r / louder; a1 *= r / louder;
+          r = louder;
           inv_r = 1.f / r;
         }
         if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
@@ -671,8 +672,9 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           l0 = l0 * a0 + (p0 + p2);
           l1 = l1 * a1 + (p1 + p3);
           if (sc.y > r) {                 // a page with a larger V scale (the same for the whole warp)
-            a0 *= r / sc.y; a1 *= r / sc.y;
-            r = sc.y;
+            const float louder = fmaxf(sc.y, kLeastScale);
+            a0 *= r / louder; a1 *= r / louder;
+            r = louder;
             inv_r = 1.f / r;
           }
           if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {

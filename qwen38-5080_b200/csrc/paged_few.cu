@@ -252,8 +252,9 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         }
       float grow = 1.f;
       if (c.y > r) {                      // a page with a larger V scale (the same for the whole warp)
-        grow = r / c.y;
-        r = c.y;
+        const float louder = fmaxf(c.y, kLeastScale);
+        grow = r / louder;
+        r = louder;
         inv_r = 1.f / r;
       }
       const float vs = c.y * inv_r;

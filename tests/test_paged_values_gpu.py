@@ -182,3 +182,27 @@ def test_a_query_that_is_nan(pkg, cuda_device, form, lens):
     ref.assert_attention(got[0], want, big, form)
     want, big = _want(form, cache, 1, lens[1], q)
     ref.assert_attention(got[1], want, big, form)
+
+
+@pytest.mark.parametrize("exponent", [-149, -140, -127, -126, -118, -110])
+@pytest.mark.parametrize("form", FORMS)
+def test_quiet_values(pkg, cuda_device, form, exponent):
+    """V scales down to the smallest positive number.  Results may be subnormal bf16: half a step of those is 2^-134."""
+    g = torch.Generator().manual_seed(8)
+    lens = [300, 40]
+    cache = _cache(g, form, lens)
+    cache[3].fill_(2.0 ** exponent)
+    q = _queries(g, form, lens)
+    _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q), slack=2.0 ** -134)
+
+
+@pytest.mark.parametrize("exponent", [-149, -127])
+@pytest.mark.parametrize("form", FORMS)
+def test_quiet_keys(pkg, cuda_device, form, exponent):
+    """K scales down to the smallest positive number: every visible key weighs the same."""
+    g = torch.Generator().manual_seed(10)
+    lens = [300, 40]
+    cache = _cache(g, form, lens)
+    cache[2].fill_(2.0 ** exponent)
+    q = _queries(g, form, lens)
+    _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q))
