@@ -40,6 +40,7 @@ constexpr int kMostPieces = 16;           // of a sequence
 constexpr int kWhole = 256;               // sequences up to this many tokens are not cut into pieces
 constexpr int kStage = 256;               // pages whose number and scales are in shared memory at a time
 constexpr float kPBits = 15.f;            // p is held times 2^15
+constexpr float kPUnit = 0x1p-15f;        // and sums leave the warp without that factor: times a loud V scale they could pass the largest float
 
 struct DecodeParams {
   PagedGeometry g;
@@ -301,8 +302,9 @@ paged_decode_kernel(const DecodeParams p) {
   }
   if (gq == 0) {
     s_ml[warp][0][2 * tq] = m0; s_ml[warp][0][2 * tq + 1] = m1;
-    s_ml[warp][1][2 * tq] = l0; s_ml[warp][1][2 * tq + 1] = l1;
+    s_ml[warp][1][2 * tq] = l0 * kPUnit; s_ml[warp][1][2 * tq + 1] = l1 * kPUnit;
   }
+  auto sum_of = [&](float x) { return x * kPUnit * r; };
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh) {
     if (2 * tq + hh < G) {
@@ -311,8 +313,8 @@ paged_decode_kernel(const DecodeParams p) {
       for (int hf = 0; hf < DH; ++hf)
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-          *reinterpret_cast<float4*>(dst + hf * 128 + 4 * w) = make_float4(o[hf * 8 + 2 * w][hh] * r, o[hf * 8 + 2 * w][2 + hh] * r,
-                                                                          o[hf * 8 + 2 * w + 1][hh] * r, o[hf * 8 + 2 * w + 1][2 + hh] * r);
+          *reinterpret_cast<float4*>(dst + hf * 128 + 4 * w) = make_float4(sum_of(o[hf * 8 + 2 * w][hh]), sum_of(o[hf * 8 + 2 * w][2 + hh]),
+                                                                          sum_of(o[hf * 8 + 2 * w + 1][hh]), sum_of(o[hf * 8 + 2 * w + 1][2 + hh]));
     }
   }
   __syncthreads();
@@ -725,15 +727,16 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         float* ml = sML + (db * kConsumerWarps + warp) * 16;
         if (gq == 0) {
           ml[2 * tq] = m0; ml[2 * tq + 1] = m1;
-          ml[8 + 2 * tq] = l0; ml[8 + 2 * tq + 1] = l1;
+          ml[8 + 2 * tq] = l0 * kPUnit; ml[8 + 2 * tq + 1] = l1 * kPUnit;
         }
         const uint32_t dbase = smem_u32(sDump + (db * kConsumerWarps + warp) * dump_warp_floats);
+        auto sum_of = [&](float x) { return x * kPUnit * r; };
 #pragma unroll
         for (int j = 0; j < KSTEPS; ++j) {   // regs 0, 1: dim (j >> 3) * 128 + 16 gq + 2 (j & 7) of heads 2 tq, 2 tq + 1; regs 2, 3: that dim + 1
           const int u = (j >> 3) * 64 + 8 * gq + (j & 7);
           const uint32_t pos8 = 8u * (uint32_t)((u & ~7) | ((j & 7) ^ gq));
-          if (2 * tq < G) sts64(dbase + 2 * tq * DP * 4 + pos8, o[j][0] * r, o[j][2] * r);
-          if (2 * tq + 1 < G) sts64(dbase + (2 * tq + 1) * DP * 4 + pos8, o[j][1] * r, o[j][3] * r);
+          if (2 * tq < G) sts64(dbase + 2 * tq * DP * 4 + pos8, sum_of(o[j][0]), sum_of(o[j][2]));
+          if (2 * tq + 1 < G) sts64(dbase + (2 * tq + 1) * DP * 4 + pos8, sum_of(o[j][1]), sum_of(o[j][3]));
         }
       }
       __syncwarp();

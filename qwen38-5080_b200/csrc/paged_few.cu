@@ -23,6 +23,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kRowsU = 16;                // tokens of a unit
 constexpr float kPBits = 15.f;            // p is held times 2^15
+constexpr float kPUnit = 0x1p-15f;        // and sums leave the warp without that factor: times a loud V scale they could pass the largest float
 constexpr int kTilesN = 2, kFewRows = 8 * kTilesN;   // column tiles, query rows of a tile
 constexpr int kMostPieces = 16;           // of the keys
 constexpr int kLeastUnits = 16;           // units of a piece, at least (8: 8 sequences of 256 keys 9.5 us for 8.0; 32: 1024 keys 14 us for 11)
@@ -337,6 +338,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   __syncthreads();                        // every ring is empty: the states go there
 
   float* s_acc = reinterpret_cast<float*>(ring_ptr);   // [warp][column][D]
+  auto sum_of = [&](float x) { return x * kPUnit * r; };
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -344,14 +346,15 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l[t][hh] += __shfl_xor_sync(0xffffffffu, l[t][hh], off);
       const int col = 8 * t + 2 * tq + hh;
-      if (gq == 0) { s_ml[warp][0][col] = m[t][hh]; s_ml[warp][1][col] = l[t][hh]; }
+      if (gq == 0) { s_ml[warp][0][col] = m[t][hh]; s_ml[warp][1][col] = l[t][hh] * kPUnit; }
       float* dst = s_acc + (warp * COLS + col) * D + 16 * gq;
 #pragma unroll
       for (int hf = 0; hf < DH; ++hf)
 #pragma unroll
         for (int w = 0; w < 4; ++w)
           *reinterpret_cast<float4*>(dst + hf * 128 + 4 * (w ^ (gq >> 1 & 3))) =
-              make_float4(o[t][hf * 8 + 2 * w][hh] * r, o[t][hf * 8 + 2 * w][2 + hh] * r, o[t][hf * 8 + 2 * w + 1][hh] * r, o[t][hf * 8 + 2 * w + 1][2 + hh] * r);
+              make_float4(sum_of(o[t][hf * 8 + 2 * w][hh]), sum_of(o[t][hf * 8 + 2 * w][2 + hh]),
+                          sum_of(o[t][hf * 8 + 2 * w + 1][hh]), sum_of(o[t][hf * 8 + 2 * w + 1][2 + hh]));
     }
   }
   __syncthreads();

@@ -43,6 +43,7 @@ constexpr int kInfo = 8;                   // tiles whose scales are in flight
 constexpr int kVRing = 2;                  // V units of 32 KB in f16
 constexpr int kUnitBytes = 32768;
 constexpr float kBitsP = 4.f, kMostP = 61440.f;   // p is held times 2^4 in f16; what 64 keys may add up to before the reference moves
+constexpr float kPUnit = 1.f / 16.f;       // pieces are left without that factor: times a loud V scale it could pass the largest float
 constexpr int kPolyEvery = 4;              // of every 4 * kPolyEvery exponentials, two by polynomial
 constexpr float kVUp = 128.f;              // V is held times 2^7 (448 * 2^7 < 65504)
 // V is held relative to the largest scale of the block's keys, but to no less than this: kVUp / 2^-126, which zero values have, is not finite.
@@ -868,12 +869,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         } else if (real) {
           float4* dst = reinterpret_cast<float4*>(part + (long long)row * D + 32 * c);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i] * unit, o[4 * i + 1] * unit, o[4 * i + 2] * unit, o[4 * i + 3] * unit);
+          for (int i = 0; i < 8; ++i) {
+            float4 sums;
+            sums.x = o[4 * i] * kPUnit * unit; sums.y = o[4 * i + 1] * kPUnit * unit; sums.z = o[4 * i + 2] * kPUnit * unit; sums.w = o[4 * i + 3] * kPUnit * unit;
+            dst[i] = sums;
+          }
         }
       }
       if (pieces > 1 && real && (!halves || grp == 0)) {
         part[kRows * D + row] = M;
-        part[kRows * D + kRows + row] = L;
+        part[kRows * D + kRows + row] = L * kPUnit;
       }
     }
     tc_fence_before();

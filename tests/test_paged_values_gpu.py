@@ -196,6 +196,17 @@ def test_quiet_values(pkg, cuda_device, form, exponent):
     _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q), slack=2.0 ** -134)
 
 
+@pytest.mark.parametrize("lens", [[300, 40], [2000, 1]])
+@pytest.mark.parametrize("form", FORMS)
+def test_loud_values(pkg, cuda_device, form, lens):
+    """Values up to 2^119, near the largest bf16: the weighted sums stay within fp32."""
+    g = torch.Generator().manual_seed(9)
+    cache = _cache(g, form, lens)
+    cache[3].fill_(2.0 ** 112)
+    q = _queries(g, form, lens)
+    _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q))
+
+
 @pytest.mark.parametrize("exponent", [-149, -127])
 @pytest.mark.parametrize("form", FORMS)
 def test_quiet_keys(pkg, cuda_device, form, exponent):
