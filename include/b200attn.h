@@ -469,12 +469,15 @@ typedef struct B200AttnRope {
  *   q_norm_weight, k_norm_weight : bf16 [n_layers][head_dim] or NULL: x * rsqrt(mean(x^2) + eps) * (1 + w) before the rotation
  *   rope     : NULL = no rotation
  *   seq_pos  : i32 [batch], tokens cached before the call; the new ones go to slots seq_pos[b], seq_pos[b] + 1, ...
- *   advance_pos : 1 -> seq_pos[b] += the new tokens (if they all fit), after everything is written
+ *   advance_pos : 1 -> seq_pos[b] += the new tokens, after everything is written.  A sequence with a token beyond its capacity or
+ *              on a page that does not exist stays where it was
  * All arithmetic is fp32 with one rounding at the end, to bf16 for q_out, to e4m3 for the cache.  The scale of a (page, kv
  * head) is the smallest power of two that brings the largest finite |value| of the page's new tokens to at most 448; where
  * the page already held tokens it only ever grows, and the earlier rows are then re-expressed in it (a power of two: exact
  * but for values that become subnormal).  Infinities saturate, NaN becomes the NaN byte.  A scale is never below 2^-126.
  * Tokens beyond a sequence's capacity are skipped (B200ATTN_STATUS_POS_AT_CAPACITY).
+ * Without q_start, a sequence at position 0 whose first table entry is -1 is idle: its token is dropped, it does not advance and
+ * nothing is reported.  (Its length stays 0, so that the attention gives zeros.)
  */
 int b200attn_paged_rope_append(const B200AttnPagedShape* shape, const B200AttnRope* rope, int n_tokens, const int* q_start,
                                const void* q_bf16, const void* k_bf16, const void* v_bf16,

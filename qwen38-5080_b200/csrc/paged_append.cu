@@ -290,7 +290,9 @@ paged_append_token_kernel(const AppendParams p) {
   const int pos = ld(p.seq_pos + b);
   const bool fits = pos >= 0 && pos < (long long)g.max_pages * g.page_size;
   const int page = fits ? page_of(p, b, pos / g.page_size) : -1, fill = fits ? pos % g.page_size : 0;
-  if (page < 0 && lr == 0) atomicOr(p.status, fits ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);
+  // a sequence without a token and without a page (-1) is idle: nothing to store, nothing to report
+  if (page < 0 && lr == 0 && (pos != 0 || ld(p.page_table + (long long)b * g.max_pages) != -1))
+    atomicOr(p.status, fits ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);
   float* sp = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv + h;
   const float old = page >= 0 && fill > 0 ? *sp : 0.f;
   float x[8];
@@ -494,12 +496,20 @@ __global__ void __launch_bounds__(kQThreads, 6) paged_rotate_queries_kernel(cons
   if (unit < p.q_units) rotate_queries<D, true>(p, unit);
 }
 
-__global__ void paged_advance_kernel(PagedGeometry g, const int* q_start, int* seq_pos) {
+// A warp per sequence: its position moves on if every new token has found a page.
+__global__ void paged_advance_kernel(PagedGeometry g, int n_tokens, const int* q_start, const int* page_table, int* seq_pos) {
   pdl_wait();
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  const int b = (int)(blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (b >= g.batch) return;
-  const int n = q_start ? q_start[b + 1] - q_start[b] : 1, p = seq_pos[b];
-  if (p >= 0 && n >= 0 && (long long)p + n <= (long long)g.max_pages * g.page_size) seq_pos[b] = p + n;
+  const int q0 = q_start ? q_start[b] : b, end = q_start ? q_start[b + 1] : b + 1, pos = seq_pos[b];
+  if (q0 < 0 || end <= q0 || end > n_tokens || pos < 0 || (long long)pos + (end - q0) > (long long)g.max_pages * g.page_size) return;
+  const int last = (pos + (end - q0) - 1) / g.page_size;
+  bool there = true;
+  for (int i = pos / g.page_size + lane; i <= last; i += 32) {
+    const int id = page_table[(long long)b * g.max_pages + i];
+    there &= id >= 0 && id < g.n_pages;
+  }
+  if (__all_sync(0xffffffffu, there) && lane == 0) seq_pos[b] = pos + (end - q0);
 }
 
 }  // namespace
@@ -572,7 +582,8 @@ cudaError_t launch_paged_append(const PagedGeometry& g, const PagedAppendArgs& a
       }
     }
   }
-  if (e == cudaSuccess && a.advance_pos) e = launch_pdl(paged_advance_kernel, (g.batch + 127) / 128, 128, 0, stream, g, a.q_start, a.seq_pos);
+  if (e == cudaSuccess && a.advance_pos)
+    e = launch_pdl(paged_advance_kernel, (g.batch + 3) / 4, 128, 0, stream, g, a.n_tokens, a.q_start, a.page_table, a.seq_pos);
   return e;
 }
 

@@ -93,8 +93,9 @@ def paged_rope_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, pag
     Without `q_start`: one token per sequence.  `cos`, `sin`: fp32 tables [n_positions, rotary_dim / 2] (None: no rotation);
     a token's row is its slot in the sequence, or `positions` int32 [n_tokens] or [n_axes, n_tokens] with `pair_axis` int32
     [rotary_dim / 2] saying which axis turns which pair.  Norm weights bf16 [n_layers, head_dim]: RMS norm with weight 1 + w
-    before the rotation.  `seq_pos`: tokens cached before the call, advanced afterwards if `advance`.  Capacity, bad pages
-    and bad positions are reported in `status`."""
+    before the rotation.  `seq_pos`: tokens cached before the call, advanced afterwards if `advance` (a sequence whose tokens did not
+    all find a page stays).  Capacity, bad pages and bad positions are reported in `status`.  Without `q_start`, a sequence at
+    position 0 whose first page is -1 is idle: nothing is stored, advanced or reported."""
     if q is not None and q_out is None:
         q_out = torch.empty_like(q)
     rc = _call(k_pages, _lib.paged_binding().append, q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, seq_pos, q_start,
@@ -141,7 +142,8 @@ class PagedFP8Cache:
     """A pool of pages for `slots` sequences, all layers: storage, page table, positions, and which pages are free.
 
     Pages are handed out on the host, ahead of the steps that need them (`reserve`); a decode step reads table and
-    positions on the device and can be captured into a CUDA graph and replayed as long as pages are reserved."""
+    positions on the device and can be captured into a CUDA graph and replayed as long as pages are reserved.
+    A slot without pages is idle: steps, captured ones too, store nothing for it, leave its position at 0 and give zeros."""
 
     def __init__(self, n_layers: int, slots: int, h_q: int, h_kv: int, head_dim: int, n_pages: int, max_pages: int,
                  page_size: int = 64, device="cuda", max_prompt_tokens: int = 0):
@@ -221,17 +223,18 @@ class PagedFP8Cache:
                                        self.seq_pos, workspace=self.prompt_workspace, causal=causal, out=out)
 
     def step(self, q, k, v, cos, sin, *, out=None, count: bool = True, **rope) -> torch.Tensor:
-        """One decode step of all slots: rotate, append, attend, advance (graph capturable; `reserve` first)."""
+        """One decode step of all slots that have pages: rotate, append, attend, advance (graph capturable; `reserve` first).  q, k
+        and v hold a row for every slot; an idle slot's result is zero."""
         if count:
             for b in range(self.slots):
-                if self.host_len[b] + 1 > len(self.pages[b]) * self.page_size:
+                if self.pages[b] and self.host_len[b] + 1 > len(self.pages[b]) * self.page_size:
                     raise ValueError(f"slot {b}: no page reserved for token {self.host_len[b]}")
         qr = paged_rope_append(q, k, v, cos, sin, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
                                self.seq_pos, advance=True, status=self.status, **rope)
         out = paged_decode_attention(qr, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table, self.seq_pos,
                                      workspace=self.workspace, out=out)
         if count:
-            self.host_len = [x + 1 for x in self.host_len]
+            self.host_len = [x + 1 if p else x for x, p in zip(self.host_len, self.pages)]
         return out
 
 
