@@ -143,6 +143,7 @@ class PagedFP8Cache:
 
     Pages are handed out on the host, ahead of the steps that need them (`reserve`); a decode step reads table and
     positions on the device and can be captured into a CUDA graph and replayed as long as pages are reserved.
+    The host counts every sequence's tokens: `prefill` and `step` do, and `replayed` says how often a captured step is to run.
     A slot without pages is idle: steps, captured ones too, store nothing for it, leave its position at 0 and give zeros."""
 
     def __init__(self, n_layers: int, slots: int, h_q: int, h_kv: int, head_dim: int, n_pages: int, max_pages: int,
@@ -222,20 +223,33 @@ class PagedFP8Cache:
         return paged_prefill_attention(qr, q_start, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
                                        self.seq_pos, workspace=self.prompt_workspace, causal=causal, out=out)
 
+    def _room(self, n: int) -> None:
+        for b in range(self.slots):
+            if self.pages[b] and self.host_len[b] + n > len(self.pages[b]) * self.page_size:
+                raise ValueError(f"slot {b}: {len(self.pages[b])} pages reserved for {self.host_len[b]} cached + {n}")
+
+    def _count(self, n: int) -> None:
+        self.host_len = [x + n if p else x for x, p in zip(self.host_len, self.pages)]
+
+    def replayed(self, n: int = 1) -> None:
+        """Count `n` replays of a captured step, before they run; refuses, and counts nothing, if the pages reserved for a sequence
+        do not hold them."""
+        self._room(n)
+        self._count(n)
+
     def step(self, q, k, v, cos, sin, *, out=None, count: bool = True, **rope) -> torch.Tensor:
         """One decode step of all slots that have pages: rotate, append, attend, advance (graph capturable; `reserve` first).  q, k
-        and v hold a row for every slot; an idle slot's result is zero."""
+        and v hold a row for every slot; an idle slot's result is zero.  A step under capture does not run and is not counted
+        (`replayed`); count=False: the caller counts this one too."""
+        count = count and not torch.cuda.is_current_stream_capturing()
         if count:
-            for b in range(self.slots):
-                if self.pages[b] and self.host_len[b] + 1 > len(self.pages[b]) * self.page_size:
-                    raise ValueError(f"slot {b}: no page reserved for token {self.host_len[b]}")
+            self._room(1)
         qr = paged_rope_append(q, k, v, cos, sin, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
                                self.seq_pos, advance=True, status=self.status, **rope)
-        out = paged_decode_attention(qr, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table, self.seq_pos,
-                                     workspace=self.workspace, out=out)
         if count:
-            self.host_len = [x + 1 if p else x for x, p in zip(self.host_len, self.pages)]
-        return out
+            self._count(1)
+        return paged_decode_attention(qr, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table, self.seq_pos,
+                                      workspace=self.workspace, out=out)
 
 
 __all__ = ["PagedFP8Cache", "PagedWorkspace", "make_paged_shape", "paged_decode_attention", "paged_prefill_attention",

@@ -92,3 +92,57 @@ def test_steps_with_a_released_slot_and_its_next_sequence(pkg, cuda_device, capt
     assert c.host_len == want
     prompt([0, 60, 3])                                     # another sequence in the released slot
     assert c.seq_pos.tolist() == [60, 60, 103] and c.read_status() == 0
+
+
+@pytest.mark.gpu
+def test_pages_reserved_between_replays(pkg, cuda_device):
+    """Capture counts nothing; replays are counted by `replayed`, so that `reserve` hands out the pages that the next ones need."""
+    dev, layers, slots, h_q, h_kv, d, page = cuda_device, 1, 2, 5, 1, 128, 16
+    c = pkg.PagedFP8Cache(layers, slots, h_q, h_kv, d, n_pages=20, max_pages=10, page_size=page, device=dev, max_prompt_tokens=64)
+    g = torch.Generator().manual_seed(1)
+    c.prefill(*(_mk(g, layers, 40, h, d).to(dev) for h in (h_q, h_kv, h_kv)), None, None, [30, 10])
+    c.reserve(0, 2)
+    c.reserve(1, 6)
+    buf = [_mk(g, layers, slots, h, d).to(dev) for h in (h_q, h_kv, h_kv)]
+    out, graph = torch.empty_like(buf[0]), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.step(*buf, None, None, out=out)
+    assert c.host_len == [30, 10] and [len(p) for p in c.pages] == [2, 1]
+    want, q = [30, 10], None
+    for turn in range(40):
+        if turn in (2, 10, 25):                            # slot 0 is full after 2 more tokens
+            with pytest.raises(ValueError, match="slot"):
+                c.replayed(17)
+            for b in range(slots):
+                c.reserve(b, 17)
+        c.replayed()
+        q = _mk(g, layers, slots, h_q, d)
+        for t, x in zip(buf, (q, _mk(g, layers, slots, h_kv, d), _mk(g, layers, slots, h_kv, d))):
+            t.copy_(x)
+        graph.replay()
+        want = [x + 1 for x in want]
+        assert c.seq_pos.tolist() == want == c.host_len and c.read_status() == 0
+    _check(c, q, out, want, [(0, 1), (1, 2)])
+
+
+def test_replays_are_counted_against_the_reserved_pages(pkg):
+    c = object.__new__(pkg.PagedFP8Cache)                  # the host side, over CPU tensors
+    c.slots, c.n_pages, c.max_pages, c.page_size, c.device = 3, 10, 6, 16, torch.device("cpu")
+    c.page_table, c.seq_pos = torch.full((3, 6), -1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    c.host_len, c.pages, c.free = [0] * 3, [[] for _ in range(3)], list(range(9, -1, -1))
+    c.reserve(0, 20)
+    c.host_len[0] = 20
+    c.reserve(2, 5)
+    c.replayed(12)                                         # 32 tokens of 32; slot 1 is idle, slot 2 holds 12 of 16
+    assert c.host_len == [32, 0, 12]
+    with pytest.raises(ValueError, match="slot 0"):
+        c.replayed()
+    assert c.host_len == [32, 0, 12]
+    c.reserve(0, 1)
+    c.replayed(4)
+    assert c.host_len == [36, 0, 16] and len(c.pages[0]) == 3
+    with pytest.raises(ValueError, match="slot 2"):
+        c.replayed()
+    c.release(2)
+    c.replayed()
+    assert c.host_len == [37, 0, 0]
