@@ -46,7 +46,10 @@ extern "C" {
 #define B200ATTN_STATUS_WAIT_TIMEOUT     4  /* a bounded wait on a copy barrier ran out */
 #define B200ATTN_STATUS_LEN_NEGATIVE     8  /* seq_len[b] < 0: treated as 0 */
 #define B200ATTN_STATUS_BAD_PAGE        32  /* paged cache: a page number the call needs is not in [0, n_pages): its tokens are skipped */
-#define B200ATTN_STATUS_BAD_POSITION    64  /* rotary: a position or axis outside the tables: clamped to them */
+#define B200ATTN_STATUS_BAD_POSITION    64  /* rotary: a position or axis outside the tables: clamped to them; packed append: new tokens
+                                                for a sequence with seq_pos[b] < 0: skipped */
+#define B200ATTN_STATUS_BAD_RANGE      128  /* packed calls: q_start[b], q_start[b + 1] decrease or leave [0, n_tokens]: the sequence
+                                                is skipped */
 #define B200ATTN_STATUS_BOUNDS          16  /* index-checking build only (-DB200ATTN_BOUNDS=1): a kernel computed an index
                                                outside its buffer (reported, never trapped) */
 

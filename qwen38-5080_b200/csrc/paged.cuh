@@ -98,6 +98,13 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
 template <class T>
 __device__ __forceinline__ T ld(const T* p) { return *p; }
 
+// Whether sequence b of a packed call may own tokens [q0, end).
+__device__ __forceinline__ bool range_fits(int q0, int end, int n_tokens, int* status, bool report) {
+  const bool fits = q0 >= 0 && end >= q0 && end <= n_tokens;
+  if (!fits && report) atomicOr(status, B200ATTN_STATUS_BAD_RANGE);
+  return fits;
+}
+
 // Valid length of a sequence: negative lengths count as 0, lengths beyond the table's capacity are clamped to it.
 __device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* status, bool report) {
   const long long cap = (long long)g.max_pages * g.page_size;

@@ -368,9 +368,12 @@ paged_append_prompt_kernel(const AppendParams p) {
       int n = 0, first = 0, q0 = 0, nt = 0, pos = 0;
       if (b < g.batch) {
         q0 = p.q_start[b];
-        nt = p.q_start[b + 1] - q0;
+        const int end = p.q_start[b + 1];
+        nt = end - q0;
         pos = p.seq_pos[b];
-        if (nt > 0 && pos >= 0 && q0 >= 0 && q0 + nt <= p.n_tokens) {
+        const bool fits = range_fits(q0, end, p.n_tokens, p.status, blockIdx.x == 0);
+        if (fits && nt > 0 && pos < 0 && blockIdx.x == 0) atomicOr(p.status, B200ATTN_STATUS_BAD_POSITION);
+        if (fits && nt > 0 && pos >= 0) {
           first = pos / g.page_size;
           n = (int)(((long long)pos + nt - 1) / g.page_size) - first + 1;
         }
@@ -384,7 +387,7 @@ paged_append_prompt_kernel(const AppendParams p) {
       const int start = before + inc - n;
       if (n > 0 && chunk >= start && chunk < start + n) { s_at[0] = b; s_at[1] = first + chunk - start; s_at[2] = q0; s_at[3] = nt; s_at[4] = pos; }
       before += __shfl_sync(0xffffffffu, inc, 31);
-      if (before > chunk) break;
+      if (before > chunk && blockIdx.x != 0) break;          // the first block has looked at every sequence
     }
   }
   __syncthreads();

@@ -272,9 +272,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       int n = 0, q0 = 0, nq = 0, raw_len = 0;
       if (b < g.batch) {
         q0 = p.q_start[b];
-        nq = p.q_start[b + 1] - q0;
+        const int end = p.q_start[b + 1];
+        nq = end - q0;
         raw_len = p.seq_len[b];
-        if (nq > 0 && q0 >= 0 && q0 + nq <= p.n_tokens) n = (nq + per_block - 1) / per_block;
+        if (range_fits(q0, end, p.n_tokens, p.status, blockIdx.x == 0) && nq > 0) n = (nq + per_block - 1) / per_block;
       }
       int inc = n;
 #pragma unroll
@@ -285,7 +286,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       const int start = before + inc - n;
       if (n > 0 && number >= start && number < start + n) { s_info[0] = b; s_info[1] = number - start; s_info[5] = q0; s_info[6] = nq; s_info[7] = raw_len; }
       before += __shfl_sync(0xffffffffu, inc, 31);
-      if (before > number) break;
+      if (before > number && blockIdx.x != 0) break;         // the first block has looked at every sequence
     }
   }
   if (tid == 32) {

@@ -1,0 +1,71 @@
+"""Packed calls whose sequences cannot be what q_start or seq_pos say: skipped, reported, and nothing else touched."""
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+# q_start of three sequences and 40 tokens (spread over layers below), and which sequences are skipped
+RANGES = [([0, 10, 5, 40], [1]), ([-1, 10, 30, 40], [0]), ([0, 10, 30, 41], [2]), ([0, 50, 30, 40], [0, 1]), ([50, 10, 30, 40], [0]), ([0, 10, 30, 1 << 30], [2]),
+          ([-(1 << 31), 10, 30, 40], [0])]
+
+
+@pytest.mark.parametrize("starts,skipped", RANGES)
+def test_append_reports_ranges_that_do_not_fit(pkg, cuda_device, starts, skipped):
+    dev, page, d = cuda_device, 16, 128
+    kp = torch.full((1, 12, 1, page, d), 0x11, dtype=torch.uint8, device=dev)
+    vp, ks, vs = kp.clone(), torch.ones(1, 12, 1, device=dev), torch.ones(1, 12, 1, device=dev)
+    table = torch.arange(12, dtype=torch.int32, device=dev).view(3, 4)
+    pos, status = torch.tensor([3, 4, 5], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    x = torch.ones(40, 1, d, dtype=torch.bfloat16, device=dev)
+    pkg.paged_rope_append(None, x, x, None, None, kp, vp, ks, vs, table, pos, q_start=torch.tensor(starts, dtype=torch.int32, device=dev), status=status)
+    assert status.item() == pkg._lib.STATUS_BAD_RANGE
+    for b in range(3):
+        n = 0 if b in skipped else starts[b + 1] - starts[b]
+        assert pos[b].item() == 3 + b + n
+        if n == 0:
+            assert (kp[0, 4 * b:4 * b + 4] == 0x11).all() and (vp[0, 4 * b:4 * b + 4] == 0x11).all()
+
+
+@pytest.mark.parametrize("rope", [False, True])
+def test_append_reports_negative_positions_of_prompts(pkg, cuda_device, rope):
+    dev, page, d = cuda_device, 16, 128
+    kp = torch.full((1, 8, 1, page, d), 0x11, dtype=torch.uint8, device=dev)
+    vp, ks, vs = kp.clone(), torch.ones(1, 8, 1, device=dev), torch.ones(1, 8, 1, device=dev)
+    table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)
+    cos, sin = pkg.rope_tables(64, d, device=dev) if rope else (None, None)
+    x = torch.ones(25, 1, d, dtype=torch.bfloat16, device=dev)
+    for pos, n, want in (([-1, 0], [20, 5], 1), ([0, -7], [20, 5], 1), ([-1, 0], [0, 25], 0)):
+        at, status = torch.tensor(pos, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+        pkg.paged_rope_append(None, x, x, cos, sin, kp, vp, ks, vs, table, at, q_start=torch.tensor([0, n[0], 25], dtype=torch.int32, device=dev), status=status)
+        assert status.item() == want * pkg._lib.STATUS_BAD_POSITION
+        assert at.tolist() == [p if p < 0 else p + m for p, m in zip(pos, n)]
+
+
+@pytest.mark.parametrize("starts,skipped", RANGES)
+@pytest.mark.parametrize("heads", [(1, 1, 128), (8, 1, 128), (7, 1, 256)])
+def test_prefill_reports_ranges_that_do_not_fit(pkg, cuda_device, heads, starts, skipped):
+    """Rows of sequences that are skipped, and of nobody, stay; the others' are right as far as no other sequence claims them."""
+    dev, page, (h_q, h_kv, d) = cuda_device, 16, heads
+    g = torch.Generator().manual_seed(1)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 30, h_kv, page, d)
+    lens = [100, 60, 200]
+    table = ref.random_table(g, lens, page, 14, 30)
+    up = [t.to(dev) for t in (kb, vb, ks, vs, table)]
+    q = torch.randn(1, 40, h_q, d, generator=g).to(torch.bfloat16)
+    ws = pkg.PagedWorkspace(pkg.make_paged_shape(h_q, kb, vb, ks, table), dev, q_tokens=40)
+    out = torch.full_like(q, 7.0).to(dev)
+    pkg.paged_prefill_attention(q.to(dev), torch.tensor(starts, dtype=torch.int32, device=dev), *up, torch.tensor(lens, dtype=torch.int32, device=dev),
+                                workspace=ws, out=out)
+    assert ws.read_status() == pkg._lib.STATUS_BAD_RANGE
+    out, owners = out[0].cpu(), torch.zeros(40, dtype=torch.int32)
+    for b in range(3):
+        if b not in skipped:
+            owners[starts[b]:starts[b + 1]] += 1
+    assert (out[owners == 0] == 7.0).all()
+    for b in range(3):
+        a, z = starts[b], starts[b + 1]
+        if b not in skipped and (owners[a:z] == 1).all():
+            want, big = ref.attention(q[0, a:z], kb[0], vb[0], ks[0], vs[0], table[b], lens[b], causal=True)
+            ref.assert_attention(out[a:z], want, big, (b, starts))
