@@ -232,7 +232,7 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t u
   if (p.q_start) {
     if (token >= ld(p.q_start + p.g.batch) || token < ld(p.q_start)) return;   // a row that belongs to nobody
     b = sequence_of(p.q_start, p.g.batch, token);
-    slot = ld(p.seq_pos + b) + token - ld(p.q_start + b);
+    slot = (int)min((long long)ld(p.seq_pos + b) + token - ld(p.q_start + b), 0x7fffffffLL);
   } else {
     slot = ld(p.seq_pos + b);
   }
@@ -394,6 +394,10 @@ paged_append_prompt_kernel(const AppendParams p) {
   const int b = s_at[0];
   if (b < 0) return;                                     // the grid is an upper bound
   const int page_index = s_at[1], q0 = s_at[2], nt = s_at[3], pos = s_at[4];
+  if (page_index >= g.max_pages) {                       // before anything is computed from it: slots behind the table can pass 31 bits
+    if (tid == 0) atomicOr(p.status, B200ATTN_STATUS_POS_AT_CAPACITY);
+    return;
+  }
   const int slot0 = page_index * g.page_size;
   const int lo = max(pos - slot0, 0);                                                   // rows [lo, hi) are new
   const int hi = (int)min((long long)g.page_size, (long long)pos + nt - slot0);
@@ -417,9 +421,9 @@ paged_append_prompt_kernel(const AppendParams p) {
     src += D;
   };
   load();
-  const int page = page_index < g.max_pages ? page_of(p, b, page_index) : -1;
+  const int page = page_of(p, b, page_index);
   if (page < 0) {
-    if (tid == 0) atomicOr(p.status, page_index < g.max_pages ? B200ATTN_STATUS_BAD_PAGE : B200ATTN_STATUS_POS_AT_CAPACITY);
+    if (tid == 0) atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
     return;
   }
   Rotation rot[NP];                                      // of this thread's rows, for all heads

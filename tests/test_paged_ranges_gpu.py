@@ -69,3 +69,24 @@ def test_prefill_reports_ranges_that_do_not_fit(pkg, cuda_device, heads, starts,
         if b not in skipped and (owners[a:z] == 1).all():
             want, big = ref.attention(q[0, a:z], kb[0], vb[0], ks[0], vs[0], table[b], lens[b], causal=True)
             ref.assert_attention(out[a:z], want, big, (b, starts))
+
+
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("start", [48, 1000, (1 << 31) - 1, (1 << 31) - 8, (1 << 31) - 130])
+def test_append_of_prompts_far_beyond_the_table(pkg, cuda_device, start, page):
+    """Positions behind the last slot, up to the largest number there is: nothing read or stored for them, the neighbour's tokens are."""
+    dev, d, m = cuda_device, 128, 5
+    kp = torch.full((1, 8, 1, page, d), 0x11, dtype=torch.uint8, device=dev)
+    vp, ks, vs = kp.clone(), torch.ones(1, 8, 1, device=dev), torch.ones(1, 8, 1, device=dev)
+    table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)[:, :3 if page == 16 else 1].contiguous()
+    start = max(start, table.shape[1] * page)
+    x = torch.randn(2 * m, 1, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    cos, sin = pkg.rope_tables(64, d, device=dev)
+    at, status = torch.tensor([3, start], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    q = x.expand(2 * m, 3, d).contiguous()
+    pkg.paged_rope_append(q, x, x, cos, sin, kp, vp, ks, vs, table, at, q_start=torch.tensor([0, m, 2 * m], dtype=torch.int32, device=dev), status=status)
+    off_the_tables = pkg._lib.STATUS_BAD_POSITION if start + m > 64 else 0
+    assert status.item() == pkg._lib.STATUS_POS_AT_CAPACITY | off_the_tables and at.tolist() == [3 + m, start]
+    assert (kp[0, 1:] == 0x11).all() and (vp[0, 1:] == 0x11).all()
+    got = ref.values(vp[0, 0, 0, 3:3 + m].cpu()) * vs[0, 0, 0].item()
+    assert ((got - x[:m, 0].cpu().double()).abs() <= x[:m, 0].cpu().double().abs() * 2.0 ** -4 + vs[0, 0, 0].item() * 2.0 ** -10).all()
