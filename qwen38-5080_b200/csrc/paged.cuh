@@ -106,7 +106,7 @@ __device__ __forceinline__ bool range_fits(int q0, int end, int n_tokens, int* s
 }
 
 // Valid length of a sequence: negative lengths count as 0, lengths beyond the table's capacity are clamped to it.
-__device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* status, bool report) {
+__device__ __forceinline__ int paged_len(const PagedGeometry& g, long long raw, int* status, bool report) {
   const long long cap = (long long)g.max_pages * g.page_size;
   if (raw < 0) {
     if (report) atomicOr(status, B200ATTN_STATUS_LEN_NEGATIVE);
@@ -116,7 +116,7 @@ __device__ __forceinline__ int paged_len(const PagedGeometry& g, int raw, int* s
     if (report) atomicOr(status, B200ATTN_STATUS_LEN_OVER_CAP);
     return (int)cap;
   }
-  return raw;
+  return (int)raw;
 }
 
 }  // namespace b200attn

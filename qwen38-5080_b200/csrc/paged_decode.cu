@@ -104,7 +104,7 @@ paged_decode_kernel(const DecodeParams p) {
 
   pdl_wait();
   pdl_launch_dependents();
-  const int len = paged_len(g, p.seq_len[b] + p.seq_len_offset, p.status, tid == 0 && split == 0 && h == 0 && layer == 0);
+  const int len = paged_len(g, (long long)p.seq_len[b] + p.seq_len_offset, p.status, tid == 0 && split == 0 && h == 0 && layer == 0);
   // pieces: as many as the grid has room for, each a whole number of rounds
   const int rounds = (len + kUnit - 1) / kUnit;
   const int per = rounds * kUnit <= kWhole ? rounds : (rounds + p.num_splits - 1) / p.num_splits;
@@ -466,7 +466,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     bool any_empty = false, uniform = true;
     for (int b0 = 0; b0 < g.batch; b0 += 32) {
       const int b = b0 + lane;
-      const int len = b < g.batch ? paged_len(pp.g, p.seq_len[b] + p.seq_len_offset, p.status, blockIdx.x == 0) : 0;
+      const int len = b < g.batch ? paged_len(pp.g, (long long)p.seq_len[b] + p.seq_len_offset, p.status, blockIdx.x == 0) : 0;
       const int n = (len + kTileT - 1) / kTileT;
       if (b0 == 0) first_tiles = __shfl_sync(0xffffffffu, n, 0);
       longest = max(longest, __reduce_max_sync(0xffffffffu, n));

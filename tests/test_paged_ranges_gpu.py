@@ -90,3 +90,21 @@ def test_append_of_prompts_far_beyond_the_table(pkg, cuda_device, start, page):
     assert (kp[0, 1:] == 0x11).all() and (vp[0, 1:] == 0x11).all()
     got = ref.values(vp[0, 0, 0, 3:3 + m].cpu()) * vs[0, 0, 0].item()
     assert ((got - x[:m, 0].cpu().double()).abs() <= x[:m, 0].cpu().double().abs() * 2.0 ** -4 + vs[0, 0, 0].item() * 2.0 ** -10).all()
+
+
+@pytest.mark.parametrize("longest", [1, None])
+def test_decode_lengths_beyond_31_bits(pkg, cuda_device, longest):
+    """A length and an offset whose sum passes 2^31: over the capacity (all of it attended), not negative."""
+    g = torch.Generator().manual_seed(2)
+    kb, vb, ks, vs = ref.random_cache(g, 1, 8, 1, 16, 128)
+    table = torch.randint(0, 8, (2, 9000), generator=g).to(torch.int32)
+    q = torch.randn(1, 2, 5, 128, generator=g).to(torch.bfloat16)
+    table[0], table[1] = table[0, 0], table[1, 0]           # every page the same: 144,000 slots like 16
+    up = [t.to(cuda_device) for t in (kb, vb, ks, vs, table)]
+    ws = pkg.PagedWorkspace(pkg.make_paged_shape(5, kb, vb, ks, table), cuda_device, max_seq_len=longest)
+    n = torch.tensor([(1 << 31) - 3, 30 - (1 << 30)], dtype=torch.int32, device=cuda_device)
+    out = pkg.paged_decode_attention(q.to(cuda_device), *up, n, workspace=ws, seq_len_offset=1 << 30).cpu()
+    assert ws.read_status() == pkg._lib.STATUS_LEN_OVER_CAP
+    for b, length in enumerate([16, 30]):
+        want, big = ref.attention(q[0, b:b + 1], kb[0], vb[0], ks[0], vs[0], table[b], length)
+        ref.assert_attention(out[0, b:b + 1], want, big, b)
