@@ -201,7 +201,7 @@ class PagedFP8Cache:
     def prefill(self, q, k, v, cos, sin, lens, *, out=None, causal: bool = True, **rope) -> torch.Tensor:
         """New tokens of every sequence (lens[b] of them, 0 allowed; packed along the token dimension): rotated, appended and
         attended.  Returns bf16 [n_layers, n_tokens, h_q, head_dim].  `rope`: further arguments of `paged_rope_append`."""
-        if len(lens) != self.slots or sum(lens) != q.shape[-3]:
+        if len(lens) != self.slots or min(lens) < 0 or sum(lens) != q.shape[-3]:
             raise ValueError("lens must give every sequence's share of the tokens")
         if self.prompt_workspace is None or self.prompt_workspace.q_tokens < sum(lens):
             raise ValueError(f"max_prompt_tokens is too small for {sum(lens)} tokens")
@@ -211,14 +211,22 @@ class PagedFP8Cache:
         for a, n in zip(self.host_len, lens):
             if a + n > self.max_pages * self.page_size:
                 raise ValueError(f"capacity {self.max_pages * self.page_size} exceeded: {a} cached + {n}")
+        had = [len(p) for p in self.pages]
         for b, n in enumerate(lens):
             self.reserve(b, n)
         starts = [0]
         for n in lens:
             starts.append(starts[-1] + n)
         q_start = torch.tensor(starts, dtype=torch.int32).to(self.device)
-        qr = paged_rope_append(q, k, v, cos, sin, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
-                               self.seq_pos, q_start=q_start, advance=True, status=self.status, **rope)
+        try:
+            qr = paged_rope_append(q, k, v, cos, sin, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
+                                   self.seq_pos, q_start=q_start, advance=True, status=self.status, **rope)
+        except Exception:
+            for b, n in reversed(list(enumerate(had))):    # the call was refused: a slot that was idle is idle
+                self.free += reversed(self.pages[b][n:])
+                del self.pages[b][n:]
+                self.page_table[b, n:] = -1
+            raise
         self.host_len = [a + n for a, n in zip(self.host_len, lens)]
         return paged_prefill_attention(qr, q_start, self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.page_table,
                                        self.seq_pos, workspace=self.prompt_workspace, causal=causal, out=out)

@@ -125,11 +125,17 @@ def test_pages_reserved_between_replays(pkg, cuda_device):
     _check(c, q, out, want, [(0, 1), (1, 2)])
 
 
-def test_replays_are_counted_against_the_reserved_pages(pkg):
-    c = object.__new__(pkg.PagedFP8Cache)                  # the host side, over CPU tensors
+def _host_side(pkg):
+    """PagedFP8Cache without a device: what it keeps on the host, over CPU tensors."""
+    c = object.__new__(pkg.PagedFP8Cache)
     c.slots, c.n_pages, c.max_pages, c.page_size, c.device = 3, 10, 6, 16, torch.device("cpu")
     c.page_table, c.seq_pos = torch.full((3, 6), -1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
     c.host_len, c.pages, c.free = [0] * 3, [[] for _ in range(3)], list(range(9, -1, -1))
+    return c
+
+
+def test_replays_are_counted_against_the_reserved_pages(pkg):
+    c = _host_side(pkg)
     c.reserve(0, 20)
     c.host_len[0] = 20
     c.reserve(2, 5)
@@ -146,3 +152,19 @@ def test_replays_are_counted_against_the_reserved_pages(pkg):
     c.release(2)
     c.replayed()
     assert c.host_len == [37, 0, 0]
+
+
+def test_a_refused_prompt_changes_nothing(pkg):
+    """Lengths that are negative, and a call that the append refuses (here: the cache is on the CPU): no page stays handed out."""
+    c = _host_side(pkg)
+    c.workspace = c.prompt_workspace = type("Scratch", (), {"q_tokens": 100, "status": torch.zeros(1, dtype=torch.int32)})()
+    c.k_pages = c.v_pages = torch.zeros(1, 10, 1, 16, 128, dtype=torch.uint8)
+    c.k_scale = c.v_scale = torch.ones(1, 10, 1)
+    c.reserve(0, 20)
+    c.host_len[0] = 20
+    before = ([list(p) for p in c.pages], list(c.free), c.page_table.clone(), list(c.host_len))
+    q, k = torch.zeros(1, 30, 5, 128, dtype=torch.bfloat16), torch.zeros(1, 30, 1, 128, dtype=torch.bfloat16)
+    for lens, what in (([40, -10, 0], "share"), ([20, 10, 0], "CUDA"), ([0, 0, 30], "CUDA")):
+        with pytest.raises(ValueError, match=what):
+            c.prefill(q, k, k, None, None, lens)
+        assert (c.pages, c.free, c.host_len) == (before[0], before[1], before[3]) and torch.equal(c.page_table, before[2])
