@@ -98,6 +98,11 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
 template <class T>
 __device__ __forceinline__ T ld(const T* p) { return *p; }
 
+// For the index checks: whether token rows [row, row + n) of a layer's pool exist.
+__device__ __forceinline__ bool rows_exist(const PagedGeometry& g, long long row, int n, int layer) {
+  return row >= 0 && row + n <= (long long)g.n_pages * g.h_kv * g.page_size && layer >= 0 && layer < g.n_layers;
+}
+
 // Whether sequence b of a packed call may own tokens [q0, end).
 __device__ __forceinline__ bool range_fits(int q0, int end, int n_tokens, int* status, bool report) {
   const bool fits = q0 >= 0 && end >= q0 && end <= n_tokens;

@@ -132,6 +132,7 @@ struct Rotation {
     const int half = p.rot >> 1, j0 = sh.on ? sh.a : 0;
     if (p.pair_axis == nullptr) {
       const int pos = clamped(p, p.positions ? ld(p.positions + token) : slot, false, sh.on);
+      B200ATTN_CHECK(p.status, pos >= 0 && pos < p.n_positions && j0 + 4 <= half);
       c = ld(reinterpret_cast<const float4*>(p.cos + (long long)pos * half + j0));
       s = ld(reinterpret_cast<const float4*>(p.sin + (long long)pos * half + j0));
     } else {
@@ -141,6 +142,7 @@ struct Rotation {
       for (int a = 0; a < 4; ++a) at[a] = !p.positions ? slot : a < p.n_axes ? ld(p.positions + (long long)a * p.n_tokens + token) : 0;
       auto pick = [&](int a) { return (long long)clamped(p, a == 1 ? at[1] : a == 2 ? at[2] : a == 3 ? at[3] : at[0], a < 0 || a >= p.n_axes, sh.on) * half + j0; };
       const long long i0 = pick(ax.x), i1 = pick(ax.y) + 1, i2 = pick(ax.z) + 2, i3 = pick(ax.w) + 3;
+      B200ATTN_CHECK(p.status, i0 >= 0 && i1 >= 0 && i2 >= 0 && i3 >= 0 && max(max(i0, i1), max(i2, i3)) < (long long)p.n_positions * half);
       c = make_float4(ld(p.cos + i0), ld(p.cos + i1), ld(p.cos + i2), ld(p.cos + i3));
       s = make_float4(ld(p.sin + i0), ld(p.sin + i1), ld(p.sin + i2), ld(p.sin + i3));
     }
@@ -217,7 +219,9 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t u
   const uint32_t r = unit / chunks;            // (layer, token)
   const int g_first = (int)(unit - r * chunks) * run, g_end = min(groups, g_first + run);
   const int layer = (int)(r / (uint32_t)p.n_tokens), token = (int)(r - (uint32_t)layer * p.n_tokens);
+  B200ATTN_CHECK(p.status, layer < p.g.n_layers && token < p.n_tokens && g_first < groups);
   const Share<D> sh(lane, p.rot);
+  B200ATTN_CHECK(p.status, sh.a >= 0 && sh.b + 4 <= D && (!sh.on || sh.b + 4 <= p.rot));
   const long long row0 = (long long)r * p.g.h_q + lane / TPR;
   Raw raw[kQLoads];
   auto load = [&](int group) {
@@ -333,6 +337,7 @@ paged_append_token_kernel(const AppendParams p) {
   }
   if (lr == 0) *sp = s;
   const float inv = __fdiv_rn(1.f, s);
+  B200ATTN_CHECK(p.status, r2 < rows && rows_exist(g, ((long long)page * g.h_kv + h) * g.page_size + fill, 1, layer) && fill < g.page_size);
   uint8_t* dst = base + (long long)fill * D;
   *reinterpret_cast<uint32_t*>(dst + sh.a) = quant4(x, inv);
   *reinterpret_cast<uint32_t*>(dst + sh.b) = quant4(x + 4, inv);
@@ -413,6 +418,7 @@ paged_append_prompt_kernel(const AppendParams p) {
     const int row = i * RPP + tid / TPR;
     is_new[i] = row >= lo && row < hi;
     raw[i] = Raw{make_uint2(0, 0), make_uint2(0, 0)};     // rows that are not new stay zero
+    B200ATTN_CHECK(p.status, !is_new[i] || (slot0 + row >= pos && slot0 + row < pos + nt && q0 + slot0 + row - pos < p.n_tokens));
   }
   auto load = [&]() {
 #pragma unroll
@@ -436,6 +442,8 @@ paged_append_prompt_kernel(const AppendParams p) {
   float* scales = (which ? p.v_scale : p.k_scale) + ((long long)layer * g.n_pages + page) * g.h_kv;
   uint8_t* base = (which ? p.v_pages : p.k_pages) + (long long)layer * (which ? g.v_layer_stride : g.k_layer_stride) +
                    ((long long)page * g.h_kv + h_first) * g.page_size * D;   // the page of the head
+  B200ATTN_CHECK(p.status, lo >= 0 && lo < hi && hi <= g.page_size && RPP * NP >= g.page_size &&
+                               rows_exist(g, ((long long)page * g.h_kv + h_first) * g.page_size, (h_end - h_first) * g.page_size, layer));
 #pragma unroll 1
   for (int h = h_first; h < h_end; ++h, base += g.page_size * D) {
     float x[NP][8];

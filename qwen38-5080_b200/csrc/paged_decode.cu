@@ -116,6 +116,7 @@ paged_decode_kernel(const DecodeParams p) {
     return;
   }
   const int t_begin = split * per * kUnit, t_end = min(len, t_begin + per * kUnit);
+  B200ATTN_CHECK(p.status, t_begin < t_end && layer < g.n_layers && pieces <= p.num_splits && pieces <= kMostPieces);
 
   // ---- query fragments: lane holds head gq, dims 16 * (4 ch + tq) + 4 w + {0, 1 | 2, 3} ----
   uint32_t qf[KS][2];
@@ -190,7 +191,9 @@ paged_decode_kernel(const DecodeParams p) {
     // offset of a 16-token step's rows, or -1: no tokens there, or a page that does not exist
     auto rows_of = [&](int t) -> long long {
       if (t >= stage_end) return -1;
+      B200ATTN_CHECK(p.status, t >= t_begin / g.page_size * g.page_size && t / g.page_size - first >= 0 && t / g.page_size - first < kStage);
       const int id = s_page[t / g.page_size - first];
+      B200ATTN_CHECK(p.status, id < 0 || rows_exist(g, ((long long)id * g.h_kv + h) * g.page_size + t % g.page_size, 16, layer));
       return id < 0 ? -1 : (((long long)id * g.h_kv + h) * g.page_size + t % g.page_size) * D;
     };
     auto load_k = [&](long long off) {
@@ -520,6 +523,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         pair_ = (c.layer * g.batch + c.b) * g.h_kv + c.h;
         const int tok = c.tile * kTileT + (lane & 3) * 16;
         if (tok >= c.len_b) return;
+        B200ATTN_CHECK(p.status, c.b >= 0 && c.b < g.batch && tok >= 0 && (tok >> pp.page_shift) < pp.g.max_pages);
         const int page = ld(pp.page_table + (long long)c.b * pp.g.max_pages + (tok >> pp.page_shift));
         if (page < 0 || page >= pp.g.n_pages) {
           atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE);
@@ -566,6 +570,7 @@ paged_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           if (lane == 0) mbar_arrive_expect_tx(fb, 2u * boxes * box_rows * D);
           __syncwarp();
           if (box) {
+            B200ATTN_CHECK(p.status, rows_exist(pp.g, row, box_rows, layer) && s >= 0 && s < stages && (lane & 3) * 16 + box_rows <= kTileT);
 #pragma unroll
             for (int hf = 0; hf < DH; ++hf) {
               const uint32_t off = (uint32_t)s * TILE_BYTES + hf * kTileT * 128 + (lane & 3) * 16 * 128;

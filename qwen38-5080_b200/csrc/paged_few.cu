@@ -128,6 +128,8 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       }
     return;
   }
+  B200ATTN_CHECK(p.status, first_tok >= 0 && ntok > 0 && ntok * G <= COLS && layer < g.n_layers && s_info[2] + first_tok + ntok <= p.n_tokens &&
+                               pieces <= p.splits && pieces <= kMostPieces && visible <= g.max_pages * g.page_size);
   const int u0 = piece * per + warp, u1 = min(units, piece * per + per);
   const int n = u1 > u0 ? (u1 - u0 + kWarps - 1) / kWarps : 0;            // units of this warp: u0, u0 + kWarps, ..
 
@@ -138,6 +140,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     sc = make_float2(-1.f, 0.f);
     if (i0 + lane >= n) return;
     const int tok = (u0 + (i0 + lane) * kWarps) * kRowsU;
+    B200ATTN_CHECK(p.status, tok < visible && (tok >> p.page_shift) < g.max_pages);
     const int page = ld(p.page_table + (long long)b * g.max_pages + (tok >> p.page_shift));
     if (page < 0 || page >= g.n_pages) { atomicOr(p.status, B200ATTN_STATUS_BAD_PAGE); return; }
     row = ((page * g.h_kv + h) << p.page_shift) + (tok & (g.page_size - 1));
@@ -158,6 +161,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       s_sc[warp][s] = sc;
       const uint32_t bar = my_bar + 8 * s, dst = my_ring + s * P::SLOT;
       if (row >= 0) {
+        B200ATTN_CHECK(p.status, rows_exist(g, row, kRowsU, layer));
         mbar_arrive_expect_tx(bar, P::SLOT);
 #pragma unroll
         for (int hf = 0; hf < DH; ++hf) {

@@ -330,6 +330,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int j0 = piece * per_piece, nt = min(per_piece, all_tiles - j0);
   const int key_end = min(len, (j0 + nt) * kKeys);
 
+  B200ATTN_CHECK(p.status, first_tok >= 0 && ntok > 0 && layer < g.n_layers && q0 + first_tok + ntok <= p.n_tokens && nt > 0 && pieces <= p.splits &&
+                               key_end <= g.max_pages * g.page_size && number >= 0);
   constexpr uint32_t tmem = 0;                              // all 512 columns are this block's: they begin at 0
 
   float r_v = 0.f;                                          // largest V scale of the block's keys (V and softmax warps)
@@ -407,6 +409,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     auto page_at = [&](int j) -> int {
       const int key = (j0 + j) * kKeys + lane * 16;
       if (lane >= 8 || j >= nt || key >= key_end) return -2;   // no key
+      B200ATTN_CHECK(p.status, key >= 0 && (key >> p.page_shift) < g.max_pages);
       return max(-1, ld(p.page_table + (long long)b * g.max_pages + (key >> p.page_shift)));
     };
     auto scales_at = [&](int id) -> float2 {
@@ -445,6 +448,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         if (lane == 0) mbar_arrive_expect_tx(kfull + 8 * st, boxes * g.page_size * D);
         __syncwarp();
         if (box) {
+          B200ATTN_CHECK(p.status, rows_exist(g, (long long)(id0 * g.h_kv + h) << p.page_shift, g.page_size, layer) && lane * 16 + g.page_size <= kKeys);
 #pragma unroll
           for (int hf = 0; hf < DH; ++hf)
             tma_load_3d(sK + st * P::KTILE + hf * kKeys * 128 + lane * 16 * 128, &kmap, hf * 128, (id0 * g.h_kv + h) << p.page_shift, layer, kfull + 8 * st);
@@ -470,6 +474,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           __syncwarp();
           if (vbox) {
             const int row = ((idp * g.h_kv + h) << p.page_shift) + ((lane * 16) & (g.page_size - 1));
+            B200ATTN_CHECK(p.status, rows_exist(g, row, vrows, layer) && (lane % UL) * 16 + vrows <= P::UNIT_KEYS);
 #pragma unroll
             for (int hf = 0; hf < DH; ++hf)
               tma_load_3d(sRaw + vs * P::RAW_BYTES + hf * P::UNIT_KEYS * 128 + (lane % UL) * 16 * 128, &vmap, hf * 128, row, layer, rfull + 8 * vs);
@@ -855,6 +860,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] += f1 == 0.f ? 0.f : __uint_as_float(x[i]) * f1;
         }
+        B200ATTN_CHECK(p.status, !real || (tok >= 0 && tok < ntok && head < G && row < kRows && (pieces == 1 || ((long long)(blockIdx.x / p.splits) * p.splits + piece < (long long)gridDim.x))));
         if (real && pieces == 1) {
           uint16_t* dst = p.out + (out_row0 + (long long)tok * g.h_q + head) * D + 32 * c;
 #pragma unroll
@@ -896,6 +902,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PrefillP
   pdl_wait();
   const int tile = (int)(blockIdx.x / (kRows / kJoinRows)), first = (int)(blockIdx.x % (kRows / kJoinRows)) * kJoinRows;
   const PrefillTile t = p.done[tile];
+  B200ATTN_CHECK(p.status, t.rows <= kRows && t.pieces <= p.splits &&
+                               (t.rows == 0 || t.row0 + (long long)((t.rows - 1) / p.g.group) * p.g.h_q + p.g.group <= (long long)p.g.n_layers * p.n_tokens * p.g.h_q));
   if (t.pieces < 2 || first >= t.rows) return;
   constexpr long long stride = kRows * (D + 2);
   const float* all = p.part + (long long)tile * p.splits * stride;
