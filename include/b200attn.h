@@ -425,8 +425,10 @@ int b200attn_calibrate_scales(const B200AttnShape* shape, int n_tokens,
  *     k_scale / v_scale : f32 [n_layers][n_pages][h_kv]       one scale per (layer, page, kv head)
  *     page_table        : i32 [batch][max_pages]              page of tokens [i * page_size, (i+1) * page_size) of a sequence
  *
- * A value is float(byte) * scale.  The attention calls take any scale that is not negative and not NaN; the append makes powers
- * of two (below).
+ * A value is float(byte) * scale.  The attention calls take any scale that is not negative and finite; the append makes powers of
+ * two (below).  They hold a value times its weight relative to the largest V scale r of the keys of one (layer, sequence, kv head) that
+ * they work on together (those that a row does not see may be among them): to 2^-31 r, so that pages whose V scale is more than
+ * 2^20 below r begin to lose bits of their values; beyond 2^40 they count as zeros.
  * Table entries at or beyond a sequence's last token are never read.  A page that the append writes must
  * belong to one sequence only; pages that are only read may be shared.  Queries and new keys / values of ragged
  * batches are packed: sequence b owns rows [q_start[b], q_start[b + 1]) of the token dimension; rows from
@@ -434,7 +436,7 @@ int b200attn_calibrate_scales(const B200AttnShape* shape, int n_tokens,
  */
 typedef struct B200AttnPagedShape {
   int n_layers;
-  int batch;         /* sequences (rows of page_table), >= 1 */
+  int batch;         /* sequences (rows of page_table), >= 1; n_layers * batch <= 65535 */
   int h_q;           /* query heads; a multiple of h_kv, group size <= 8 */
   int h_kv;
   int head_dim;      /* 128 or 256 */
@@ -518,8 +520,11 @@ int b200attn_paged_decode(const B200AttnPagedShape* shape, const void* q_bf16,
  * The queries of sequence b are its last tokens: with causal = 1, query i of n attends slots t <= seq_len[b] - n + i (none:
  * its row is zero); with causal = 0 all seq_len[b] slots (cross attention to states of another length).
  *   q, out  : bf16 [n_layers][n_tokens][h_q][head_dim], q_start i32 [batch + 1]
- * Keys that a row does not see have no influence on it, NaN keys included; a NaN among the values of one of a sequence's last
- * n tokens can reach the rows before it as well (0 * NaN).
+ * A row that sees a NaN key, or whose query holds a NaN, is NaN.  Keys that a row does not see have no influence on it, NaN keys
+ * included; but a NaN among the values of one of a sequence's last n tokens can reach the rows before it as well (0 * NaN), and their
+ * V scales take part in r above.
+ * One kernel runs per call, by its average tokens per sequence.  A call that mixes single tokens with a long chunk is right but
+ * takes longer than one call for each kind.
  */
 int b200attn_paged_prefill(const B200AttnPagedShape* shape, int n_tokens, const void* q_bf16, const int* q_start,
                            const void* k_pages_u8, const void* v_pages_u8, const float* k_scale, const float* v_scale,

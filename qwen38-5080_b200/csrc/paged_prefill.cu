@@ -5,7 +5,8 @@
 // A thread block owns one tile of 128 query rows of one (layer, sequence, kv head): 128 / G tokens times the G query
 // heads that share the kv head, so that a key serves all of them; it walks the visible keys 128 at a time.
 //   * K stays in 8 bits: the tile's bytes go from TMA to the tensor core.  A query row is normalised by a power of two and
-//     written once as two e4m3 rows, leading part + remainder (a bf16 value has 8 significant bits, e4m3 holds 4): two
+//     written once as two e4m3 rows, leading part + remainder (a bf16 value has 8 significant bits, e4m3 holds 4; exact for
+//     elements within 2^9 of the row's largest, smaller ones are off by at most 2^-16 of it): two
 //     kind::f8f6f4 products cost what one 16-bit product would, and no key is converted.
 //   * V's bytes come by TMA too; four warps widen them to f16, shared memory to shared memory (exact; times the page's scale relative to
 //     the largest scale of the block's keys), because P needs more than 8 bits: P is f16 in tensor memory, in the columns
@@ -82,7 +83,7 @@ struct PrefillPlan {
   static constexpr int WARPS = 4 * NS + 8;                 // softmax, V, and a group of TMA, MMA and two idle warps
   static constexpr int THREADS = WARPS * 32;
   static constexpr int SMEM = 1024 + NS * QTILE + KST * KTILE + kVRing * kUnitBytes + RAW * RAW_BYTES;
-  // Registers per thread after the roles part: softmax keeps a row's 128 scores.  The shares add up to what the block
+  // Registers per thread after the roles part: softmax keeps 64 scores of a row and their P.  The shares add up to what the block
   // is launched with (512 x 128; 384 x 168): 256 x 184 + 256 x 72; 128 x 232 + 256 x 136.
   static constexpr int REGS_SOFTMAX = D == 128 ? 184 : 232;
   static constexpr int REGS_OTHER = D == 128 ? 72 : 136;

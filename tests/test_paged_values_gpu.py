@@ -217,3 +217,22 @@ def test_quiet_keys(pkg, cuda_device, form, exponent):
     cache[2].fill_(2.0 ** exponent)
     q = _queries(g, form, lens)
     _compare(form, cache, lens, q, _attend(pkg, cuda_device, form, cache, lens, q))
+
+
+@pytest.mark.parametrize("below", [10, 20, 30, 45])
+@pytest.mark.parametrize("form", FORMS)
+def test_quiet_values_beside_loud_ones(pkg, cuda_device, form, below):
+    """All the weight lies on a key whose page's V scale is 2^-below of the others': it is held to 2^-31 of the largest scale."""
+    g = torch.Generator().manual_seed(11)
+    lens = [300, 290]
+    cache = _cache(g, form, lens)
+    cache[3].fill_(1.0)
+    for b in range(2):
+        _far_key(cache, b, 100 + b, 150.0, FORMS[form][0][2])
+        cache[3][0, cache[4][b, 100 // PAGE]] = 2.0 ** -below
+    q = (1 + 0.1 * _queries(g, form, lens).float()).to(torch.bfloat16)
+    for b, (rows, n) in enumerate(zip(_attend(pkg, cuda_device, form, cache, lens, q), lens)):
+        want, _ = _want(form, cache, b, n, q)
+        off = (rows.double() - want).abs()
+        # bf16: half a step 2^-9 of the value; p of the one key that counts in f16: 2^-12 of it
+        assert (off <= want.abs() * (2.0 ** -9 + 2.0 ** -11) + 2.0 ** -30).all(), (b, float(off.max()))
