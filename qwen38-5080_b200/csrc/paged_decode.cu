@@ -6,7 +6,8 @@
 //
 // Two kernels (use_streamk says which, with the figures): one that starts and ends quickly for short caches and few of them,
 // described here, and one that streams at the copy rate for everything else, described at its place.  One layer of one user on 512
-// tokens takes 8 us; 64 layers of one on 8192 tokens 166 us, 6.5 TB/s; 8 users on 65536 tokens with heads of 256 168 us, 6.1 TB/s.
+// tokens takes 8 us; 64 layers of one on 8192 tokens 171 to 188 us issued from the host, by GPU and how warm it is (5.7 to 6.3 TB/s; 166 in a
+// graph), 8 users on 65536 tokens with heads of 256 172 to 189 us (5.5 to 6.0 TB/s; 168 in a graph).
 //
 // A thread block of four warps takes a piece of one (layer, sequence, kv head) pair; a warp takes 16 tokens at a time,
 // straight from global memory into registers in the layout that the tensor core wants, so there is nothing to fill, no

@@ -441,8 +441,9 @@ int few_blocks(const PagedGeometry& g) { return g.head_dim == 128 ? FewPlan<128,
 
 }  // namespace
 
-// The host knows the tokens and sequences of a call, not how they are spread; a sequence with more rows than a tile takes several,
-// each of which reads the keys again.
+// The host knows the tokens and sequences of a call, not how they are spread.  A sequence with more rows than a tile takes several,
+// each of which reads the keys again; single tokens beside enough others for the larger tiles take 128 rows each.  (Caches of 8192 tokens,
+// 40 / 8 heads of 128: 255 single tokens and one chunk of 500 in one call 1184 us, in two calls 723 + 146.)
 bool few_rows(const PagedGeometry& g, int n_tokens) {
   return ((long long)n_tokens + g.batch - 1) / g.batch * g.group <= kFewRows && (long long)g.n_pages * g.h_kv * g.page_size <= 0x7fffffffLL;
 }

@@ -25,7 +25,7 @@
 //
 // Bound: the tensor cores (4 D flops per row, key and head), and as much the exponentials, one per row and key:
 // 16 a cycle per SM make 1024 cycles a tile, the products of a 128-wide head 1048; a tile takes 1,800 to 2,100 (heads of 256: 3,400
-// for 2,096), a block's start 7,000 (15,000) and its end 4,000.  An 8192-token prompt, 40 / 8 heads of 128: 690 us, 1.0 PFLOP/s.
+// for 2,096), a block's start 7,000 (15,000) and its end 4,000.  An 8192-token prompt, 40 / 8 heads of 128: 705 to 730 us by GPU, 0.94 to 0.97 PFLOP/s.
 //
 // Few rows on a long cache: the keys are cut into pieces over several thread blocks, which leave (m, l, O) in the
 // workspace, and a second kernel joins them in order.  Nobody waits for another thread block; waits inside one are bounded.
