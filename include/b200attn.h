@@ -482,7 +482,8 @@ typedef struct B200AttnRope {
  * but for values that become subnormal).  Infinities saturate, NaN becomes the NaN byte.  A scale is never below 2^-126.
  * Tokens beyond a sequence's capacity are skipped (B200ATTN_STATUS_POS_AT_CAPACITY).
  * Without q_start, a sequence at position 0 whose first table entry is -1 is idle: its token is dropped, it does not advance and
- * nothing is reported.  (Its length stays 0, so that the attention gives zeros.)
+ * nothing is reported.  (Its length stays 0, so that the attention gives zeros.  Its query is rotated like any other: a row of
+ * `positions` for it has to be within the tables.)
  */
 int b200attn_paged_rope_append(const B200AttnPagedShape* shape, const B200AttnRope* rope, int n_tokens, const int* q_start,
                                const void* q_bf16, const void* k_bf16, const void* v_bf16,
