@@ -88,6 +88,9 @@ struct Cache {
   }
 };
 
+// Whether a tensor that names its layers has them first: [n_tokens, n_layers, ..] has as many elements.
+bool layers_first(Tensor t, int64_t n_layers) { return !t || n_layers == 1 || t->dim() < 4 || t->size(0) == n_layers; }
+
 bool args_ok(Py_ssize_t n, Py_ssize_t want) { return n == want || refuse("wrong number of arguments"); }
 
 // q's heads: its last dimension but one; without q the kv heads.
@@ -123,9 +126,9 @@ bool append(PyObject* const* a, int& rc) {
   const B200AttnPagedShape& s = c.shape;
   const int64_t n = s.n_layers, d = s.head_dim, row = n * s.h_kv * d;
   const int64_t n_tokens = row ? k->numel() / row : 0;
-  if (n_tokens > 0x7fffffff || k->numel() != row * n_tokens || v->sizes() != k->sizes() || k->dim() < 2 || k->size(-2) != s.h_kv || k->size(-1) != d)
+  if (n_tokens > 0x7fffffff || k->numel() != row * n_tokens || v->sizes() != k->sizes() || k->dim() < 2 || k->size(-2) != s.h_kv || k->size(-1) != d || !layers_first(k, n))
     return refuse("k and v must be [n_layers, n_tokens, h_kv, head_dim]");
-  if (q && (q->numel() != n * n_tokens * h_q * d || q->size(-1) != d)) return refuse("q must be [n_layers, n_tokens, h_q, head_dim]");
+  if (q && (q->numel() != n * n_tokens * h_q * d || q->size(-1) != d || !layers_first(q, n))) return refuse("q must be [n_layers, n_tokens, h_q, head_dim]");
   if (pos->numel() != s.batch) return refuse("seq_pos must be int32 [batch]");
   if (!start && n_tokens != s.batch) return refuse("without q_start there is one token per sequence");
   if (start && start->numel() != (int64_t)s.batch + 1) return refuse("q_start must be int32 [batch + 1]");
@@ -142,7 +145,7 @@ bool append(PyObject* const* a, int& rc) {
     rope = B200AttnRope{(const float*)address(cos), (const float*)address(sin), (const int*)address(positions), (const int*)address(axis),
                         (int)cos->size(0), (int)axes, (int)(2 * cos->size(1)), 0};
   }
-  if (q && (!q_out || q_out->numel() != q->numel())) return refuse("q_out must have q's shape");
+  if (q && (!q_out || q_out->numel() != q->numel() || !layers_first(q_out, n))) return refuse("q_out must have q's shape");
   if (n_tokens == 0) return true;
   rc = call_append(&s, turns ? &rope : nullptr, (int)n_tokens, (const int*)address(start), address(q), address(k), address(v), address(wq), address(wk),
                    (float)eps, q ? address(q_out) : nullptr, address(c.k), address(c.v), (float*)address(c.ks), (float*)address(c.vs),
@@ -166,7 +169,7 @@ struct Scratch {   // buffer, bytes, status, longest sequence, softmax scale (No
     stream = PyLong_AsVoidPtr(a[6]);
     if (PyErr_Occurred()) return false;
     if (longest < 0 || longest > 0x7fffffff || bytes > (size_t)buf->numel()) return refuse("the workspace does not fit");
-    if (out->numel() != q->numel()) return refuse("out must have q's shape");
+    if (out->numel() != q->numel() || !layers_first(out, c.shape.n_layers)) return refuse("out must have q's shape");
     return true;
   }
 };
@@ -179,7 +182,8 @@ bool decode(PyObject* const* a, int& rc) {
   Scratch w;
   if (!heads_of(a[0], a[1], h_q) || !c.read(a + 1, h_q) || !need(a[0], "q", c.dev, kBf16, q) || !need(a[6], "seq_len", c.dev, kI32, len)) return false;
   const B200AttnPagedShape& s = c.shape;
-  if (q->size(-1) != s.head_dim || q->numel() != (int64_t)s.n_layers * s.batch * h_q * s.head_dim) return refuse("q must be [n_layers, batch, h_q, head_dim]");
+  if (q->size(-1) != s.head_dim || q->numel() != (int64_t)s.n_layers * s.batch * h_q * s.head_dim || !layers_first(q, s.n_layers))
+    return refuse("q must be [n_layers, batch, h_q, head_dim]");
   if (len->numel() != s.batch) return refuse("seq_len must be int32 [batch]");
   const long offset = PyLong_AsLong(a[7]);
   if (PyErr_Occurred()) return false;
@@ -201,7 +205,8 @@ bool prefill(PyObject* const* a, int& rc) {
     return false;
   const B200AttnPagedShape& s = c.shape;
   const int64_t row = (int64_t)s.n_layers * h_q * s.head_dim, n_tokens = row ? q->numel() / row : 0;
-  if (n_tokens > 0x7fffffff || q->size(-1) != s.head_dim || q->numel() != row * n_tokens) return refuse("q must be [n_layers, n_tokens, h_q, head_dim]");
+  if (n_tokens > 0x7fffffff || q->size(-1) != s.head_dim || q->numel() != row * n_tokens || !layers_first(q, s.n_layers))
+    return refuse("q must be [n_layers, n_tokens, h_q, head_dim]");
   if (len->numel() != s.batch || start->numel() != (int64_t)s.batch + 1) return refuse("seq_len must be int32 [batch], q_start int32 [batch + 1]");
   const long most = PyLong_AsLong(a[8]);
   const int causal = PyObject_IsTrue(a[9]);

@@ -108,3 +108,31 @@ def test_decode_lengths_beyond_31_bits(pkg, cuda_device, longest):
     for b, length in enumerate([16, 30]):
         want, big = ref.attention(q[0, b:b + 1], kb[0], vb[0], ks[0], vs[0], table[b], length)
         ref.assert_attention(out[0, b:b + 1], want, big, b)
+
+
+def test_calls_refuse_tensors_whose_layers_are_not_first(pkg, cuda_device):
+    """[n_tokens, n_layers, ..] has the right number of elements, and its rows would be read as other tokens' and layers'."""
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device=cuda_device)  # noqa: E731
+    layers, n, h_q, h_kv, d = 3, 2, 5, 1, 128
+    cache = (z(layers, 4, h_kv, 16, d, t=torch.uint8), z(layers, 4, h_kv, 16, d, t=torch.uint8), z(layers, 4, h_kv, t=torch.float32),
+             z(layers, 4, h_kv, t=torch.float32), torch.arange(4, dtype=torch.int32, device=cuda_device).view(n, 2))
+    pos, status, starts = z(n, t=torch.int32), z(1, t=torch.int32), torch.arange(n + 1, dtype=torch.int32, device=cuda_device)
+    shape = pkg.make_paged_shape(h_q, *cache[:3], cache[4])
+    wd, wp = pkg.PagedWorkspace(shape, cuda_device), pkg.PagedWorkspace(shape, cuda_device, q_tokens=n)
+    good, bad = (layers, n), (n, layers)
+
+    def append(q=good, k=good, v=good, out=good):
+        pkg.paged_rope_append(z(*q, h_q, d), z(*k, h_kv, d), z(*v, h_kv, d), None, None, *cache, pos, advance=False, status=status, q_out=z(*out, h_q, d))
+
+    def decode(q=good, out=good):
+        pkg.paged_decode_attention(z(*q, h_q, d), *cache, pos, workspace=wd, out=z(*out, h_q, d))
+
+    def prefill(q=good, out=good):
+        pkg.paged_prefill_attention(z(*q, h_q, d), starts, *cache, pos, workspace=wp, out=z(*out, h_q, d))
+    for call, names in ((append, ("q", "k", "v", "out")), (decode, ("q", "out")), (prefill, ("q", "out"))):
+        call()
+        for name in names:
+            with pytest.raises(ValueError):
+                call(**{name: bad})
+    torch.cuda.synchronize()
+    assert status.item() == 0 and wd.read_status() == 0 and wp.read_status() == 0
